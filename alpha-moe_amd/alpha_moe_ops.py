@@ -53,6 +53,31 @@ def _fused_experts_fake(hidden_states, topk_ids, w, w_scale, w2, w2_scale, topk_
     return None
 
 
+@torch.library.register_fake("alpha_moe::rms_norm_quant_fp8")
+def _rms_norm_quant_fp8_fake(x, weight, eps, residual, keep_norm, group_size):
+    return (*_per_token_group_quant_fp8_fake(x, group_size),
+            torch.empty_like(x) if residual is not None else x.new_empty((0,)),
+            torch.empty_like(x) if keep_norm else x.new_empty((0,)))
+
+
+@torch.library.register_fake("alpha_moe::swiglu_quant_fp8")
+def _swiglu_quant_fp8_fake(gate_up, group_size):
+    M, I = gate_up.shape[0], gate_up.shape[1] // 2
+    return (gate_up.new_empty((M, I), dtype=torch.float8_e4m3fn),
+            gate_up.new_empty((M, I // group_size), dtype=torch.float32))
+
+
+@torch.library.register_fake("alpha_moe::block_scaled_mm")
+def _block_scaled_mm_fake(x, x_scale, w, w_scale):
+    return x.new_empty((x.shape[0], w.shape[0]), dtype=torch.bfloat16)
+
+
+@torch.library.register_fake("alpha_moe::route_topk")
+def _route_topk_fake(logits, bias, top_k, sigmoid, num_groups, top_groups, renormalize, shared_experts, shared_weight):
+    shape = (logits.shape[0], top_k + shared_experts)
+    return logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int32)
+
+
 def fused_moe_w8a8_up_down(
     x: torch.Tensor,
     x_scale: torch.Tensor,

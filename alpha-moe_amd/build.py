@@ -26,8 +26,8 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 # packed-fp32 VALU forms are switched off for every kernel in this library
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Wno-unused-command-line-argument"]
-# Per-source extras.  The group kernel scales every matrix-instruction result into vector-register accumulators, so
-# the results must land in vector registers, not in accumulation registers that only a copy can read.
+# Per-source extras.  The group kernel and the dense product scale every matrix-instruction result into vector-register accumulators,
+# so the results must land in vector registers, not in accumulation registers that only a copy can read.
 HIP_SOURCES = {
     "moe_api.hip": [],
     "moe_direct.hip": [],
@@ -36,6 +36,9 @@ HIP_SOURCES = {
     "moe_group.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "moe_reduce.hip": [],
     "moe_prep.hip": [],
+    "moe_norm.hip": [],
+    "moe_route.hip": [],
+    "moe_mm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

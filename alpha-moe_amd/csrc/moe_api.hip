@@ -374,6 +374,7 @@ extern "C" const char *alpha_moe_status_string(int status)
     case ALPHA_MOE_ERR_SCRATCH_LIMIT:
         return "the call needs more scratch memory than the library's built-in buffer holds "
                "(alpha_moe_fused_moe_w8a8_up_down_static): use the entry point that takes a workspace";
+    case ALPHA_MOE_ERR_ALIGNMENT: return "a matrix does not start at a multiple of 16 bytes";
     default: return "unknown status";
     }
 }

@@ -412,6 +412,135 @@ void fused_experts(at::Tensor &hidden, const at::Tensor &topk_ids, const at::Ten
     TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_layer_call failed: ", alpha_moe_status_string(rc));
 }
 
+// ---- the operators around the layer call ---------------------------------------------------------------------
+int is_f32_or_bf16(const at::Tensor &t, const char *name)
+{
+    TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat, name, " must be bfloat16 or float32");
+    return t.scalar_type() == at::kFloat;
+}
+
+// (q, scale, residual, norm): y = rms_norm(x + residual) * weight quantised as above; the sum and y in x's type, each empty
+// if it is not asked for.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+rms_norm_quant_fp8(const at::Tensor &x, const at::Tensor &weight, double eps, const c10::optional<at::Tensor> &residual,
+                   bool keep_norm, int64_t group_size)
+{
+    TORCH_CHECK(x.is_cuda(), "x must be a GPU tensor");
+    TORCH_CHECK(group_size == 128, "group_size must be 128");
+    const at::Device dev = x.device();
+    const int x_is_f32 = is_f32_or_bf16(x, "x"), weight_is_f32 = is_f32_or_bf16(weight, "weight");
+    check_tensor(x, "x", x.scalar_type(), dev);
+    TORCH_CHECK(x.dim() == 2 && x.size(1) > 0 && x.size(1) % 128 == 0 && x.size(1) <= 65536,
+                "x must be [M, K] with K % 128 == 0 and K <= 65536");
+    const int64_t M = x.size(0), K = x.size(1);
+    TORCH_CHECK(M <= INT32_MAX, "too many rows");
+    check_tensor(weight, "weight", weight.scalar_type(), dev);
+    TORCH_CHECK(weight.dim() == 1 && weight.size(0) == K, "weight must be [K]");
+    if (residual.has_value()) {
+        check_tensor(*residual, "residual", x.scalar_type(), dev);
+        TORCH_CHECK(residual->sizes() == x.sizes(), "residual must have the shape of x");
+    }
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    at::Tensor q = empty_on(dev, {M, K}, at::kFloat8_e4m3fn), scale = empty_on(dev, {M, K / 128}, at::kFloat);
+    at::Tensor sum = residual.has_value() ? empty_on(dev, {M, K}, x.scalar_type()) : empty_on(dev, {0}, x.scalar_type());
+    at::Tensor norm = keep_norm ? empty_on(dev, {M, K}, x.scalar_type()) : empty_on(dev, {0}, x.scalar_type());
+    const int rc = alpha_moe_rms_norm_quant_fp8(
+        x.const_data_ptr(), residual.has_value() ? residual->const_data_ptr() : nullptr, weight.const_data_ptr(), x_is_f32,
+        weight_is_f32, static_cast<float>(eps), static_cast<uint8_t *>(q.data_ptr()), scale.data_ptr<float>(),
+        residual.has_value() ? sum.data_ptr() : nullptr, keep_norm ? norm.data_ptr() : nullptr, static_cast<int>(M),
+        static_cast<int>(K), static_cast<void *>(stream));
+    TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_rms_norm_quant_fp8 failed: ", alpha_moe_status_string(rc));
+    return {q, scale, sum, norm};
+}
+
+// (q, scale) of silu(gate) * up, gate_up [M, 2 I] with the gate in front.
+std::tuple<at::Tensor, at::Tensor> swiglu_quant_fp8(const at::Tensor &gate_up, int64_t group_size)
+{
+    TORCH_CHECK(gate_up.is_cuda(), "gate_up must be a GPU tensor");
+    TORCH_CHECK(group_size == 128, "group_size must be 128");
+    const at::Device dev = gate_up.device();
+    const int is_f32 = is_f32_or_bf16(gate_up, "gate_up");
+    check_tensor(gate_up, "gate_up", gate_up.scalar_type(), dev);
+    TORCH_CHECK(gate_up.dim() == 2 && gate_up.size(1) > 0 && gate_up.size(1) % 256 == 0, "gate_up must be [M, 2 I] with I % 128 == 0");
+    const int64_t M = gate_up.size(0), I = gate_up.size(1) / 2;
+    TORCH_CHECK(M <= INT32_MAX && I <= INT32_MAX / 2, "sizes exceed int32");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    at::Tensor q = empty_on(dev, {M, I}, at::kFloat8_e4m3fn), scale = empty_on(dev, {M, I / 128}, at::kFloat);
+    const int rc = alpha_moe_swiglu_quant_fp8(gate_up.const_data_ptr(), is_f32, static_cast<uint8_t *>(q.data_ptr()),
+                                              scale.data_ptr<float>(), static_cast<int>(M), static_cast<int>(I),
+                                              static_cast<void *>(stream));
+    TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_swiglu_quant_fp8 failed: ", alpha_moe_status_string(rc));
+    return {q, scale};
+}
+
+// out [M, N] = the block-scaled product of x [M, K] and w [N, K].
+at::Tensor block_scaled_mm(const at::Tensor &x, const at::Tensor &x_scale, const at::Tensor &w, const at::Tensor &w_scale)
+{
+    TORCH_CHECK(x.is_cuda(), "x must be a GPU tensor");
+    const at::Device dev = x.device();
+    check_tensor(x, "x", at::kFloat8_e4m3fn, dev);
+    check_tensor(x_scale, "x_scale", at::kFloat, dev);
+    check_tensor(w, "w", at::kFloat8_e4m3fn, dev);
+    check_tensor(w_scale, "w_scale", at::kFloat, dev);
+    TORCH_CHECK(x.dim() == 2 && x.size(1) > 0 && x.size(1) % 128 == 0 && x.size(1) <= 65536,
+                "x must be [M, K] with K % 128 == 0 and K <= 65536");
+    const int64_t M = x.size(0), K = x.size(1);
+    TORCH_CHECK(w.dim() == 2 && w.size(1) == K && w.size(0) > 0, "w must be [N, K] with the K of x");
+    const int64_t N = w.size(0);
+    TORCH_CHECK(M <= INT32_MAX && N <= INT32_MAX, "sizes exceed int32");
+    TORCH_CHECK(x_scale.dim() == 2 && x_scale.size(0) == M && x_scale.size(1) == K / 128, "x_scale must be [M, K/128]");
+    TORCH_CHECK(w_scale.dim() == 2 && w_scale.size(0) == (N + 127) / 128 && w_scale.size(1) == K / 128,
+                "w_scale must be [ceil(N/128), K/128]");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    at::Tensor out = empty_on(dev, {M, N}, at::kBFloat16), ws;
+    const size_t ws_bytes =
+        alpha_moe_block_scaled_mm_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
+    if (ws_bytes > 0) ws = empty_on(dev, {static_cast<int64_t>(ws_bytes)}, at::kByte);
+    const int rc = alpha_moe_block_scaled_mm(
+        static_cast<const uint8_t *>(x.const_data_ptr()), x_scale.const_data_ptr<float>(),
+        static_cast<const uint8_t *>(w.const_data_ptr()), w_scale.const_data_ptr<float>(),
+        static_cast<uint16_t *>(out.data_ptr()), static_cast<int>(M), static_cast<int>(N), static_cast<int>(K),
+        ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, static_cast<void *>(stream));
+    TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_block_scaled_mm failed: ", alpha_moe_status_string(rc));
+    return out;
+}
+
+// (topk_weights f32, topk_ids i32), both [M, top_k + shared_experts].
+std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor &logits, const c10::optional<at::Tensor> &bias, int64_t top_k,
+                                              bool sigmoid, int64_t num_groups, int64_t top_groups, bool renormalize,
+                                              int64_t shared_experts, double shared_weight)
+{
+    TORCH_CHECK(logits.is_cuda(), "logits must be a GPU tensor");
+    const at::Device dev = logits.device();
+    const int is_f32 = is_f32_or_bf16(logits, "logits");
+    check_tensor(logits, "logits", logits.scalar_type(), dev);
+    TORCH_CHECK(logits.dim() == 2 && logits.size(1) > 0 && logits.size(1) <= 4096, "logits must be [M, E] with 1 to 4096 experts");
+    const int64_t M = logits.size(0), E = logits.size(1);
+    TORCH_CHECK(M <= INT32_MAX, "too many rows");
+    if (bias.has_value()) {
+        check_tensor(*bias, "bias", at::kFloat, dev);
+        TORCH_CHECK(bias->dim() == 1 && bias->size(0) == E, "bias must be [E]");
+    }
+    TORCH_CHECK(top_k > 0 && top_k <= 64 && top_k <= E, "top_k must be in [1, min(E, 64)]");
+    TORCH_CHECK(num_groups > 0 && num_groups <= 64 && E % num_groups == 0, "num_groups must divide the experts, at most 64");
+    TORCH_CHECK(top_groups > 0 && top_groups <= num_groups, "top_groups must be in [1, num_groups]");
+    TORCH_CHECK(top_k <= top_groups * (E / num_groups), "top_k must not be more than the experts of top_groups groups");
+    TORCH_CHECK(shared_experts >= 0 && shared_experts <= 4096, "shared_experts must be in [0, 4096]");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    at::Tensor weights = empty_on(dev, {M, top_k + shared_experts}, at::kFloat), ids = empty_on(dev, {M, top_k + shared_experts}, at::kInt);
+    const int rc = alpha_moe_route_topk(
+        logits.const_data_ptr(), is_f32, bias.has_value() ? bias->const_data_ptr<float>() : nullptr, weights.data_ptr<float>(),
+        ids.data_ptr<int32_t>(), static_cast<int>(M), static_cast<int>(E), static_cast<int>(top_k), sigmoid,
+        static_cast<int>(num_groups), static_cast<int>(top_groups), renormalize, static_cast<int>(shared_experts),
+        static_cast<float>(shared_weight), static_cast<void *>(stream));
+    TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_route_topk failed: ", alpha_moe_status_string(rc));
+    return {weights, ids};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(alpha_moe, m)
@@ -426,6 +555,16 @@ TORCH_LIBRARY_FRAGMENT(alpha_moe, m)
     m.def("fused_experts(Tensor(a!) hidden_states, Tensor topk_ids, Tensor w, Tensor w_scale, Tensor w2, Tensor w2_scale, "
           "Tensor topk_weights, int group_size, int block_m, int block_n, int warp_n, int stages, float scaling_factor) -> ()");
     m.impl("fused_experts", c10::DispatchKey::CUDA, &fused_experts);
+    m.def("rms_norm_quant_fp8(Tensor x, Tensor weight, float eps, Tensor? residual, bool keep_norm, int group_size) -> "
+          "(Tensor, Tensor, Tensor, Tensor)");
+    m.impl("rms_norm_quant_fp8", c10::DispatchKey::CUDA, &rms_norm_quant_fp8);
+    m.def("swiglu_quant_fp8(Tensor gate_up, int group_size) -> (Tensor, Tensor)");
+    m.impl("swiglu_quant_fp8", c10::DispatchKey::CUDA, &swiglu_quant_fp8);
+    m.def("block_scaled_mm(Tensor x, Tensor x_scale, Tensor w, Tensor w_scale) -> Tensor");
+    m.impl("block_scaled_mm", c10::DispatchKey::CUDA, &block_scaled_mm);
+    m.def("route_topk(Tensor logits, Tensor? bias, int top_k, bool sigmoid, int num_groups, int top_groups, bool renormalize, "
+          "int shared_experts, float shared_weight) -> (Tensor, Tensor)");
+    m.impl("route_topk", c10::DispatchKey::CUDA, &route_topk);
     m.def("reserve_workspace(Tensor like, int bytes) -> ()");
     m.impl("reserve_workspace", c10::DispatchKey::CUDA, &reserve_workspace);
     m.def("scratch_buffers(Tensor like) -> int[]");

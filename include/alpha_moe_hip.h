@@ -25,7 +25,8 @@ enum alpha_moe_status {
     ALPHA_MOE_ERR_LAUNCH = 6,         /* the HIP runtime refused the launch (see hipGetLastError) */
     ALPHA_MOE_ERR_WORKSPACE = 7,      /* workspace null, misaligned or smaller than alpha_moe_workspace_bytes() */
     ALPHA_MOE_ERR_WAIT_EXPIRED = 8,   /* alpha_moe_workspace_check: a bounded wait between workgroups ran out */
-    ALPHA_MOE_ERR_SCRATCH_LIMIT = 9   /* ..._static: the call needs more than ALPHA_MOE_STATIC_SCRATCH_BYTES of scratch */
+    ALPHA_MOE_ERR_SCRATCH_LIMIT = 9,  /* ..._static: the call needs more than ALPHA_MOE_STATIC_SCRATCH_BYTES of scratch */
+    ALPHA_MOE_ERR_ALIGNMENT = 10      /* the operators around the layer: a matrix does not start at a multiple of 16 bytes */
 };
 
 /*
@@ -232,6 +233,53 @@ int alpha_moe_layer_call(const uint16_t *x, const int32_t *topk_ids, const uint8
                          const uint8_t *w2, const float *w2_scale, const float *topk_weights, uint16_t *out, int top_k, int M,
                          int K, int N, int num_experts, int block_m, int block_n, int warp_n, int stages,
                          float scaling_factor, void *workspace, size_t workspace_bytes, void *stream /* hipStream_t */);
+
+/*
+ * The operators around the layer call, which callers of the reference take from their engine.  All of them take M = 0 (nothing
+ * is launched), need no state between calls, and write every element of their results; matrices start at multiples of 16 bytes.
+ *
+ * alpha_moe_rms_norm_quant_fp8: h = x + residual (residual NULL: h = x), y = h / sqrt(mean(h^2) + eps) * weight in fp32;
+ * q [M, K] and scale [M, K/128] are the codes and scales of y as alpha_moe_per_token_group_quant_fp8 defines them.  x, residual,
+ * residual_out (h, rounded to x's type; NULL exactly if residual is) and norm_out (y, rounded to x's type; may be NULL) are
+ * [M, K], bf16 or (x_is_f32 != 0) fp32; weight [K] is bf16 or (weight_is_f32 != 0) fp32.  K % 128 == 0, K <= 65536.  residual_out
+ * may be residual or x.  A NaN in a group of y makes the group's scale and codes NaN.
+ */
+int alpha_moe_rms_norm_quant_fp8(const void *x, const void *residual, const void *weight, int x_is_f32, int weight_is_f32,
+                                 float eps, uint8_t *q, float *scale, void *residual_out, void *norm_out, int M, int K,
+                                 void *stream /* hipStream_t */);
+
+/*
+ * gate_up [M, 2 I] bf16 or (is_f32 != 0) fp32, the gate in the first I columns (not interleaved): q [M, I] and scale [M, I/128]
+ * are the codes and scales of gate / (1 + exp(-gate)) * up, computed in fp32.  I % 128 == 0.
+ */
+int alpha_moe_swiglu_quant_fp8(const void *gate_up, int is_f32, uint8_t *q, float *scale, int M, int I,
+                               void *stream /* hipStream_t */);
+
+/*
+ * out[m, n] = sum over blocks kb of 128 columns of x_scale[m, kb] * w_scale[n / 128, kb] * (x[m, kb] . w[n, kb]), rounded once.
+ *   x [M, K] fp8, x_scale [M, K/128] f32, w [N, K] fp8, w_scale [ceil(N / 128), K/128] f32, out [M, N] bf16.  K % 128 == 0,
+ *   K <= 65536; any N.
+ * workspace: at least alpha_moe_block_scaled_mm_workspace_bytes(M, N, K) bytes (0: it may be NULL), 256-byte aligned, any contents;
+ * calls that share one must be ordered on one stream.
+ */
+size_t alpha_moe_block_scaled_mm_workspace_bytes(int M, int N, int K);
+int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale, const uint8_t *w, const float *w_scale,
+                              uint16_t *out, int M, int N, int K, void *workspace, size_t workspace_bytes,
+                              void *stream /* hipStream_t */);
+
+/*
+ * The experts of each token from logits [M, E] (bf16, or fp32 with is_f32 != 0), in the form alpha_moe_moe_align_block_size and the
+ * fused calls take: topk_ids and topk_weights [M, top_k + shared_experts].
+ *   score s = softmax(logits) or (sigmoid != 0) sigmoid(logits); choice = s + bias[e] in 64 bits, or the logit itself if bias is NULL;
+ *   with num_groups > 1 only experts of the top_groups best of num_groups equal runs of experts stay, a run being worth the sum of its
+ *   two largest choices (its largest if bias is NULL); then the top_k largest choices, descending, equal ones by ascending index.
+ *   weights s, divided by their sum if renormalize != 0; the last shared_experts columns are E, E + 1, ... with shared_weight.
+ * A NaN choice ranks as -infinity and every id is valid; a row that holds a NaN logit has NaN weights; a row whose chosen scores
+ * are all 0 has weights of 0.  E <= 4096, top_k <= 64, num_groups <= 64, top_k <= top_groups * E / num_groups.
+ */
+int alpha_moe_route_topk(const void *logits, int is_f32, const float *bias, float *topk_weights, int32_t *topk_ids, int M, int E,
+                         int top_k, int sigmoid, int num_groups, int top_groups, int renormalize, int shared_experts,
+                         float shared_weight, void *stream /* hipStream_t */);
 
 /* Human-readable text for a status code (static storage). */
 const char *alpha_moe_status_string(int status);
