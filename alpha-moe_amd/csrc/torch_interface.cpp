@@ -495,15 +495,12 @@ at::Tensor block_scaled_mm(const at::Tensor &x, const at::Tensor &x_scale, const
                 "w_scale must be [ceil(N/128), K/128]");
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
-    at::Tensor out = empty_on(dev, {M, N}, at::kBFloat16), ws;
-    const size_t ws_bytes =
-        alpha_moe_block_scaled_mm_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
-    if (ws_bytes > 0) ws = empty_on(dev, {static_cast<int64_t>(ws_bytes)}, at::kByte);
+    at::Tensor out = empty_on(dev, {M, N}, at::kBFloat16);
     const int rc = alpha_moe_block_scaled_mm(
         static_cast<const uint8_t *>(x.const_data_ptr()), x_scale.const_data_ptr<float>(),
         static_cast<const uint8_t *>(w.const_data_ptr()), w_scale.const_data_ptr<float>(),
         static_cast<uint16_t *>(out.data_ptr()), static_cast<int>(M), static_cast<int>(N), static_cast<int>(K),
-        ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, static_cast<void *>(stream));
+        static_cast<void *>(stream));
     TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_block_scaled_mm failed: ", alpha_moe_status_string(rc));
     return out;
 }

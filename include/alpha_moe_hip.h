@@ -258,14 +258,10 @@ int alpha_moe_swiglu_quant_fp8(const void *gate_up, int is_f32, uint8_t *q, floa
 /*
  * out[m, n] = sum over blocks kb of 128 columns of x_scale[m, kb] * w_scale[n / 128, kb] * (x[m, kb] . w[n, kb]), rounded once.
  *   x [M, K] fp8, x_scale [M, K/128] f32, w [N, K] fp8, w_scale [ceil(N / 128), K/128] f32, out [M, N] bf16.  K % 128 == 0,
- *   K <= 65536; any N.
- * workspace: at least alpha_moe_block_scaled_mm_workspace_bytes(M, N, K) bytes (0: it may be NULL), 256-byte aligned, any contents;
- * calls that share one must be ordered on one stream.
+ *   K <= 65536; any N.  Sums are taken in an order that depends on M, N and K only.
  */
-size_t alpha_moe_block_scaled_mm_workspace_bytes(int M, int N, int K);
 int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale, const uint8_t *w, const float *w_scale,
-                              uint16_t *out, int M, int N, int K, void *workspace, size_t workspace_bytes,
-                              void *stream /* hipStream_t */);
+                              uint16_t *out, int M, int N, int K, void *stream /* hipStream_t */);
 
 /*
  * The experts of each token from logits [M, E] (bf16, or fp32 with is_f32 != 0), in the form alpha_moe_moe_align_block_size and the

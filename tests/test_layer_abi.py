@@ -46,15 +46,14 @@ def test_swiglu_refusals():
 
 def test_mm_refusals():
     def call(x=4096, xs=4096, w=4096, ws=4096, out=4096, M=4, N=100, K=256):
-        return c("alpha_moe_block_scaled_mm", [P, P, P, P, P, I, I, I, P, ctypes.c_size_t, P], x, xs, w, ws, out, M, N, K, None,
-                 0, None)
+        return c("alpha_moe_block_scaled_mm", [P, P, P, P, P, I, I, I, P], x, xs, w, ws, out, M, N, K, None)
     assert call(M=0) == OK and call(M=-1) == SHAPE and call(N=0) == SHAPE and call(K=0) == SHAPE and call(K=64) == SHAPE
     assert call(K=65536 + 128) == SHAPE
     for name in ("x", "xs", "w", "ws", "out"):
         assert call(**{name: None}) == NULL, name
     for name in ("x", "w", "out"):
         assert call(**{name: 4104}) == ALIGN, name
-    assert c("alpha_moe_block_scaled_mm_workspace_bytes", [I, I, I], 0, 128, 128, restype=ctypes.c_size_t) == 0
+    assert call(M=2 ** 31 - 1) == SHAPE and call(N=2 ** 31 - 1) == SHAPE and call(M=2 ** 30, N=2 ** 30) == SHAPE
 
 
 def test_route_refusals():
