@@ -295,7 +295,10 @@ ROUTES = [dict(E=1, top_k=1), dict(E=8, top_k=8), dict(E=60, top_k=4), dict(E=64
           dict(E=160, top_k=6, num_groups=8, top_groups=3), dict(E=256, top_k=8, num_groups=8, top_groups=4, shared_experts=1, shared_weight=0.4),
           dict(E=256, top_k=8, num_groups=64, top_groups=3), dict(E=64, top_k=3, num_groups=64, top_groups=3), dict(E=257, top_k=9),
           dict(E=512, top_k=10), dict(E=700, top_k=20, num_groups=7, top_groups=2), dict(E=1024, top_k=8, num_groups=16, top_groups=1),
-          dict(E=4096, top_k=33, num_groups=4, top_groups=2, shared_experts=70), dict(E=1500, top_k=2)]
+          dict(E=4096, top_k=33, num_groups=4, top_groups=2, shared_experts=70), dict(E=1500, top_k=2),
+          dict(E=4095, top_k=12, num_groups=5, top_groups=2), dict(E=4096, top_k=5, num_groups=64, top_groups=7),
+          dict(E=48, top_k=5, num_groups=3, top_groups=2), dict(E=36, top_k=4, num_groups=6, top_groups=3),
+          dict(E=128, top_k=6, num_groups=2, top_groups=1), dict(E=512, top_k=16, num_groups=4, top_groups=2)]
 
 
 @pytest.mark.parametrize("renormalize", [True, False])
@@ -334,6 +337,55 @@ def test_route_scores_nearer_than_fp32_tells():
     assert_route(logits, 16, scoring="sigmoid", bias=bias)
     assert_route(40 + logits * 20, 16, scoring="sigmoid", bias=torch.zeros(64))       # saturated: equal in fp32
     assert_route(40 + logits * 20, 16, scoring="sigmoid")
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups,scale", [(64, 1, 0.3), (256, 8, 0.1), (200, 4, 0.1), (96, 6, 1000.0), (700, 7, 0.1)])
+def test_route_neighbours_and_groups_that_are_almost_equal(E, groups, scale, scoring):
+    """in every row one pair of good experts, or a pair of groups, whose choices differ by fp32's last bits of a logit or not at all:
+    the order of two, the last that is chosen and the first that is not, and the last group that stays"""
+    g = torch.Generator().manual_seed(E)
+    bias = (scale * torch.randn(E, generator=g)).float()
+    size = E // groups
+    if groups > 1:
+        bias = bias[:size].repeat(groups)            # (groups alike, so that equal logits make equal groups)
+    M, top_k = 150, 8
+    logits = torch.randn((M, E), generator=g)
+    for m in range(M):
+        if groups > 1 and m % 2:
+            worth = (torch.sigmoid(logits[m].double()) + bias.double()).view(groups, size).topk(2).values.sum(-1)
+            order = worth.argsort(descending=True)
+            a, b = order[groups // 2 - 1].item(), order[groups // 2].item()
+            copy = logits[m, a * size:(a + 1) * size].clone()
+            logits[m, b * size:(b + 1) * size] = copy
+            if m % 3:
+                logits[m, b * size:(b + 1) * size] = torch.nextafter(copy, torch.tensor(9.0 if m % 3 == 1 else -9.0))
+        elif scoring == "sigmoid":
+            choice = torch.sigmoid(logits[m].double()) + bias.double()
+            order = choice.argsort(descending=True)
+            i = m % (top_k + 1)
+            a, b = order[i].item(), order[i + 1].item()
+            want = choice[a] - bias[b].double()      # the score that makes b's choice a's
+            if 0.01 < want < 0.99:
+                logits[m, b] = torch.log(want / (1 - want)).float()
+        else:
+            logits[m, m % E] = logits[m, (m * 7 + 1) % E]
+    for kw in (dict(), dict(num_groups=groups, top_groups=max(1, groups // 2))):
+        assert_route(logits, top_k, scoring=scoring, bias=bias, **kw)
+    assert_route(logits, 64, scoring=scoring, bias=bias)
+    assert_route(logits, 63, scoring=scoring, bias=bias)
+
+
+def test_route_with_infinite_biases():
+    g = torch.Generator().manual_seed(11)
+    logits = torch.randn((20, 64), generator=g)
+    bias = 0.1 * torch.randn(64, generator=g)
+    bias[3], bias[50] = float("inf"), float("inf")
+    bias[10:30] = -float("inf")
+    for scoring in ("softmax", "sigmoid"):
+        assert_route(logits, 8, scoring=scoring, bias=bias)
+        assert_route(logits, 60, scoring=scoring, bias=bias)
+        assert_route(logits, 8, scoring=scoring, bias=bias.clamp(max=0), num_groups=8, top_groups=6)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
