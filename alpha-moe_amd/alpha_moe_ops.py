@@ -54,10 +54,23 @@ def _fused_experts_fake(hidden_states, topk_ids, w, w_scale, w2, w2_scale, topk_
 
 
 @torch.library.register_fake("alpha_moe::rms_norm_quant_fp8")
-def _rms_norm_quant_fp8_fake(x, weight, eps, residual, keep_norm, group_size):
-    return (*_per_token_group_quant_fp8_fake(x, group_size),
-            torch.empty_like(x) if residual is not None else x.new_empty((0,)),
-            torch.empty_like(x) if keep_norm else x.new_empty((0,)))
+def _rms_norm_quant_fp8_fake(x, weight, eps, group_size):
+    return _per_token_group_quant_fp8_fake(x, group_size)
+
+
+@torch.library.register_fake("alpha_moe::rms_norm_quant_fp8.keep_norm")
+def _rms_norm_quant_fp8_keep_fake(x, weight, eps, group_size):
+    return (*_per_token_group_quant_fp8_fake(x, group_size), torch.empty_like(x))
+
+
+@torch.library.register_fake("alpha_moe::add_rms_norm_quant_fp8")
+def _add_rms_norm_quant_fp8_fake(x, residual, weight, eps, group_size):
+    return (*_per_token_group_quant_fp8_fake(x, group_size), torch.empty_like(x))
+
+
+@torch.library.register_fake("alpha_moe::add_rms_norm_quant_fp8.keep_norm")
+def _add_rms_norm_quant_fp8_keep_fake(x, residual, weight, eps, group_size):
+    return (*_per_token_group_quant_fp8_fake(x, group_size), torch.empty_like(x), torch.empty_like(x))
 
 
 @torch.library.register_fake("alpha_moe::swiglu_quant_fp8")

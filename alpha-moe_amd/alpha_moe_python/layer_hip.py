@@ -16,7 +16,10 @@ import torch
 import alpha_moe  # noqa: F401  (registers the operators; fails if the libraries are not built)
 
 # (the overloads themselves: the lookup of one by name is a microsecond of a call on a few tokens)
-_rms_norm_quant_fp8 = torch.ops.alpha_moe.rms_norm_quant_fp8.default
+_norm = torch.ops.alpha_moe.rms_norm_quant_fp8.default
+_norm_keep = torch.ops.alpha_moe.rms_norm_quant_fp8.keep_norm
+_add_norm = torch.ops.alpha_moe.add_rms_norm_quant_fp8.default
+_add_norm_keep = torch.ops.alpha_moe.add_rms_norm_quant_fp8.keep_norm
 _swiglu_quant_fp8 = torch.ops.alpha_moe.swiglu_quant_fp8.default
 _block_scaled_mm = torch.ops.alpha_moe.block_scaled_mm.default
 _route_topk = torch.ops.alpha_moe.route_topk.default
@@ -39,8 +42,14 @@ def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     in a group that holds one), ``residual`` = ``h`` in x's dtype (a new tensor), and with ``keep_norm`` ``norm`` = ``y`` in x's
     dtype, which a router or a bf16 product reads.
     """
-    q, scale, total, norm = _rms_norm_quant_fp8(x, weight, eps, residual, keep_norm, group_size)
-    return NormQuant(q, scale, total if residual is not None else None, norm if keep_norm else None)
+    if residual is None:
+        if not keep_norm:
+            return NormQuant(*_norm(x, weight, eps, group_size), None, None)
+        q, scale, norm = _norm_keep(x, weight, eps, group_size)
+        return NormQuant(q, scale, None, norm)
+    if not keep_norm:
+        return NormQuant(*_add_norm(x, residual, weight, eps, group_size), None)
+    return NormQuant(*_add_norm_keep(x, residual, weight, eps, group_size))
 
 
 def swiglu_quant_fp8(gate_up: torch.Tensor, group_size: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -15,42 +15,76 @@
 namespace alpha_moe {
 namespace {
 
+// What a lane loads at a time: N values in 16 bytes (of a row of another type than the activations', the same N values).
 template <typename T>
-struct Lane;   // what a lane loads at a time: 16 bytes
+struct Lane;
 template <>
 struct Lane<uint16_t> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ void load(const void *p, size_t at, float (&v)[N])
-    {
-        const v4i raw = *reinterpret_cast<const v4i *>(static_cast<const uint16_t *>(p) + at);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[2 * i] = __builtin_bit_cast(float, (uint32_t)raw[i] << 16);
-            v[2 * i + 1] = __builtin_bit_cast(float, (uint32_t)raw[i] & 0xffff0000u);
-        }
-    }
-    static __device__ __forceinline__ void store(void *p, size_t at, const float (&v)[N])
-    {
-        v4i raw;
-#pragma unroll
-        for (int i = 0; i < 4; i++) raw[i] = (int)pack_bf16x2(v[2 * i], v[2 * i + 1]);
-        *reinterpret_cast<v4i *>(static_cast<uint16_t *>(p) + at) = raw;
-    }
 };
 template <>
 struct Lane<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ void load(const void *p, size_t at, float (&v)[N])
-    {
-        const v4f raw = *reinterpret_cast<const v4f *>(static_cast<const float *>(p) + at);
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = raw[i];
-    }
-    static __device__ __forceinline__ void store(void *p, size_t at, const float (&v)[N])
-    {
-        *reinterpret_cast<v4f *>(static_cast<float *>(p) + at) = (v4f){v[0], v[1], v[2], v[3]};
-    }
 };
+
+template <typename T, int N>
+struct Raw {
+    static constexpr int kBytes = N * (int)sizeof(T);   // 8, 16 or 32
+    static constexpr int kWords = kBytes < 16 ? kBytes / 4 : 4;
+    typedef uint32_t Piece __attribute__((ext_vector_type(kWords)));
+    Piece piece[kBytes / (4 * kWords)];
+    __device__ __forceinline__ void load(const void *p, size_t at)
+    {
+#pragma unroll
+        for (int i = 0; i < kBytes / (4 * kWords); i++) piece[i] = reinterpret_cast<const Piece *>(static_cast<const T *>(p) + at)[i];
+    }
+    __device__ __forceinline__ void store(void *p, size_t at) const
+    {
+#pragma unroll
+        for (int i = 0; i < kBytes / (4 * kWords); i++) reinterpret_cast<Piece *>(static_cast<T *>(p) + at)[i] = piece[i];
+    }
+    __device__ __forceinline__ float value(int i) const
+    {
+        // (a copy first: the builtin takes element 0 of a vector for any element of it)
+        const uint32_t word = sizeof(T) == 4 ? piece[i / 4][i % 4] : piece[0][i / 2];
+        return __builtin_bit_cast(float, sizeof(T) == 4 ? word : i % 2 ? word & 0xffff0000u : word << 16);
+    }
+    __device__ __forceinline__ explicit Raw(const float (&v)[N])
+    {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if constexpr (sizeof(T) == 4) piece[i / 4][i % 4] = __builtin_bit_cast(uint32_t, v[i]);
+            else if (i % 2 == 0) piece[0][i / 2] = pack_bf16x2(v[i], v[i + 1]);
+        }
+    }
+    Raw() = default;
+};
+
+__device__ __forceinline__ float wave_sum(float v)   // in lane 63
+{
+#define NORM_STEP(ctrl, rows) \
+    v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), ctrl, rows, 0xf, false))
+    NORM_STEP(0x111, 0xf);   // from 1, 2, 4, 8 lanes below in the row
+    NORM_STEP(0x112, 0xf);
+    NORM_STEP(0x114, 0xf);
+    NORM_STEP(0x118, 0xf);
+    NORM_STEP(0x142, 0xa);   // lane 15 of rows 0 and 2 to rows 1 and 3
+    NORM_STEP(0x143, 0xc);   // lane 31 to rows 2 and 3
+#undef NORM_STEP
+    return v;
+}
+
+// The largest of the 16 or 32 lanes of a group, in all of them.
+template <int LANES>
+__device__ __forceinline__ uint32_t group_max(uint32_t m)
+{
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xb1, 0xf, 0xf, false));    // lanes 1, 0, 3, 2
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4e, 0xf, 0xf, false));    // lanes 2, 3, 0, 1
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xf, 0xf, false));   // mirrored in eight
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xf, 0xf, false));   // mirrored in sixteen
+    if constexpr (LANES == 32) m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+    return m;
+}
 
 // The codes of N values of a lane whose group of 128 is held by 128 / N neighbouring lanes; every lane of the group calls it.
 template <int N>
@@ -62,8 +96,7 @@ struct GroupQuant {
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < N; i++) m = max(m, __builtin_bit_cast(uint32_t, y[i]) & 0x7fffffffu);
-#pragma unroll
-        for (int d = 1; d < 128 / N; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+        m = group_max<128 / N>(m);
         scale = m < 0x7f800000u ? fmaxf(__builtin_bit_cast(float, m), kAmaxFloor) / kFp8Max : __builtin_bit_cast(float, m);
         if (m < 0x7f800000u) {
             float r = __builtin_amdgcn_rcpf(scale);
@@ -89,27 +122,6 @@ struct GroupQuant {
     }
 };
 
-// N values of a row of another type than the activations'
-template <typename W, int N>
-__device__ __forceinline__ void load_weight(const void *p, int at, float (&v)[N])
-{
-    if constexpr (Lane<W>::N == N) {
-        Lane<W>::load(p, at, v);
-    } else if constexpr (sizeof(W) == 4) {
-        float lo[4], hi[4];
-        Lane<W>::load(p, at, lo);
-        Lane<W>::load(p, at + 4, hi);
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = lo[i], v[4 + i] = hi[i];
-    } else {
-        const uint2 raw = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(p) + at);
-        v[0] = __builtin_bit_cast(float, raw.x << 16);
-        v[1] = __builtin_bit_cast(float, raw.x & 0xffff0000u);
-        v[2] = __builtin_bit_cast(float, raw.y << 16);
-        v[3] = __builtin_bit_cast(float, raw.y & 0xffff0000u);
-    }
-}
-
 struct NormParams {
     const void *x, *residual, *weight;
     void *residual_out, *norm_out;
@@ -119,59 +131,69 @@ struct NormParams {
     int M, K;
 };
 
-__device__ __forceinline__ float wave_sum(float v)
-{
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
-}
-
-// One workgroup to a row, which stays in registers between its sum of squares and its codes: P pieces of 16 bytes a thread.
+// One workgroup to a row, which stays in registers between its sum of squares and its codes: P pieces of 16 bytes a thread, all
+// loads of them in flight at once (pieces behind the row's end: its last one again, and not used).
 template <typename T, typename W, int P>
 __global__ __launch_bounds__(1024) void rms_norm_kernel(const NormParams s)
 {
     constexpr int N = Lane<T>::N;
     __shared__ float sums[16];
-    const int K = s.K, tid = threadIdx.x;
+    const int K = s.K, tid = threadIdx.x, step = (int)blockDim.x * N;
     const size_t row = (size_t)blockIdx.x * K;
+    Raw<T, N> x[P], add[P];
+    Raw<W, N> weight[P];
+#pragma unroll
+    for (int p = 0; p < P; p++) {
+        const int c = min(p * step + tid * N, K - N);
+        x[p].load(s.x, row + c);
+        if (s.residual) add[p].load(s.residual, row + c);
+    }
+#pragma unroll
+    for (int p = 0; p < P; p++) weight[p].load(s.weight, min(p * step + tid * N, K - N));
     float h[P][N];
     float sum = 0.f;
 #pragma unroll
     for (int p = 0; p < P; p++) {
-        const int c = (p * (int)blockDim.x + tid) * N;
-        if (c < K) {
-            Lane<T>::load(s.x, row + c, h[p]);
-            if (s.residual) {
-                float add[N];
-                Lane<T>::load(s.residual, row + c, add);
+        const int c = p * step + tid * N;
 #pragma unroll
-                for (int i = 0; i < N; i++) h[p][i] += add[i];
-                Lane<T>::store(s.residual_out, row + c, h[p]);
-            }
+        for (int i = 0; i < N; i++) h[p][i] = x[p].value(i);
+        if (s.residual) {
 #pragma unroll
-            for (int i = 0; i < N; i++) sum += h[p][i] * h[p][i];
+            for (int i = 0; i < N; i++) h[p][i] += add[p].value(i);
+            if (c < K) Raw<T, N>(h[p]).store(s.residual_out, row + c);
         }
+        float part = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) part += h[p][i] * h[p][i];
+        sum += c < K ? part : 0.f;
     }
     sum = wave_sum(sum);
-    if ((tid & 63) == 0) sums[tid >> 6] = sum;
+    if ((tid & 63) == 63) sums[tid >> 6] = sum;
     __syncthreads();
     sum = 0.f;
     for (int w = 0; w < (int)blockDim.x >> 6; w++) sum += sums[w];
     const float r = 1.0f / sqrtf(sum / (float)K + s.eps);
 #pragma unroll
     for (int p = 0; p < P; p++) {
-        const int c = (p * (int)blockDim.x + tid) * N;
+        const int c = p * step + tid * N;
         if (c < K) {   // (a group's lanes agree)
             float y[N];
-            load_weight<W>(s.weight, c, y);
 #pragma unroll
-            for (int i = 0; i < N; i++) y[i] = h[p][i] * r * y[i];
-            if (s.norm_out) Lane<T>::store(s.norm_out, row + c, y);
+            for (int i = 0; i < N; i++) y[i] = h[p][i] * r * weight[p].value(i);
+            if (s.norm_out) Raw<T, N>(y).store(s.norm_out, row + c);
             const GroupQuant<N> g(y);
             g.store(s.q, row + c);
             if ((c & 127) == 0) s.scale[(row + c) >> 7] = g.scale;
         }
     }
+}
+
+// g / (1 + exp(-g)) within (1.25 |g| + 9) roundings: the exponent's counts 1.25 |g|, the others one or two each.  The reciprocal is of
+// a quarter of 1 + exp(-g): where that is infinite the result is g * 0, and elsewhere it is a normal number.
+__device__ __forceinline__ float silu(float g)
+{
+    const float den = __builtin_fmaf(__builtin_amdgcn_exp2f(g * -1.44269504f), 0.25f, 0.25f);
+    return 0.25f * g * __builtin_amdgcn_rcpf(den);
 }
 
 template <typename T>
@@ -184,11 +206,12 @@ __global__ __launch_bounds__(256) void swiglu_kernel(const void *gate_up, uint8_
     for (long long g = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; g < n_groups; g += stride) {
         const long long row = g / per_row;
         const size_t at = (size_t)row * 2 * I + (size_t)(g - row * per_row) * 128 + sub * N;
-        float a[N], u[N];
-        Lane<T>::load(gate_up, at, a);
-        Lane<T>::load(gate_up, at + I, u);
+        Raw<T, N> gate, up;
+        gate.load(gate_up, at);
+        up.load(gate_up, at + I);
+        float a[N];
 #pragma unroll
-        for (int i = 0; i < N; i++) a[i] = a[i] / (1.0f + expf(-a[i])) * u[i];
+        for (int i = 0; i < N; i++) a[i] = silu(gate.value(i)) * up.value(i);
         const GroupQuant<N> c(a);
         c.store(q, (size_t)g * 128 + sub * N);
         if (sub == 0) scale[g] = c.scale;
@@ -202,7 +225,8 @@ hipError_t launch_norm(const NormParams &s, hipStream_t stream)
     typedef void (*Fn)(const NormParams);
     Fn fn;
     int per;
-    if (pieces <= 1024) fn = rms_norm_kernel<T, W, 1>, per = 1;
+    // (one piece a thread: 8192 x 7168 bf16 79 us, two 73, four 75; up to 512 threads the first is as good or better: 64 x 4096 3.3, 3.4)
+    if (pieces <= 512) fn = rms_norm_kernel<T, W, 1>, per = 1;
     else if (pieces <= 2048) fn = rms_norm_kernel<T, W, 2>, per = 2;
     else if (pieces <= 4096) fn = rms_norm_kernel<T, W, 4>, per = 4;
     else if (pieces <= 8192) fn = rms_norm_kernel<T, W, 8>, per = 8;

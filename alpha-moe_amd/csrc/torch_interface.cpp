@@ -419,11 +419,13 @@ int is_f32_or_bf16(const at::Tensor &t, const char *name)
     return t.scalar_type() == at::kFloat;
 }
 
-// (q, scale, residual, norm): y = rms_norm(x + residual) * weight quantised as above; the sum and y in x's type, each empty
-// if it is not asked for.
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
-rms_norm_quant_fp8(const at::Tensor &x, const at::Tensor &weight, double eps, const c10::optional<at::Tensor> &residual,
-                   bool keep_norm, int64_t group_size)
+// y = rms_norm(x + residual) * weight quantised as above, and - where they are asked for, otherwise undefined - the sum and y in x's
+// type.
+struct NormQuant {
+    at::Tensor q, scale, residual, norm;
+};
+NormQuant run_norm(const at::Tensor &x, const at::Tensor *residual, const at::Tensor &weight, double eps, int64_t group_size,
+                   bool keep_norm)
 {
     TORCH_CHECK(x.is_cuda(), "x must be a GPU tensor");
     TORCH_CHECK(group_size == 128, "group_size must be 128");
@@ -436,22 +438,49 @@ rms_norm_quant_fp8(const at::Tensor &x, const at::Tensor &weight, double eps, co
     TORCH_CHECK(M <= INT32_MAX, "too many rows");
     check_tensor(weight, "weight", weight.scalar_type(), dev);
     TORCH_CHECK(weight.dim() == 1 && weight.size(0) == K, "weight must be [K]");
-    if (residual.has_value()) {
+    if (residual) {
         check_tensor(*residual, "residual", x.scalar_type(), dev);
         TORCH_CHECK(residual->sizes() == x.sizes(), "residual must have the shape of x");
     }
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
-    at::Tensor q = empty_on(dev, {M, K}, at::kFloat8_e4m3fn), scale = empty_on(dev, {M, K / 128}, at::kFloat);
-    at::Tensor sum = residual.has_value() ? empty_on(dev, {M, K}, x.scalar_type()) : empty_on(dev, {0}, x.scalar_type());
-    at::Tensor norm = keep_norm ? empty_on(dev, {M, K}, x.scalar_type()) : empty_on(dev, {0}, x.scalar_type());
+    NormQuant r;
+    r.q = empty_on(dev, {M, K}, at::kFloat8_e4m3fn);
+    r.scale = empty_on(dev, {M, K / 128}, at::kFloat);
+    if (residual) r.residual = empty_on(dev, {M, K}, x.scalar_type());
+    if (keep_norm) r.norm = empty_on(dev, {M, K}, x.scalar_type());
     const int rc = alpha_moe_rms_norm_quant_fp8(
-        x.const_data_ptr(), residual.has_value() ? residual->const_data_ptr() : nullptr, weight.const_data_ptr(), x_is_f32,
-        weight_is_f32, static_cast<float>(eps), static_cast<uint8_t *>(q.data_ptr()), scale.data_ptr<float>(),
-        residual.has_value() ? sum.data_ptr() : nullptr, keep_norm ? norm.data_ptr() : nullptr, static_cast<int>(M),
+        x.const_data_ptr(), residual ? residual->const_data_ptr() : nullptr, weight.const_data_ptr(), x_is_f32, weight_is_f32,
+        static_cast<float>(eps), static_cast<uint8_t *>(r.q.data_ptr()), r.scale.data_ptr<float>(),
+        residual ? r.residual.data_ptr() : nullptr, keep_norm ? r.norm.data_ptr() : nullptr, static_cast<int>(M),
         static_cast<int>(K), static_cast<void *>(stream));
     TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_rms_norm_quant_fp8 failed: ", alpha_moe_status_string(rc));
-    return {q, scale, sum, norm};
+    return r;
+}
+
+// One operator for each set of results: a tensor that nobody asked for costs a call on a few tokens as much as a fifth of it.
+std::tuple<at::Tensor, at::Tensor> rms_norm_quant_fp8(const at::Tensor &x, const at::Tensor &weight, double eps, int64_t group_size)
+{
+    NormQuant r = run_norm(x, nullptr, weight, eps, group_size, false);
+    return {std::move(r.q), std::move(r.scale)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_quant_fp8_keep(const at::Tensor &x, const at::Tensor &weight, double eps,
+                                                                       int64_t group_size)
+{
+    NormQuant r = run_norm(x, nullptr, weight, eps, group_size, true);
+    return {std::move(r.q), std::move(r.scale), std::move(r.norm)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_quant_fp8(const at::Tensor &x, const at::Tensor &residual,
+                                                                      const at::Tensor &weight, double eps, int64_t group_size)
+{
+    NormQuant r = run_norm(x, &residual, weight, eps, group_size, false);
+    return {std::move(r.q), std::move(r.scale), std::move(r.residual)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>
+add_rms_norm_quant_fp8_keep(const at::Tensor &x, const at::Tensor &residual, const at::Tensor &weight, double eps, int64_t group_size)
+{
+    NormQuant r = run_norm(x, &residual, weight, eps, group_size, true);
+    return {std::move(r.q), std::move(r.scale), std::move(r.residual), std::move(r.norm)};
 }
 
 // (q, scale) of silu(gate) * up, gate_up [M, 2 I] with the gate in front.
@@ -552,9 +581,16 @@ TORCH_LIBRARY_FRAGMENT(alpha_moe, m)
     m.def("fused_experts(Tensor(a!) hidden_states, Tensor topk_ids, Tensor w, Tensor w_scale, Tensor w2, Tensor w2_scale, "
           "Tensor topk_weights, int group_size, int block_m, int block_n, int warp_n, int stages, float scaling_factor) -> ()");
     m.impl("fused_experts", c10::DispatchKey::CUDA, &fused_experts);
-    m.def("rms_norm_quant_fp8(Tensor x, Tensor weight, float eps, Tensor? residual, bool keep_norm, int group_size) -> "
-          "(Tensor, Tensor, Tensor, Tensor)");
+    m.def("rms_norm_quant_fp8(Tensor x, Tensor weight, float eps, int group_size) -> (Tensor, Tensor)");
     m.impl("rms_norm_quant_fp8", c10::DispatchKey::CUDA, &rms_norm_quant_fp8);
+    m.def("rms_norm_quant_fp8.keep_norm(Tensor x, Tensor weight, float eps, int group_size) -> (Tensor, Tensor, Tensor)");
+    m.impl("rms_norm_quant_fp8.keep_norm", c10::DispatchKey::CUDA, &rms_norm_quant_fp8_keep);
+    m.def("add_rms_norm_quant_fp8(Tensor x, Tensor residual, Tensor weight, float eps, int group_size) -> "
+          "(Tensor, Tensor, Tensor)");
+    m.impl("add_rms_norm_quant_fp8", c10::DispatchKey::CUDA, &add_rms_norm_quant_fp8);
+    m.def("add_rms_norm_quant_fp8.keep_norm(Tensor x, Tensor residual, Tensor weight, float eps, int group_size) -> "
+          "(Tensor, Tensor, Tensor, Tensor)");
+    m.impl("add_rms_norm_quant_fp8.keep_norm", c10::DispatchKey::CUDA, &add_rms_norm_quant_fp8_keep);
     m.def("swiglu_quant_fp8(Tensor gate_up, int group_size) -> (Tensor, Tensor)");
     m.impl("swiglu_quant_fp8", c10::DispatchKey::CUDA, &swiglu_quant_fp8);
     m.def("block_scaled_mm(Tensor x, Tensor x_scale, Tensor w, Tensor w_scale) -> Tensor");
