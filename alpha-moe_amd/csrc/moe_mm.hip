@@ -264,37 +264,44 @@ hipError_t launch_stream_mm(MmParams p, hipStream_t stream)
 //
 // One barrier to a K block, in front of the last token tile's pass: by then all fragments of the stage are in registers, so the stage
 // behind the barrier can be refilled at once and has nearly S - 1 K blocks of time for it, and the pass replaces each weight
-// fragment by the next K block's as it is used for the last time, so the next K block starts without a wait.  The loads of a stage go
-// out one by one between matrix instructions (in a burst, wavefronts wait for the path into the compute unit instead).
+// fragment by the next K block's as it is used for the last time, so the next K block starts without a wait.
+//
+// The loads: a wavefront that hands loads to the path into the compute unit (64 bytes a cycle) waits for it, and its matrix
+// instructions with it.  Where registers allow, LOADERS more wavefronts do nothing but load (128 x 128 tile, 1024 x 4096 x 7168 43.5 ->
+// 35.8 us, 128 x 64, 256 x 7168 x 2048 9.9 -> 9.4).  The 256 x 256 tile has no registers left for them: there the loads of a stage go
+// out one by one between matrix instructions, over the first three eighths of a K block (8192 x 4096 x 7168 in a burst 226, over three
+// eighths 221, over all of it 231).
 //
 // What bounds it: matrix instructions and their scaling multiply-adds (19.3 ns a pair on random operands, where the clock gives way:
-// 138 us for 8192 x 4096 x 7168) and, with all compute units at work, the tiles' way from L2 (a K block of a 256 x 256 tile 1.45 us with
-// few tiles, 1.95 with 256).  MI355X: 8192 x 4096 x 7168 225 us (2.14 PFLOP/s; a library product of the same size without block
-// scales 188), 4096 x 4096 x 7168 107, 1024 x 7168 x 2048 20.6, 256 x 7168 x 2048 9.7.  With the stage's loads in a burst and all fragments read
-// behind the barrier 239 us; 128 columns x 64 tokens a wavefront (2 x 4 wavefronts) 237.
-template <int TN, int TM, int WN, int WM, int S>
+// 138 us for 8192 x 4096 x 7168; on equal operands 14.8), and LDS, which takes loads in at 64 bytes a cycle while fragments are
+// read from it (without any loads the same kernel takes 137 us).  MI355X: 8192 x 4096 x 7168 221 us (2.18 PFLOP/s; a library product of
+// the same size without block scales 188), 4096 x 4096 x 7168 105, 1024 x 7168 x 2048 20.5, 256 x 7168 x 2048 9.4.  Also
+// tried: 128 columns x 64 tokens a wavefront 237; token fragments read two passes ahead 228; all fragments read behind the barrier 239.
+template <int TN, int TM, int WN, int WM, int S, int LOADERS>
 struct Tile {
-    static constexpr int kWaves = WN * WM, kCols = TN * 16 * WN, kTokens = TM * 16 * WM;
+    static constexpr int kWaves = WN * WM, kLoaders = LOADERS > 0 ? LOADERS : kWaves, kCols = TN * 16 * WN, kTokens = TM * 16 * WM;
     static constexpr int kStage = (kCols + kTokens) * 128 + kTokens * 4;
     static constexpr int kScaleRows = (kCols + 127) / 128;   // a tile starts at a multiple of its columns
     static constexpr int kBytes = S * kStage + kScaleRows * kMaxKBlocks * 4;
-    static constexpr int kW = kCols / 8 / kWaves, kX = kTokens / 8 / kWaves;   // 1 KiB pieces a wavefront loads per stage
+    static constexpr int kW = kCols / 8 / kLoaders, kX = kTokens / 8 / kLoaders;   // 1 KiB pieces a loading wavefront has per stage
     static constexpr int kLoads = kW + kX + 1;   // of a wavefront and stage; the last: its share of the tokens' scales
-    static constexpr int kScaleLanes = kTokens / kWaves;
+    static constexpr int kScaleLanes = kTokens / kLoaders;
     // Piece j of a stage is issued behind matrix instruction at(j) of the TN * TM that follow the barrier which frees its place.
-    static constexpr int at(int j) { return S == 2 ? j * TN / kLoads : j * (TN * TM) / kLoads; }
+    static constexpr int at(int j) { return j * (S == 2 ? TN * TM * 3 / 8 : TN * TM) / kLoads; }
     static constexpr int early() { int c = 0; while (c < kLoads && at(c) < TN) c++; return c; }   // those in the first TN
-    static_assert(kCols % (8 * kWaves) == 0 && kTokens % (8 * kWaves) == 0 && kScaleLanes <= 64 && kBytes <= 160 * 1024, "");
+    static_assert(kCols % (8 * kLoaders) == 0 && kTokens % (8 * kLoaders) == 0 && kScaleLanes <= 64 && kBytes <= 160 * 1024, "");
     static_assert(kCols >= 128 ? (TN * 16) <= 128 : 128 % kCols == 0, "a wavefront's columns share their scales");
 };
 
-template <int TN, int TM, int WN, int WM, int S>
-__global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(const MmParams p)
+template <int TN, int TM, int WN, int WM, int S, int LOADERS>
+__global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(const MmParams p)
 {
-    typedef Tile<TN, TM, WN, WM, S> T;
+    typedef Tile<TN, TM, WN, WM, S, LOADERS> T;
     __shared__ __attribute__((aligned(128))) uint8_t lds[T::kBytes];
     const int tid = threadIdx.x, lane = tid & 63, w = rfl(tid >> 6);
     const int wn = w % WN, wm = w / WN;
+    const int lw = LOADERS > 0 ? w - T::kWaves : w;   // which of the loading wavefronts it is
+    const bool loads = LOADERS == 0 || lw >= 0;
     const int n = lane & 15, q = lane >> 4;
 
     // each XCD gets a run of tiles, in groups of eight tiles of tokens, so that those at work at a time share rows and columns
@@ -314,19 +321,19 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(const MmParams
     const int ld_row = lane >> 3;
 #pragma unroll
     for (int j = 0; j < T::kW; j++) {
-        const int i = w * T::kW + j, r = 8 * (i & 1) + ld_row, k = (i >> 1) % TN;
+        const int i = lw * T::kW + j, r = 8 * (i & 1) + ld_row, k = (i >> 1) % TN;
         int c = (i >> 1) / TN * (TN * 16) + 4 * TN * (r >> 2) + 4 * k + (r & 3);
         c = c0 + c < p.N ? c : p.N - 1 - c0;
         w_off[j] = (unsigned)c * (unsigned)K + 16u * ((lane & 7) ^ ((r >> 1) & 7));
     }
 #pragma unroll
     for (int j = 0; j < T::kX; j++) {
-        const int i = w * T::kX + j, r = 8 * (i & 1) + ld_row;
+        const int i = lw * T::kX + j, r = 8 * (i & 1) + ld_row;
         int m = (i >> 1) * 16 + r;
         m = m0 + m < p.M ? m : p.M - 1 - m0;
         x_off[j] = (unsigned)m * (unsigned)K + 16u * ((lane & 7) ^ ((r >> 1) & 7));
     }
-    const int my_token = w * T::kScaleLanes + (lane < T::kScaleLanes ? lane : 0);
+    const int my_token = lw * T::kScaleLanes + (lane < T::kScaleLanes ? lane : 0);
     const unsigned xs_off = 4u * (unsigned)((m0 + my_token < p.M ? my_token : p.M - 1 - m0) * nkb);
     uint8_t *ws = lds + S * T::kStage;
 
@@ -338,22 +345,40 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(const MmParams
         constexpr int j = decltype(jc)::value;
         uint8_t *at = lds + stage * T::kStage;
         const int limit = kb < nkb ? -1 : 0;
-        if constexpr (j < T::kW) dma16<0>(buffer(w_base, limit), w_off[j], 128u * kb, at + (w * T::kW + j) * 1024);
+        if constexpr (j < T::kW) dma16<0>(buffer(w_base, limit), w_off[j], 128u * kb, at + (lw * T::kW + j) * 1024);
         else if constexpr (j < T::kW + T::kX)
-            dma16<0>(buffer(x_base, limit), x_off[j - T::kW], 128u * kb, at + T::kCols * 128 + (w * T::kX + j - T::kW) * 1024);
+            dma16<0>(buffer(x_base, limit), x_off[j - T::kW], 128u * kb, at + T::kCols * 128 + (lw * T::kX + j - T::kW) * 1024);
         else if (lane < T::kScaleLanes)
-            dma4(buffer(xs_base, limit), xs_off, 4u * kb, at + (T::kCols + T::kTokens) * 128 + w * (T::kScaleLanes * 4));
+            dma4(buffer(xs_base, limit), xs_off, 4u * kb, at + (T::kCols + T::kTokens) * 128 + lw * (T::kScaleLanes * 4));
     };
-    for (int i = w; i < T::kScaleRows * ((nkb + 63) >> 6); i += T::kWaves) {   // the columns' scales of all K blocks
+    for (int i = lw; loads && i < T::kScaleRows * ((nkb + 63) >> 6); i += T::kLoaders) {   // the columns' scales of all K blocks
         const int row = i % T::kScaleRows, c = i / T::kScaleRows * 64;
         const int last = (p.N - 1) >> 7;
         const int block = (c0 >> 7) + row < last ? (c0 >> 7) + row : last;
         if (c + lane < nkb)
             dma4(agent_buffer(p.w_scale + (size_t)block * nkb + c), 4u * lane, 0u, ws + 4 * (row * kMaxKBlocks + c));
     }
+    if constexpr (LOADERS > 0) {
+        if (loads) {
 #pragma unroll
-    for (int i = 0; i < S - 1; i++) for_each<T::kLoads>([&](auto j) { issue(i, i, j); });
-    for_each<T::early()>([&](auto j) { issue(S - 1, S - 1, j); });
+            for (int i = 0; i < S; i++) for_each<T::kLoads>([&](auto j) { issue(i, i, j); });
+            wait_vmcnt<T::kLoads *(S - 1)>();
+            lds_barrier();
+            int stage = 0;
+            for (int kb = 0; kb < nkb; kb++) {
+                wait_vmcnt<T::kLoads *(S - 2)>();   // the next K block's loads have landed
+                lds_barrier();                      // and this one's stage has been read
+                for_each<T::kLoads>([&](auto j) { issue(stage, kb + S, j); });
+                stage = stage + 1 < S ? stage + 1 : 0;
+            }
+            wait_vmcnt<0>();   // (the workgroup's memory is given back)
+            return;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < S - 1; i++) for_each<T::kLoads>([&](auto j) { issue(i, i, j); });
+        for_each<T::early()>([&](auto j) { issue(S - 1, S - 1, j); });
+    }
 
     const int f_n = (n >> 1) & 7;
     const int frag_lo = n * 128 + 16 * (q ^ f_n), frag_hi = n * 128 + 16 * ((q ^ f_n) ^ 4);
@@ -373,7 +398,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(const MmParams
     v4f prod[2] = {};
     float fac[2] = {0.f, 0.f};
     v8i a[TN];
-    wait_vmcnt<T::kLoads *(S - 2) + T::early()>();
+    if constexpr (LOADERS == 0) wait_vmcnt<T::kLoads *(S - 2) + T::early()>();
     lds_barrier();
     aim(0);
     v4i b_lo = x_lo[0], b_hi = x_hi[0];
@@ -394,7 +419,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(const MmParams
                 // The last token tile is in registers: behind the barrier everybody is done with this stage, and its place is
                 // refilled.  The weight tiles are replaced by the next K block's as they are used for the last time.
                 // (Behind the last K block, what is read is not used.)
-                wait_vmcnt<T::kLoads *(S - 2)>();   // the next K block's loads have landed
+                if constexpr (LOADERS == 0) wait_vmcnt<T::kLoads *(S - 2)>();   // the next K block's loads have landed
                 lds_barrier();
                 freed = stage;
                 stage = stage + 1 < S ? stage + 1 : 0;
@@ -418,7 +443,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(const MmParams
                 if constexpr (t + 1 == TM) a[k] = cat(w_lo[k * 128], w_hi[k * 128]);
                 constexpr int slot = t + 1 == TM ? k : TN + j;   // matrix instructions since the barrier
                 for_each<T::kLoads>([&](auto piece) {
-                    if constexpr (T::at(decltype(piece)::value) == slot) issue(freed, t + 1 == TM ? kb + S : kb + S - 1, piece);
+                    if constexpr (LOADERS == 0 && T::at(decltype(piece)::value) == slot) issue(freed, t + 1 == TM ? kb + S : kb + S - 1, piece);
                 });
                 __builtin_amdgcn_sched_barrier(0);
             };
@@ -426,7 +451,7 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(const MmParams
         };
         for_each<TM>(pass);
     }
-    wait_vmcnt<0>();   // (the workgroup's memory is given back)
+    if constexpr (LOADERS == 0) wait_vmcnt<0>();   // (the workgroup's memory is given back)
     static_assert(TN * TM % 2 == 0, "");
     acc[TN - 2][TM - 1] += prod[0] * fac[0];
     acc[TN - 1][TM - 1] += prod[1] * fac[1];
@@ -450,23 +475,25 @@ __global__ __launch_bounds__(WN * WM * 64, 2) void mm_tile_kernel(const MmParams
     }
 }
 
-template <int TN, int TM, int WN, int WM, int S>
+template <int TN, int TM, int WN, int WM, int S, int LOADERS>
 hipError_t launch_tile_mm(MmParams p, hipStream_t stream)
 {
-    typedef Tile<TN, TM, WN, WM, S> T;
+    typedef Tile<TN, TM, WN, WM, S, LOADERS> T;
     p.row_groups = (p.N + T::kCols - 1) / T::kCols;
     p.token_groups = (p.M + T::kTokens - 1) / T::kTokens;
     const int run = (p.row_groups * p.token_groups + 7) / 8;
     void *args[] = {&p};
-    return hipLaunchKernel(reinterpret_cast<const void *>(mm_tile_kernel<TN, TM, WN, WM, S>), dim3((unsigned)run * 8),
-                           dim3(T::kWaves * 64), args, 0, stream);
+    return hipLaunchKernel(reinterpret_cast<const void *>(mm_tile_kernel<TN, TM, WN, WM, S, LOADERS>), dim3((unsigned)run * 8),
+                           dim3((T::kWaves + LOADERS) * 64), args, 0, stream);
 }
 
 // What a call takes.  Few tiles: the largest tile of the streaming kernel of which there are more than half as many as compute
 // units - a smaller one reads more, a larger one leaves the memory idle (MI355X, us, K = 7168; M x N, 32x32 / 64x32 / 64x64 tile:
-// 61 x 2112 8.2 / 11.1 / 16.0, 128 x 4096 14.4 / 11.5 / 16.1, 256 x 4096 25.2 / 20.4 / 16.1).  More: the tile whose rounds
-// take the least time by what a K block of one was measured at, us, with at most one workgroup on a compute unit and with all
-// of them full.
+// 61 x 2112 8.2 / 11.1 / 16.0, 128 x 4096 14.4 / 11.5 / 16.1, 256 x 4096 25.2 / 20.4 / 16.1).  More: the tile whose rounds over the compute
+// units take the least time.  What a round takes for each K block was measured, us: with tiles for half the units, and with as many
+// as run at a time; between the two it is taken in proportion where a unit holds one tile, and as a whole where it holds two.
+// (K = 7168, us, 128x64 / 128x128 / 256x128 / 256x256 tile: 384 x 4096 22.9 / 30.1 / 41.5 / 73.7, 700 x 4096 38.9 / 30.9 / 41.7 / 74.5,
+// 1500 x 4096 64.7 / 63.7 / 48.5 / 75.9, 3000 x 4096 123 / 106 / 98 / 84, 8192 x 2112 187 / 203 / 158 / 172.)
 enum Plan { kStreamHalf1, kStreamHalf2, kStream1x1, kStream2x1, kStream2x2, kStream4x2, kStream4x4, kTile128x64, kTile128x128,
             kTile256x128, kTile256x256 };
 constexpr int kUnits = 256;
@@ -484,16 +511,18 @@ Plan plan(int M, int N)
     static const struct {
         Plan plan;
         int cols, tokens, resident;
-        float one, full;
+        float half, full;
     } kinds[] = {
-        {kStream4x4, 64, 64, 2, 0.24f, 0.46f},       {kTile128x64, 128, 64, 2, 0.42f, 0.74f}, {kTile128x128, 128, 128, 2, 0.75f, 1.15f},
-        {kTile256x128, 256, 128, 1, 0.85f, 1.12f}, {kTile256x256, 256, 256, 1, 1.45f, 1.95f},
+        {kStream4x4, 64, 64, 2, 0.24f, 0.46f},      {kTile128x64, 128, 64, 2, 0.38f, 0.73f},   {kTile128x128, 128, 128, 1, 0.50f, 0.58f},
+        {kTile256x128, 256, 128, 1, 0.70f, 1.03f}, {kTile256x256, 256, 256, 1, 1.28f, 1.88f},
     };
     Plan best = kStream4x4;
     float least = 0.f;
     for (const auto &k : kinds) {
         const int64_t tiles = tiles_of(M, N, k.cols, k.tokens), slots = kUnits * k.resident, rest = tiles % slots;
-        const float time = (float)(tiles / slots) * k.full + (rest == 0 ? 0.f : rest <= slots / 2 ? k.one : k.full);
+        float time = (float)(tiles / slots) * k.full;
+        if (rest > 0 && rest <= slots / 2) time += k.half;
+        else if (rest > 0) time += k.resident > 1 ? k.full : k.half + (k.full - k.half) * (float)(2 * rest - slots) / (float)slots;
         if (k.plan == kStream4x4 || time < least) best = k.plan, least = time;
     }
     return best;
@@ -526,10 +555,10 @@ extern "C" int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale,
     case kStream2x2: err = launch_stream_mm<2, 2, 4, 2, false>(p, hs); break;
     case kStream4x2: err = launch_stream_mm<4, 2, 4, 2, false>(p, hs); break;
     case kStream4x4: err = launch_stream_mm<4, 4, 4, 1, false>(p, hs); break;
-    case kTile128x64: err = launch_tile_mm<4, 2, 2, 2, 3>(p, hs); break;
-    case kTile128x128: err = launch_tile_mm<4, 4, 2, 2, 2>(p, hs); break;
-    case kTile256x128: err = launch_tile_mm<4, 4, 4, 2, 3>(p, hs); break;
-    case kTile256x256: err = launch_tile_mm<4, 8, 4, 2, 2>(p, hs); break;
+    case kTile128x64: err = launch_tile_mm<4, 2, 2, 2, 3, 4>(p, hs); break;
+    case kTile128x128: err = launch_tile_mm<4, 4, 2, 2, 4, 4>(p, hs); break;
+    case kTile256x128: err = launch_tile_mm<4, 4, 4, 2, 3, 4>(p, hs); break;
+    case kTile256x256: err = launch_tile_mm<4, 8, 4, 2, 2, 0>(p, hs); break;
     }
     return err == hipSuccess ? ALPHA_MOE_OK : ALPHA_MOE_ERR_LAUNCH;
 }
