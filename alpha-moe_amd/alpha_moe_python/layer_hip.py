@@ -7,7 +7,8 @@ products of its dense layers.  Callers of the reference take these from their se
 * :func:`swiglu_quant_fp8`   - SwiGLU and quantisation between the two products of a dense layer.
 
 HIP kernels on the current stream of the inputs' device; nothing is kept between calls, so they may be captured into HIP graphs
-and run on several streams at once.  Inputs are contiguous.  Inference only: no gradients.
+and run on several streams at once.  Inputs are contiguous.  Inference only: inputs that require gradients are refused while
+gradients are recorded.
 """
 from typing import NamedTuple, Optional, Tuple
 

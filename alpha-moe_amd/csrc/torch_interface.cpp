@@ -8,6 +8,7 @@
 //   * the device guard is installed before the stream is fetched;
 //   * a refused launch or an unsupported knob raises instead of printing or doing nothing.
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -419,6 +420,13 @@ int is_f32_or_bf16(const at::Tensor &t, const char *name)
     return t.scalar_type() == at::kFloat;
 }
 
+// These operators have no backward pass; a gradient that somebody waits for would be missing without a word.
+void check_inference(const at::Tensor &t, const char *name)
+{
+    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name, " requires a gradient, and this operator has none: call it "
+                "under torch.no_grad() or torch.inference_mode()");
+}
+
 // y = rms_norm(x + residual) * weight quantised as above, and - where they are asked for, otherwise undefined - the sum and y in x's
 // type.
 struct NormQuant {
@@ -438,7 +446,9 @@ NormQuant run_norm(const at::Tensor &x, const at::Tensor *residual, const at::Te
     TORCH_CHECK(M <= INT32_MAX, "too many rows");
     check_tensor(weight, "weight", weight.scalar_type(), dev);
     TORCH_CHECK(weight.dim() == 1 && weight.size(0) == K, "weight must be [K]");
+    check_inference(x, "x"), check_inference(weight, "weight");
     if (residual) {
+        check_inference(*residual, "residual");
         check_tensor(*residual, "residual", x.scalar_type(), dev);
         TORCH_CHECK(residual->sizes() == x.sizes(), "residual must have the shape of x");
     }
@@ -492,6 +502,7 @@ std::tuple<at::Tensor, at::Tensor> swiglu_quant_fp8(const at::Tensor &gate_up, i
     const int is_f32 = is_f32_or_bf16(gate_up, "gate_up");
     check_tensor(gate_up, "gate_up", gate_up.scalar_type(), dev);
     TORCH_CHECK(gate_up.dim() == 2 && gate_up.size(1) > 0 && gate_up.size(1) % 256 == 0, "gate_up must be [M, 2 I] with I % 128 == 0");
+    check_inference(gate_up, "gate_up");
     const int64_t M = gate_up.size(0), I = gate_up.size(1) / 2;
     TORCH_CHECK(M <= INT32_MAX && I <= INT32_MAX / 2, "sizes exceed int32");
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
@@ -522,6 +533,7 @@ at::Tensor block_scaled_mm(const at::Tensor &x, const at::Tensor &x_scale, const
     TORCH_CHECK(x_scale.dim() == 2 && x_scale.size(0) == M && x_scale.size(1) == K / 128, "x_scale must be [M, K/128]");
     TORCH_CHECK(w_scale.dim() == 2 && w_scale.size(0) == (N + 127) / 128 && w_scale.size(1) == K / 128,
                 "w_scale must be [ceil(N/128), K/128]");
+    check_inference(x_scale, "x_scale"), check_inference(w_scale, "w_scale");
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
     at::Tensor out = empty_on(dev, {M, N}, at::kBFloat16);
@@ -549,7 +561,9 @@ std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor &logits, const c1
     if (bias.has_value()) {
         check_tensor(*bias, "bias", at::kFloat, dev);
         TORCH_CHECK(bias->dim() == 1 && bias->size(0) == E, "bias must be [E]");
+        check_inference(*bias, "bias");
     }
+    check_inference(logits, "logits");
     TORCH_CHECK(top_k > 0 && top_k <= 64 && top_k <= E, "top_k must be in [1, min(E, 64)]");
     TORCH_CHECK(num_groups > 0 && num_groups <= 64 && E % num_groups == 0, "num_groups must divide the experts, at most 64");
     TORCH_CHECK(top_groups > 0 && top_groups <= num_groups, "top_groups must be in [1, num_groups]");

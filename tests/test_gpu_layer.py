@@ -535,3 +535,24 @@ def test_refusals():
         with pytest.raises((RuntimeError, ValueError, NotImplementedError)):
             call()
             print(f"refusal {i} went through", flush=True)
+
+
+def test_inputs_that_require_gradients_are_refused():
+    from alpha_moe_python import layer_hip as H
+    x = torch.zeros((4, 256), dtype=torch.bfloat16, device=DEV)
+    w = torch.nn.Parameter(torch.ones(256, device=DEV))
+    leaf = torch.zeros((4, 256), dtype=torch.bfloat16, device=DEV, requires_grad=True)
+    logits = torch.zeros((4, 64), device=DEV, requires_grad=True)
+    bias = torch.zeros(64, device=DEV, requires_grad=True)
+    q, s, mw, ms = (t.to(DEV) for t in mm_problem(4, 100, 256, 0))
+    calls = [lambda: H.rms_norm_quant_fp8(x, w), lambda: H.rms_norm_quant_fp8(leaf, w.detach()),
+             lambda: H.rms_norm_quant_fp8(x, w.detach(), residual=leaf), lambda: H.swiglu_quant_fp8(leaf),
+             lambda: H.block_scaled_mm(q, s.requires_grad_(), mw, ms), lambda: H.route_topk(logits, 4),
+             lambda: H.route_topk(logits.detach(), 4, bias=bias)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            call()
+        with torch.no_grad():
+            call()
+        with torch.inference_mode():
+            call()
