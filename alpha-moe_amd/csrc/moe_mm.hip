@@ -31,6 +31,7 @@ struct MmParams {
     uint16_t *out;
     int M, N, K, nkb;
     int row_groups, token_groups;   // tiles of the launch
+    int quads;   // 1: a token's scales of four K blocks start at a multiple of 16 bytes, and are loaded together
 };
 
 __device__ __forceinline__ int rfl(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -71,6 +72,25 @@ __device__ __forceinline__ lds_v4i lds_tile(const void *p) { return (lds_v4i)(ui
 __device__ __forceinline__ v4i lds_read(const void *p) { return *lds_tile(p); }
 __device__ __forceinline__ float lds_float(const void *p) { return *(lds_f32)(uint32_t)(uintptr_t)p; }
 
+// The scales of a tile's tokens in LDS, loaded four K blocks at a time where they can be (one by one, every scale is a line of its own
+// on the path into the compute unit, half as many again as the data is; 8192 x 4096 x 7168 221 us, by fours 207; 2048 x 4096 x 7168 57.0
+// and 56.0): two places of [token][K block & 3], or eight of [token].
+struct TokenScales {
+    int quads, tokens;
+    __device__ __forceinline__ bool loads(int kb, bool first) const { return !quads || first || (kb & 3) == 0; }
+    __device__ __forceinline__ int place(int kb) const { return quads ? ((kb >> 2) & 1) * tokens * 16 + (kb & 3) * 4 : (kb & 7) * tokens * 4; }
+    __device__ __forceinline__ int stride() const { return quads ? 16 : 4; }   // from token to token
+    // lanes [0, count) load the scales of as many tokens, from `token` on, that K block kb is the first to ask for
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t base, unsigned offset, int kb, int token, bool mine, uint8_t *area) const
+    {
+        if (quads) {
+            if (mine) dma16<0>(base, offset, 4u * (unsigned)(kb & ~3), area + place(kb & ~3) + token * 16);
+        } else {
+            if (mine) dma4(base, offset, 4u * (unsigned)kb, area + place(kb) + token * 4);
+        }
+    }
+};
+
 // Columns n .. n + 3 of row m; what is behind the last row or column is not there.
 __device__ __forceinline__ void store4(const MmParams &p, int m, int n, v4f v)
 {
@@ -93,18 +113,19 @@ __device__ __forceinline__ void store4(const MmParams &p, int m, int n, v4f v)
 // column's result depends on its own token alone, and theirs are not stored.
 //
 // What bounds it: the weights' way from memory at few tokens, the path into a compute unit (128 bytes times rows plus tokens per K
-// block, 70 - 100 GB/s) from some thirty on.  MI355X, back to back: 1 x 4096 x 7168 (29 MB) 6.1 us, of which 2.5 are an
-// empty call's, 61 x 2112 x 7168 8.1, 64 x 7168 x 2048 5.9, 256 x 4096 x 7168 16.1.  Why not the contraction split over workgroups: the
+// block, 70 - 100 GB/s) from some thirty on.  MI355X, back to back: 1 x 4096 x 7168 (29 MB) 6.0 us, of which 2.5 are an
+// empty call's, 61 x 2112 x 7168 8.3, 64 x 7168 x 2048 6.0, 256 x 4096 x 7168 15.  Why not the contraction split over workgroups: the
 // partial sums' second launch costs 3 - 4 us, more than the idle compute units it fills (61 x 2112 x 7168 in seven parts 11.6 us).
 // Weights are loaded non-temporally only with at most eight tokens, where they are read once and there is little else to read
 // (1 x 4096 x 7168 from HBM 6.7 us against 7.5, from the last-level cache 6.4 and 6.6; but 61 x 2112 x 7168 11.9 and 8.3).
 // Deeper rings change nothing (16 x 4096 x 7168 with two, four K blocks 7.0, 7.05 us).
 template <int R, int T, int WAVES, int D, bool HALF>
 struct StreamRing {
-    static constexpr int kSlot = (R + T) * 2048 + 256;
+    static constexpr bool kRun = T >= 4;   // the tokens' scales four K blocks at a time
+    static constexpr int kSlot = (R + T) * 2048 + (kRun ? 0 : 256);
     static constexpr int kScales = 4 * (kMaxKBlocks / WAVES);   // bytes: the weights' scales of a wavefront's K blocks
-    static constexpr int kLoads = 2 * R + (HALF ? 1 : 2 * T) + 1;   // of a slot
-    static constexpr int kWave = D * kSlot + kScales;
+    static constexpr int kData = 2 * R + (HALF ? 1 : 2 * T), kLoads = kData + 1;   // loads of a slot without, with tokens' scales
+    static constexpr int kWave = D * kSlot + kScales + (kRun ? T * 512 : 0);
     static constexpr bool kSpread = R * T <= 8;   // the refill's loads between the matrix instructions, or in front of them
     static constexpr int kSums = WAVES * R * T * 1024;              // the sums at the end take the rings' place
     static constexpr int kBytes = WAVES * kWave > kSums ? WAVES * kWave : kSums;
@@ -115,7 +136,7 @@ template <int R, int T, int WAVES, int D, bool HALF>
 __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(const MmParams p)
 {
     typedef StreamRing<R, T, WAVES, D, HALF> Ring;
-    constexpr int L = Ring::kLoads;
+    constexpr int L = Ring::kLoads, DATA = Ring::kData;
     __shared__ __attribute__((aligned(128))) uint8_t lds[Ring::kBytes];
     const int tid = threadIdx.x, lane = tid & 63, w = rfl(tid >> 6);
     const int n = lane & 15, q = lane >> 4;
@@ -127,7 +148,13 @@ __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(const MmParams p)
     const int rg = tile / p.token_groups, tg = tile - rg * p.token_groups;
     const int c0 = rg * (R * 16), m0 = tg * (T * 16);
     const int K = p.K, nkb = p.nkb;
-    const int count = w < nkb ? (nkb - w + WAVES - 1) / WAVES : 0;   // this wavefront's K blocks: w, w + WAVES, ...
+    // This wavefront's K blocks: every WAVES-th one, so that a workgroup reads on along its rows; with four tiles of tokens a run of
+    // them, for the sake of the tokens' scales.  61 tokens, 2112 columns, K = 7168: with four tiles 14.4 us as a run against 16.5 in turn,
+    // with two of 32 columns 8.7 against 8.3; one token, 4096 columns: 6.2 against 6.0.
+    constexpr bool RUN = Ring::kRun;
+    constexpr int STEP = RUN ? 1 : WAVES;
+    const int first = RUN ? w * nkb / WAVES : w;
+    const int count = RUN ? (w + 1) * nkb / WAVES - first : w < nkb ? (nkb - w + WAVES - 1) / WAVES : 0;
 
     const __amdgpu_buffer_rsrc_t wbuf = agent_buffer(p.w + (size_t)c0 * K);
     const __amdgpu_buffer_rsrc_t xbuf = agent_buffer(p.x + (size_t)m0 * K);
@@ -157,18 +184,22 @@ __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(const MmParams p)
     const unsigned xs_off = 4u * (unsigned)((m0 + lane < p.M ? lane : p.M - 1 - m0) * nkb);
 
     uint8_t *ring = lds + w * Ring::kWave;
-    uint8_t *ws = ring + D * Ring::kSlot;
+    uint8_t *ws = ring + D * Ring::kSlot, *xs = ws + Ring::kScales;
+    const TokenScales scales = {p.quads, T * 16};   // (RUN)
     for (int c = 0; c < count; c += 64)
-        if (c + lane < count) dma4(wsbuf, 4u * (unsigned)(w + (c + lane) * WAVES), 0u, ws + 4 * c);
-    // Load j of a slot for the i-th of this wavefront's K blocks: weights, scales of the tokens, tokens.
+        if (c + lane < count) dma4(wsbuf, 4u * (unsigned)(first + (c + lane) * STEP), 0u, ws + 4 * c);
+    // Load j of a slot for the i-th of this wavefront's K blocks: weights and tokens, the tokens' scales between them, or in front of
+    // both where there are not always any.
     auto issue = [&](int slot, int i, auto jc) {
-        constexpr int j = decltype(jc)::value, tj = j - 2 * R - 1;
-        const int kb = w + i * WAVES;
+        constexpr int at_scales = RUN ? 0 : 2 * R, at_j = decltype(jc)::value;
+        constexpr int j = at_j == at_scales ? -1 : at_j > at_scales ? at_j - 1 : at_j, tj = j - 2 * R;
+        const int kb = first + i * STEP;
         uint8_t *at = ring + slot * Ring::kSlot;
-        if constexpr (j < 2 * R) {
+        if constexpr (j < 0) {
+            if (!RUN && lane < T * 16) dma4(xsbuf, xs_off, 4u * (unsigned)kb, at + (R + T) * 2048);
+            if (RUN && scales.loads(kb, i == 0)) scales.load(xsbuf, xs_off, kb, 0, lane < T * 16, xs);
+        } else if constexpr (j < 2 * R) {
             dma16<HALF ? 2 : 0>(wbuf, w_off[j / 2][j % 2], 128u * kb, at + j * 1024);
-        } else if constexpr (j == 2 * R) {
-            if (lane < T * 16) dma4(xsbuf, xs_off, 4u * kb, at + (R + T) * 2048);
         } else {
             constexpr int t = HALF ? tj : tj / 2, h = HALF ? 0 : tj % 2;
             dma16<0>(xbuf, x_off[t][h], 128u * kb, at + (R + t) * 2048 + h * 1024);
@@ -183,13 +214,13 @@ __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(const MmParams p)
     v4f acc[R][T] = {};
     int slot = 0;
     for (int i = 0; i < count; i++) {
-        // of what was issued behind this K block all may still be on its way
-        const int behind = count - 1 - i;
-        if (behind >= D - 1) wait_vmcnt<L * (D - 1)>();
-        else if (D > 2 && behind == D - 2) wait_vmcnt<L * (D > 2 ? D - 2 : 0)>();
-        else if (D > 3 && behind == D - 3) wait_vmcnt<L * (D > 3 ? D - 3 : 0)>();
+        // of what was issued behind this K block, all may still be on its way (with a run, at least the data)
+        static_assert(D <= 2, "the last K blocks are waited for as if there were nothing behind them");
+        if (i + D <= count) wait_vmcnt<(RUN ? DATA : L) * (D - 1)>();
         else wait_vmcnt<0>();
         const uint8_t *at = ring + slot * Ring::kSlot;
+        const uint8_t *my_xs = RUN ? xs + scales.place(first + i) : at + (R + T) * 2048;
+        const int xs_token = RUN ? scales.stride() : 4;
         v8i a[R], b[T];
         float f[T];
 #pragma unroll
@@ -197,7 +228,7 @@ __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(const MmParams p)
 #pragma unroll
         for (int t = 0; t < T; t++) {
             b[t] = cat(lds_read(at + (R + t) * 2048 + frag_lo), lds_read(at + (R + t) * 2048 + frag_hi));
-            f[t] = lds_float(at + (R + T) * 2048 + 4 * (16 * t + n));
+            f[t] = lds_float(my_xs + xs_token * (16 * t + n));
         }
         const float sc = lds_float(ws + 4 * i);
 #pragma unroll
@@ -268,28 +299,28 @@ hipError_t launch_stream_mm(MmParams p, hipStream_t stream)
 //
 // The loads: a wavefront that hands loads to the path into the compute unit (64 bytes a cycle) waits for it, and its matrix
 // instructions with it.  Where registers allow, LOADERS more wavefronts do nothing but load (128 x 128 tile, 1024 x 4096 x 7168 43.5 ->
-// 35.8 us, 128 x 64, 256 x 7168 x 2048 9.9 -> 9.4).  The 256 x 256 tile has no registers left for them: there the loads of a stage go
+// 35.8 us, 128 x 64, 256 x 7168 x 2048 9.9 -> 9.3).  The 256 x 256 tile has no registers left for them: there the loads of a stage go
 // out one by one between matrix instructions, over the first three eighths of a K block (8192 x 4096 x 7168 in a burst 226, over three
-// eighths 221, over all of it 231).
+// eighths 221, over all of it 231; with the tokens' scales four K blocks at a time then 207).
 //
 // What bounds it: matrix instructions and their scaling multiply-adds (19.3 ns a pair on random operands, where the clock gives way:
 // 138 us for 8192 x 4096 x 7168; on equal operands 14.8), and LDS, which takes loads in at 64 bytes a cycle while fragments are
-// read from it (without any loads the same kernel takes 137 us).  MI355X: 8192 x 4096 x 7168 221 us (2.18 PFLOP/s; a library product of
-// the same size without block scales 188), 4096 x 4096 x 7168 105, 1024 x 7168 x 2048 20.5, 256 x 7168 x 2048 9.4.  Also
-// tried: 128 columns x 64 tokens a wavefront 237; token fragments read two passes ahead 228; all fragments read behind the barrier 239.
+// read from it (without any loads the same kernel takes 137 us).  MI355X: 8192 x 4096 x 7168 207 us (2.33 PFLOP/s; a library product of
+// the same size without block scales 188), 4096 x 4096 x 7168 99, 1024 x 7168 x 2048 18.7, 256 x 7168 x 2048 9.4.  Also
+// tried, against 221: 128 columns x 64 tokens a wavefront 237; token fragments read two passes ahead 228; all fragments read behind the barrier 239.
 template <int TN, int TM, int WN, int WM, int S, int LOADERS>
 struct Tile {
     static constexpr int kWaves = WN * WM, kLoaders = LOADERS > 0 ? LOADERS : kWaves, kCols = TN * 16 * WN, kTokens = TM * 16 * WM;
-    static constexpr int kStage = (kCols + kTokens) * 128 + kTokens * 4;
+    static constexpr int kStage = (kCols + kTokens) * 128;
     static constexpr int kScaleRows = (kCols + 127) / 128;   // a tile starts at a multiple of its columns
-    static constexpr int kBytes = S * kStage + kScaleRows * kMaxKBlocks * 4;
+    static constexpr int kBytes = S * kStage + kTokens * 32 + kScaleRows * kMaxKBlocks * 4;
     static constexpr int kW = kCols / 8 / kLoaders, kX = kTokens / 8 / kLoaders;   // 1 KiB pieces a loading wavefront has per stage
-    static constexpr int kLoads = kW + kX + 1;   // of a wavefront and stage; the last: its share of the tokens' scales
+    static constexpr int kData = kW + kX, kLoads = kData + 1;   // of a wavefront and stage, the first: its share of the tokens' scales, if any
     static constexpr int kScaleLanes = kTokens / kLoaders;
     // Piece j of a stage is issued behind matrix instruction at(j) of the TN * TM that follow the barrier which frees its place.
     static constexpr int at(int j) { return j * (S == 2 ? TN * TM * 3 / 8 : TN * TM) / kLoads; }
     static constexpr int early() { int c = 0; while (c < kLoads && at(c) < TN) c++; return c; }   // those in the first TN
-    static_assert(kCols % (8 * kLoaders) == 0 && kTokens % (8 * kLoaders) == 0 && kScaleLanes <= 64 && kBytes <= 160 * 1024, "");
+    static_assert(kCols % (8 * kLoaders) == 0 && kTokens % (8 * kLoaders) == 0 && kScaleLanes <= 64 && S <= 4 && kBytes <= 160 * 1024, "");
     static_assert(kCols >= 128 ? (TN * 16) <= 128 : 128 % kCols == 0, "a wavefront's columns share their scales");
 };
 
@@ -335,21 +366,21 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(co
     }
     const int my_token = lw * T::kScaleLanes + (lane < T::kScaleLanes ? lane : 0);
     const unsigned xs_off = 4u * (unsigned)((m0 + my_token < p.M ? my_token : p.M - 1 - m0) * nkb);
-    uint8_t *ws = lds + S * T::kStage;
+    uint8_t *xs = lds + S * T::kStage, *ws = xs + T::kTokens * 32;
+    const TokenScales scales = {p.quads, T::kTokens};
 
     // (a tile's offsets are below 2^25: rows of up to 64 KiB)
     const uint8_t *w_base = p.w + (size_t)c0 * K, *x_base = p.x + (size_t)m0 * K;
     const float *xs_base = p.x_scale + (size_t)m0 * nkb;
     // Load j of a stage.  Behind the last K block nothing is loaded, but the loads are still counted.
     auto issue = [&](int stage, int kb, auto jc) {
-        constexpr int j = decltype(jc)::value;
+        constexpr int j = decltype(jc)::value - 1;
         uint8_t *at = lds + stage * T::kStage;
         const int limit = kb < nkb ? -1 : 0;
-        if constexpr (j < T::kW) dma16<0>(buffer(w_base, limit), w_off[j], 128u * kb, at + (lw * T::kW + j) * 1024);
-        else if constexpr (j < T::kW + T::kX)
-            dma16<0>(buffer(x_base, limit), x_off[j - T::kW], 128u * kb, at + T::kCols * 128 + (lw * T::kX + j - T::kW) * 1024);
-        else if (lane < T::kScaleLanes)
-            dma4(buffer(xs_base, limit), xs_off, 4u * kb, at + (T::kCols + T::kTokens) * 128 + lw * (T::kScaleLanes * 4));
+        if constexpr (j < 0) {
+            if (scales.loads(kb, false)) scales.load(buffer(xs_base, limit), xs_off, kb, lw * T::kScaleLanes, lane < T::kScaleLanes, xs);
+        } else if constexpr (j < T::kW) dma16<0>(buffer(w_base, limit), w_off[j], 128u * kb, at + (lw * T::kW + j) * 1024);
+        else dma16<0>(buffer(x_base, limit), x_off[j - T::kW], 128u * kb, at + T::kCols * 128 + (lw * T::kX + j - T::kW) * 1024);
     };
     for (int i = lw; loads && i < T::kScaleRows * ((nkb + 63) >> 6); i += T::kLoaders) {   // the columns' scales of all K blocks
         const int row = i % T::kScaleRows, c = i / T::kScaleRows * 64;
@@ -362,12 +393,12 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(co
         if (loads) {
 #pragma unroll
             for (int i = 0; i < S; i++) for_each<T::kLoads>([&](auto j) { issue(i, i, j); });
-            wait_vmcnt<T::kLoads *(S - 1)>();
+            wait_vmcnt<T::kData *(S - 1)>();
             lds_barrier();
             int stage = 0;
             for (int kb = 0; kb < nkb; kb++) {
-                wait_vmcnt<T::kLoads *(S - 2)>();   // the next K block's loads have landed
-                lds_barrier();                      // and this one's stage has been read
+                wait_vmcnt<T::kData *(S - 2)>();   // the next K block's loads have landed
+                lds_barrier();                     // and this one's stage has been read
                 for_each<T::kLoads>([&](auto j) { issue(stage, kb + S, j); });
                 stage = stage + 1 < S ? stage + 1 : 0;
             }
@@ -384,25 +415,26 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(co
     const int frag_lo = n * 128 + 16 * (q ^ f_n), frag_hi = n * 128 + 16 * ((q ^ f_n) ^ 4);
     const uint8_t *my_ws = ws + 4 * kMaxKBlocks * ((wn * TN * 16) >> 7);
     lds_v4i w_lo, w_hi, x_lo, x_hi;   // this wavefront's part of a stage
-    lds_f32 xs;
-    auto aim = [&](int stage) {
+    const uint8_t *my_xs;
+    const int xs_row = (wm * TM * 16 + n) * scales.stride(), xs_tile = 16 * scales.stride();
+    auto aim = [&](int stage, int kb) {
         const uint8_t *at = lds + stage * T::kStage;
         w_lo = lds_tile(at + wn * TN * 2048 + frag_lo);
         w_hi = lds_tile(at + wn * TN * 2048 + frag_hi);
         x_lo = lds_tile(at + T::kCols * 128 + wm * TM * 2048 + frag_lo);
         x_hi = lds_tile(at + T::kCols * 128 + wm * TM * 2048 + frag_hi);
-        xs = (lds_f32)(uint32_t)(uintptr_t)(at + (T::kCols + T::kTokens) * 128 + 4 * (wm * TM * 16 + n));
+        my_xs = xs + scales.place(kb) + xs_row;
     };
     v4f acc[TN][TM] = {};
     // A product is scaled into its accumulator two matrix instructions after its own, so no wait states stand between the two.
     v4f prod[2] = {};
     float fac[2] = {0.f, 0.f};
     v8i a[TN];
-    if constexpr (LOADERS == 0) wait_vmcnt<T::kLoads *(S - 2) + T::early()>();
+    if constexpr (LOADERS == 0) wait_vmcnt<T::kData *(S - 2) + T::early() - 1>();
     lds_barrier();
-    aim(0);
+    aim(0, 0);
     v4i b_lo = x_lo[0], b_hi = x_hi[0];
-    float f = xs[0], sc = lds_float(my_ws);
+    float f = lds_float(my_xs), sc = lds_float(my_ws);
 #pragma unroll
     for (int k = 0; k < TN; k++) a[k] = cat(w_lo[k * 128], w_hi[k * 128]);
     int stage = 0, freed = S - 1;   // freed: the stage whose loads are being issued, for K block kb + S - 1, then kb + S
@@ -414,19 +446,19 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(co
             if constexpr (t + 1 < TM) {
                 b_lo = x_lo[(t + 1) * 128];
                 b_hi = x_hi[(t + 1) * 128];
-                f = xs[16 * (t + 1)];
+                f = lds_float(my_xs + (t + 1) * xs_tile);
             } else {
                 // The last token tile is in registers: behind the barrier everybody is done with this stage, and its place is
                 // refilled.  The weight tiles are replaced by the next K block's as they are used for the last time.
                 // (Behind the last K block, what is read is not used.)
-                if constexpr (LOADERS == 0) wait_vmcnt<T::kLoads *(S - 2)>();   // the next K block's loads have landed
+                if constexpr (LOADERS == 0) wait_vmcnt<T::kData *(S - 2)>();   // the next K block's loads have landed
                 lds_barrier();
                 freed = stage;
                 stage = stage + 1 < S ? stage + 1 : 0;
-                aim(stage);
+                aim(stage, kb + 1);
                 b_lo = x_lo[0];
                 b_hi = x_hi[0];
-                f = xs[0];
+                f = lds_float(my_xs);
                 sc = lds_float(my_ws + 4 * (kb + 1 < nkb ? kb + 1 : kb));
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -489,11 +521,11 @@ hipError_t launch_tile_mm(MmParams p, hipStream_t stream)
 
 // What a call takes.  Few tiles: the largest tile of the streaming kernel of which there are more than half as many as compute
 // units - a smaller one reads more, a larger one leaves the memory idle (MI355X, us, K = 7168; M x N, 32x32 / 64x32 / 64x64 tile:
-// 61 x 2112 8.2 / 11.1 / 16.0, 128 x 4096 14.4 / 11.5 / 16.1, 256 x 4096 25.2 / 20.4 / 16.1).  More: the tile whose rounds over the compute
+// 61 x 2112 8.4 / 11.3 / 14.5, 128 x 4096 14.3 / 11.6 / 14.6, 192 x 4096 19.2 / 20.9 / 14.6).  More: the tile whose rounds over the compute
 // units take the least time.  What a round takes for each K block was measured, us: with tiles for half the units, and with as many
 // as run at a time; between the two it is taken in proportion where a unit holds one tile, and as a whole where it holds two.
-// (K = 7168, us, 128x64 / 128x128 / 256x128 / 256x256 tile: 384 x 4096 22.9 / 30.1 / 41.5 / 73.7, 700 x 4096 38.9 / 30.9 / 41.7 / 74.5,
-// 1500 x 4096 64.7 / 63.7 / 48.5 / 75.9, 3000 x 4096 123 / 106 / 98 / 84, 8192 x 2112 187 / 203 / 158 / 172.)
+// (K = 7168, us, 128x64 / 128x128 / 256x128 / 256x256 tile: 384 x 4096 22.7 / 30.2 / 41.1 / 77, 700 x 4096 34.6 / 30.8 / 41.6 / 78,
+// 1500 x 4096 57 / 61 / 46 / 79, 3000 x 4096 109 / 98 / 92 / 83, 8192 x 2112 168 / 166 / 145 / 172.)
 enum Plan { kStreamHalf1, kStreamHalf2, kStream1x1, kStream2x1, kStream2x2, kStream4x2, kStream4x4, kTile128x64, kTile128x128,
             kTile256x128, kTile256x256 };
 constexpr int kUnits = 256;
@@ -513,8 +545,8 @@ Plan plan(int M, int N)
         int cols, tokens, resident;
         float half, full;
     } kinds[] = {
-        {kStream4x4, 64, 64, 2, 0.24f, 0.46f},      {kTile128x64, 128, 64, 2, 0.38f, 0.73f},   {kTile128x128, 128, 128, 1, 0.50f, 0.58f},
-        {kTile256x128, 256, 128, 1, 0.70f, 1.03f}, {kTile256x256, 256, 256, 1, 1.28f, 1.88f},
+        {kStream4x4, 64, 64, 2, 0.23f, 0.43f},      {kTile128x64, 128, 64, 2, 0.38f, 0.67f},   {kTile128x128, 128, 128, 1, 0.50f, 0.59f},
+        {kTile256x128, 256, 128, 1, 0.70f, 0.97f}, {kTile256x256, 256, 256, 1, 1.36f, 1.80f},
     };
     Plan best = kStream4x4;
     float least = 0.f;
@@ -545,6 +577,7 @@ extern "C" int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale,
     MmParams p = {};
     p.x = x, p.x_scale = x_scale, p.w = w, p.w_scale = w_scale, p.out = out;
     p.M = M, p.N = N, p.K = K, p.nkb = K / 128;
+    p.quads = p.nkb % 4 == 0 && (reinterpret_cast<uintptr_t>(x_scale) & 15) == 0;
     hipStream_t hs = static_cast<hipStream_t>(stream);
     hipError_t err = hipErrorInvalidValue;
     switch (plan(M, N)) {

@@ -216,6 +216,22 @@ def test_mm_puts_every_element_and_scale_in_its_place(M, N, K):
     assert torch.equal(want.float().double(), want) and torch.equal(out.cpu(), want.float().to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 300, 2048), (61, 520, 2048), (200, 4200, 2048), (260, 7200, 1024), (700, 4100, 1024), (1500, 4100, 1024),
+                                   (4090, 4088, 2048)])
+def test_mm_with_scales_at_any_multiple_of_four_bytes(M, N, K):
+    """how the tokens' scales are loaded depends on where they lie; which sums are made, and their order, does not"""
+    from alpha_moe_python import layer_hip
+    print(f"case mm scales M={M} N={N} K={K}", flush=True)
+    x, xs, w, ws = [t.to(DEV) for t in mm_problem(M, N, K, M + N + K)]
+    want = layer_hip.block_scaled_mm(x, xs, w, ws)
+    for shift in (1, 2, 3):
+        store = torch.full((xs.numel() + 8,), float("nan"), device=DEV)
+        moved = store[shift:shift + xs.numel()].view_as(xs)
+        moved.copy_(xs)
+        assert moved.data_ptr() % 16 == 4 * shift
+        assert torch.equal(layer_hip.block_scaled_mm(x, moved, w, ws), want)
+
+
 @pytest.mark.parametrize("M", [1, 40, 300, 9000, 40000])
 def test_mm_keeps_what_is_not_a_number(M):
     from alpha_moe_python import layer_hip
