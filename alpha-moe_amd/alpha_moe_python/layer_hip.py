@@ -40,8 +40,8 @@ def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
 
     x ``[M, K]`` bf16 or fp32, K a multiple of 128 up to 65536; weight ``[K]`` bf16 or fp32; residual None or like x.  Returns
     ``q [M, K]`` float8_e4m3fn and ``scale [M, K/128]`` float32 of ``y`` (as ``per_token_group_quant_fp8`` defines them, but NaN
-    in a group that holds one), ``residual`` = ``h`` in x's dtype (a new tensor), and with ``keep_norm`` ``norm`` = ``y`` in x's
-    dtype, which a router or a bf16 product reads.
+    in a group that holds one; a row whose squares add up to more than fp32 holds becomes 0), ``residual`` = ``h`` in x's
+    dtype (a new tensor), and with ``keep_norm`` ``norm`` = ``y`` in x's dtype, which a router or a bf16 product reads.
     """
     if residual is None:
         if not keep_norm:
@@ -63,7 +63,7 @@ def block_scaled_mm(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_s
     """``out [M, N] = (x * x_scale) (w * w_scale)^T``, rounded once to bfloat16.
 
     x ``[M, K]`` float8_e4m3fn with x_scale ``[M, K/128]``; w ``[N, K]`` float8_e4m3fn with w_scale ``[ceil(N/128), K/128]``.
-    N is of any size, K a multiple of 128 up to 65536.  Bit for bit the same from run to run.
+    N is of any size, K a multiple of 128 up to 65536 (a multiple of 512 is loaded with fewer instructions).  Bit for bit the same from run to run.
     """
     return _block_scaled_mm(x, x_scale, w, w_scale)
 

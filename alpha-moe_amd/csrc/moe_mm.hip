@@ -279,9 +279,18 @@ __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(const MmParams p)
     }
 }
 
+int64_t tiles_of(int M, int N, int cols, int tokens)
+{
+    return (int64_t)((N + cols - 1) / cols) * ((M + tokens - 1) / tokens);
+}
+
+// A launch has less than 2^32 threads.
+bool grid_fits(int64_t tiles, int threads) { return (tiles + 7) * threads < (int64_t(1) << 32); }
+
 template <int R, int T, int WAVES, int D, bool HALF>
 hipError_t launch_stream_mm(MmParams p, hipStream_t stream)
 {
+    if (!grid_fits(tiles_of(p.M, p.N, R * 16, T * 16), WAVES * 64)) return hipErrorInvalidConfiguration;
     p.row_groups = (p.N + R * 16 - 1) / (R * 16);
     p.token_groups = (p.M + T * 16 - 1) / (T * 16);
     const int run = (p.row_groups * p.token_groups + 7) / 8;
@@ -511,6 +520,7 @@ template <int TN, int TM, int WN, int WM, int S, int LOADERS>
 hipError_t launch_tile_mm(MmParams p, hipStream_t stream)
 {
     typedef Tile<TN, TM, WN, WM, S, LOADERS> T;
+    if (!grid_fits(tiles_of(p.M, p.N, T::kCols, T::kTokens), (T::kWaves + LOADERS) * 64)) return hipErrorInvalidConfiguration;
     p.row_groups = (p.N + T::kCols - 1) / T::kCols;
     p.token_groups = (p.M + T::kTokens - 1) / T::kTokens;
     const int run = (p.row_groups * p.token_groups + 7) / 8;
@@ -529,11 +539,6 @@ hipError_t launch_tile_mm(MmParams p, hipStream_t stream)
 enum Plan { kStreamHalf1, kStreamHalf2, kStream1x1, kStream2x1, kStream2x2, kStream4x2, kStream4x4, kTile128x64, kTile128x128,
             kTile256x128, kTile256x256 };
 constexpr int kUnits = 256;
-
-int64_t tiles_of(int M, int N, int cols, int tokens)
-{
-    return (int64_t)((N + cols - 1) / cols) * ((M + tokens - 1) / tokens);
-}
 
 Plan plan(int M, int N)
 {
@@ -570,7 +575,6 @@ extern "C" int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale,
     if (M < 0 || N <= 0 || K <= 0 || K % 128 != 0 || K > 128 * kMaxKBlocks || M > INT32_MAX - 255 || N > INT32_MAX - 255)
         return ALPHA_MOE_ERR_SHAPE;
     if (M == 0) return ALPHA_MOE_OK;
-    if (tiles_of(M, N, 256, 256) > (1 << 22)) return ALPHA_MOE_ERR_SHAPE;   // (half a terabyte of results)
     if (!x || !x_scale || !w || !w_scale || !out) return ALPHA_MOE_ERR_NULL_POINTER;
     if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
         return ALPHA_MOE_ERR_ALIGNMENT;
@@ -593,5 +597,5 @@ extern "C" int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale,
     case kTile256x128: err = launch_tile_mm<4, 4, 4, 2, 3, 4>(p, hs); break;
     case kTile256x256: err = launch_tile_mm<4, 8, 4, 2, 2, 0>(p, hs); break;
     }
-    return err == hipSuccess ? ALPHA_MOE_OK : ALPHA_MOE_ERR_LAUNCH;
+    return err == hipSuccess ? ALPHA_MOE_OK : err == hipErrorInvalidConfiguration ? ALPHA_MOE_ERR_SHAPE : ALPHA_MOE_ERR_LAUNCH;
 }

@@ -246,7 +246,7 @@ extern "C" int alpha_moe_rms_norm_quant_fp8(const void *x, const void *residual,
                                             void *norm_out, int M, int K, void *stream)
 {
     using namespace alpha_moe;
-    if (M < 0 || K <= 0 || K % 128 != 0 || K > 128 * kMaxKBlocks) return ALPHA_MOE_ERR_SHAPE;
+    if (M < 0 || M >= 1 << 22 || K <= 0 || K % 128 != 0 || K > 128 * kMaxKBlocks) return ALPHA_MOE_ERR_SHAPE;   // (2^32 threads a launch)
     if (M == 0) return ALPHA_MOE_OK;
     if (!x || !weight || !q || !scale || !residual != !residual_out) return ALPHA_MOE_ERR_NULL_POINTER;
     if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(q) || !aligned16(residual_out) ||

@@ -497,10 +497,10 @@ extern "C" int alpha_moe_route_topk(const void *logits, int is_f32, const float 
                                     int shared_experts, float shared_weight, void *stream)
 {
     using namespace alpha_moe;
-    if (M < 0 || M > INT32_MAX - 64 || E <= 0 || E > kRouteMaxExperts || top_k <= 0 || top_k > kRouteMaxTopK || num_groups <= 0 ||
+    if (M < 0 || M >= 1 << 26 || E <= 0 || E > kRouteMaxExperts || top_k <= 0 || top_k > kRouteMaxTopK || num_groups <= 0 ||
         num_groups > kRouteMaxGroups || E % num_groups != 0 || top_groups <= 0 || top_groups > num_groups ||
         top_k > top_groups * (E / num_groups) || shared_experts < 0 || shared_experts > kRouteMaxExperts)
-        return ALPHA_MOE_ERR_SHAPE;
+        return ALPHA_MOE_ERR_SHAPE;   // (2^26 tokens: 2^32 threads a launch)
     if (M == 0) return ALPHA_MOE_OK;
     if (!logits || !topk_weights || !topk_ids) return ALPHA_MOE_ERR_NULL_POINTER;
     const RouteVariant variant = is_f32 ? (bias ? route_variant<uint32_t, true>(E) : route_variant<uint32_t, false>(E))

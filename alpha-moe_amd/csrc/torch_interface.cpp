@@ -533,7 +533,7 @@ at::Tensor block_scaled_mm(const at::Tensor &x, const at::Tensor &x_scale, const
     TORCH_CHECK(x_scale.dim() == 2 && x_scale.size(0) == M && x_scale.size(1) == K / 128, "x_scale must be [M, K/128]");
     TORCH_CHECK(w_scale.dim() == 2 && w_scale.size(0) == (N + 127) / 128 && w_scale.size(1) == K / 128,
                 "w_scale must be [ceil(N/128), K/128]");
-    check_inference(x_scale, "x_scale"), check_inference(w_scale, "w_scale");
+    check_inference(x, "x"), check_inference(x_scale, "x_scale"), check_inference(w, "w"), check_inference(w_scale, "w_scale");
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
     at::Tensor out = empty_on(dev, {M, N}, at::kBFloat16);

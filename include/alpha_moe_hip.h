@@ -242,7 +242,7 @@ int alpha_moe_layer_call(const uint16_t *x, const int32_t *topk_ids, const uint8
  * q [M, K] and scale [M, K/128] are the codes and scales of y as alpha_moe_per_token_group_quant_fp8 defines them.  x, residual,
  * residual_out (h, rounded to x's type; NULL exactly if residual is) and norm_out (y, rounded to x's type; may be NULL) are
  * [M, K], bf16 or (x_is_f32 != 0) fp32; weight [K] is bf16 or (weight_is_f32 != 0) fp32.  K % 128 == 0, K <= 65536.  residual_out
- * may be residual or x.  A NaN in a group of y makes the group's scale and codes NaN.
+ * may be residual or x.  A NaN in a group of y makes the group's scale and codes NaN.  M < 2^22.
  */
 int alpha_moe_rms_norm_quant_fp8(const void *x, const void *residual, const void *weight, int x_is_f32, int weight_is_f32,
                                  float eps, uint8_t *q, float *scale, void *residual_out, void *norm_out, int M, int K,
@@ -258,7 +258,7 @@ int alpha_moe_swiglu_quant_fp8(const void *gate_up, int is_f32, uint8_t *q, floa
 /*
  * out[m, n] = sum over blocks kb of 128 columns of x_scale[m, kb] * w_scale[n / 128, kb] * (x[m, kb] . w[n, kb]), rounded once.
  *   x [M, K] fp8, x_scale [M, K/128] f32, w [N, K] fp8, w_scale [ceil(N / 128), K/128] f32, out [M, N] bf16.  K % 128 == 0,
- *   K <= 65536; any N.  Sums are taken in an order that depends on M, N and K only.
+ *   K <= 65536; any N (what takes more than 2^32 threads is refused).  Sums are taken in an order that depends on M, N and K only.
  */
 int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale, const uint8_t *w, const float *w_scale,
                               uint16_t *out, int M, int N, int K, void *stream /* hipStream_t */);
@@ -271,7 +271,7 @@ int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale, const uint
  *   two largest choices (its largest if bias is NULL); then the top_k largest choices, descending, equal ones by ascending index.
  *   weights s, divided by their sum if renormalize != 0; the last shared_experts columns are E, E + 1, ... with shared_weight.
  * A NaN choice ranks as -infinity and every id is valid; a row that holds a NaN logit has NaN weights; a row whose chosen scores
- * are all 0 has weights of 0.  E <= 4096, top_k <= 64, num_groups <= 64, top_k <= top_groups * E / num_groups.
+ * are all 0 has weights of 0.  M < 2^26, E <= 4096, top_k <= 64, num_groups <= 64, top_k <= top_groups * E / num_groups.
  */
 int alpha_moe_route_topk(const void *logits, int is_f32, const float *bias, float *topk_weights, int32_t *topk_ids, int M, int E,
                          int top_k, int sigmoid, int num_groups, int top_groups, int renormalize, int shared_experts,

@@ -553,6 +553,16 @@ def test_refusals():
             print(f"refusal {i} went through", flush=True)
 
 
+def test_products_of_codes_that_require_gradients_are_refused():
+    from alpha_moe_python import layer_hip as H
+    q, s, mw, ms = (t.to(DEV) for t in mm_problem(4, 100, 256, 0))
+    for args in ((q.clone().requires_grad_(), s, mw, ms), (q, s, mw.clone().requires_grad_(), ms), (q, s, mw, ms.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            H.block_scaled_mm(*args)
+        with torch.no_grad():
+            H.block_scaled_mm(*args)
+
+
 def test_inputs_that_require_gradients_are_refused():
     from alpha_moe_python import layer_hip as H
     x = torch.zeros((4, 256), dtype=torch.bfloat16, device=DEV)

@@ -69,6 +69,13 @@ def test_route_refusals():
     assert call(logits=None) == NULL and call(weights=None) == NULL and call(ids=None) == NULL
 
 
+def test_more_rows_than_a_launch_has_threads_for_are_refused():
+    assert norm(M=2 ** 22) == SHAPE
+    assert c("alpha_moe_route_topk", [P, I, P, P, P] + [I] * 8 + [F, P], 4096, 1, None, 4096, 4096, 2 ** 26, 8, 2, 0, 1, 1, 1, 0, 1.0, None) == SHAPE
+    for M, N in ((1, 2 ** 31 - 300), (2 ** 31 - 300, 1), (2 ** 24, 2 ** 24), (8, 2 ** 30)):
+        assert c("alpha_moe_block_scaled_mm", [P] * 5 + [I] * 3 + [P], 4096, 4096, 4096, 4096, 4096, M, N, 128, None) == SHAPE, (M, N)
+
+
 def test_cpu_tensors_and_unknown_scoring_are_refused():
     x = torch.zeros((2, 128), dtype=torch.bfloat16)
     q, s = x.to(torch.float8_e4m3fn), torch.ones((2, 1))
