@@ -64,7 +64,7 @@ def fused_experts(hidden_states: torch.Tensor, w13: torch.Tensor, w2: torch.Tens
 def norm_moe(hidden_states: torch.Tensor, residual: torch.Tensor, norm_weight: torch.Tensor, gate_weight: torch.Tensor,
              w13: torch.Tensor, w2: torch.Tensor, w13_scale: torch.Tensor, w2_scale: torch.Tensor, top_k: int,
              scoring: str = "softmax", correction_bias: Optional[torch.Tensor] = None, num_groups: int = 1, top_groups: int = 1,
-             renormalize: bool = True, routed_scaling_factor: float = 1.0, eps: float = 1e-6,
+             renormalize: bool = True, routed_scaling_factor: Optional[float] = None, eps: float = 1e-6,
              config_path: Optional[str] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """An expert layer from the residual addition on: ``(output, residual)``, both ``[M, K]`` bf16.
 
@@ -80,18 +80,20 @@ def norm_moe(hidden_states: torch.Tensor, residual: torch.Tensor, norm_weight: t
     shared = experts - gate_weight.shape[0]
     if shared < 0:
         raise ValueError(f"the gate has {gate_weight.shape[0]} experts, w13 only {experts}")
+    scaling = routed_scaling_factor or 1.0
+    bias = None if correction_bias is None else correction_bias.to(torch.float32)
     cfg = get_best_config(config_path or os.environ["ALPHA_MOE_CONFIG"], hidden_states.shape[0])
     x = rms_norm_quant_fp8(hidden_states, norm_weight, eps, residual=residual, keep_norm=True)
     out = torch.empty_like(hidden_states)
     if hidden_states.shape[0] == 0:
         return out, x.residual
     logits = torch.nn.functional.linear(x.norm.to(gate_weight.dtype), gate_weight)
-    weights, ids = route_topk(logits, top_k, scoring=scoring, bias=correction_bias, num_groups=num_groups, top_groups=top_groups,
-                              renormalize=renormalize, shared_experts=shared, shared_weight=1.0 / routed_scaling_factor)
+    weights, ids = route_topk(logits, top_k, scoring=scoring, bias=bias, num_groups=num_groups, top_groups=top_groups,
+                              renormalize=renormalize, shared_experts=shared, shared_weight=1.0 / scaling)
     aligned = moe_align_block_size(ids, cfg["block_m"], experts)
     torch.ops.alpha_moe.fused_moe_w8a8_up_down_store(
         x.q, x.scale, w13, w13_scale, w2, w2_scale, *aligned, weights, out, top_k + shared, cfg["block_m"], cfg["block_n"],
-        cfg["warp_n"], cfg["stages"], routed_scaling_factor)
+        cfg["warp_n"], cfg["stages"], scaling)
     return out, x.residual
 
 

@@ -100,6 +100,51 @@ def test_expert_layer(M, E, top_k, kw, shared, tmp_path):
         assert all(torch.equal(a, b) for a, b in zip(call(), (out, total)))
 
 
+def expert_layer(M, tmp_path):
+    K, I, E = 512, 256, 16
+    table = os.path.join(tmp_path, "table.json")
+    with open(table, "w") as fh:
+        json.dump({"1": {"block_m": 16, "block_n": 32, "warp_n": 8, "stages": 4},
+                   "512": {"block_m": 64, "block_n": 64, "warp_n": 4, "stages": 3}}, fh)
+    g = torch.Generator().manual_seed(M)
+    hidden, residual = (torch.randn((M, K), generator=g).to(torch.bfloat16) for _ in range(2))
+    gate, bias = torch.randn((E, K), generator=g) * 0.05, (0.1 * torch.randn(E, generator=g)).to(torch.bfloat16)
+    w13, s13 = block_quant_fp8(torch.randn((E + 1, 2 * I, K), generator=g) * 0.05)
+    w2, s2 = block_quant_fp8(torch.randn((E + 1, K, I), generator=g) * 0.05)
+    args = [t.to(DEV) for t in (hidden, residual, torch.ones(K), gate, interleave_tensor(w13, 8), w2, interleave_tensor(s13, 1), s2)]
+    return g, args, bias.to(DEV), dict(scoring="sigmoid", num_groups=4, top_groups=2, config_path=table)
+
+
+def test_expert_layer_with_a_bf16_bias_and_no_scaling(tmp_path):
+    _, args, bias, kw = expert_layer(7, tmp_path)
+    a = norm_moe(*args, 4, correction_bias=bias, routed_scaling_factor=None, **kw)
+    b = norm_moe(*args, 4, correction_bias=bias.float(), routed_scaling_factor=1.0, **kw)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and bool(a[0].isfinite().all())
+
+
+@pytest.mark.parametrize("M", [1, 20, 600])
+def test_expert_layer_captured_and_replayed(M, tmp_path):
+    print(f"case captured experts M={M}", flush=True)
+    g, args, bias, kw = expert_layer(M, tmp_path)
+
+    def call():
+        return norm_moe(*args, 4, correction_bias=bias, routed_scaling_factor=2.5, **kw)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        call()                                  # the fused operator's scratch memory of this stream
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        again = call()
+    for step in range(4):
+        args[0].copy_(torch.randn(args[0].shape, generator=g).to(torch.bfloat16))
+        want = call()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(again, want)), step
+
+
 def test_no_tokens_and_refusals(tmp_path):
     table = os.path.join(tmp_path, "table.json")
     with open(table, "w") as fh:
