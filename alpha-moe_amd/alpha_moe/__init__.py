@@ -1,6 +1,8 @@
 """``import alpha_moe`` registers ``torch.ops.alpha_moe.fused_moe_w8a8_up_down`` (as the reference's extension
 module of the same name does, csrc/torch_interface.cpp:105-131) by loading the in-tree HIP libraries, together with
-the two input-preparation operators ``per_token_group_quant_fp8`` and ``moe_align_block_size``.
+the two input-preparation operators ``per_token_group_quant_fp8`` and ``moe_align_block_size`` and the operators that run
+around a layer call: ``rms_norm_quant_fp8``, ``add_rms_norm_quant_fp8``, ``swiglu_quant_fp8``, ``block_scaled_mm`` and
+``route_topk`` (``alpha_moe_python.layer_hip`` is their front).
 
 There is no fallback: if the libraries are not built the import fails.
 """
@@ -70,6 +72,17 @@ c_abi.alpha_moe_moe_align_block_size.argtypes = (
 c_abi.alpha_moe_prepare_inputs.restype = ctypes.c_int
 c_abi.alpha_moe_prepare_inputs.argtypes = (
     c_abi.alpha_moe_per_token_group_quant_fp8.argtypes[:-1] + c_abi.alpha_moe_moe_align_block_size.argtypes)
+c_abi.alpha_moe_rms_norm_quant_fp8.restype = ctypes.c_int
+c_abi.alpha_moe_rms_norm_quant_fp8.argtypes = (
+    [ctypes.c_void_p] * 3 + [ctypes.c_int] * 2 + [ctypes.c_float] + [ctypes.c_void_p] * 4 + [ctypes.c_int] * 2 + [ctypes.c_void_p])
+c_abi.alpha_moe_swiglu_quant_fp8.restype = ctypes.c_int
+c_abi.alpha_moe_swiglu_quant_fp8.argtypes = (
+    [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p])
+c_abi.alpha_moe_block_scaled_mm.restype = ctypes.c_int
+c_abi.alpha_moe_block_scaled_mm.argtypes = [ctypes.c_void_p] * 5 + [ctypes.c_int] * 3 + [ctypes.c_void_p]
+c_abi.alpha_moe_route_topk.restype = ctypes.c_int
+c_abi.alpha_moe_route_topk.argtypes = (
+    [ctypes.c_void_p, ctypes.c_int] + [ctypes.c_void_p] * 3 + [ctypes.c_int] * 8 + [ctypes.c_float, ctypes.c_void_p])
 
 __version__ = c_abi.alpha_moe_version().decode()
 
