@@ -118,7 +118,9 @@ __device__ __forceinline__ void store4(const MmParams &p, int m, int n, v4f v)
 // partial sums' second launch costs 3 - 4 us, more than the idle compute units it fills (61 x 2112 x 7168 in seven parts 11.6 us).
 // Weights are loaded non-temporally only with at most eight tokens, where they are read once and there is little else to read
 // (1 x 4096 x 7168 from HBM 6.7 us against 7.5, from the last-level cache 6.4 and 6.6; but 61 x 2112 x 7168 11.9 and 8.3).
-// Deeper rings change nothing (16 x 4096 x 7168 with two, four K blocks 7.0, 7.05 us).
+// Deeper rings change nothing (16 x 4096 x 7168 with two, four K blocks 7.0, 7.05 us).  Eight wavefronts where a tile is 16 x 16 or
+// the tokens are few, four for larger ones, of which two fit a compute unit (17 x 4096 x 7168, 32 x 16 tile, eight 7.7, four 6.9 us; 32 x
+// 4096 x 7168 7.4, 7.1; 32 x 32 tile 61 x 2112 x 7168 8.7, 8.4; 16 x 16 tile, 16 x 4096 x 7168, 6.8 with eight).
 template <int R, int T, int WAVES, int D, bool HALF>
 struct StreamRing {
     static constexpr bool kRun = T >= 4;   // the tokens' scales four K blocks at a time
@@ -588,7 +590,7 @@ extern "C" int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale,
     case kStreamHalf1: err = launch_stream_mm<1, 1, 8, 2, true>(p, hs); break;
     case kStreamHalf2: err = launch_stream_mm<2, 1, 8, 2, true>(p, hs); break;
     case kStream1x1: err = launch_stream_mm<1, 1, 8, 2, false>(p, hs); break;
-    case kStream2x1: err = launch_stream_mm<2, 1, 8, 2, false>(p, hs); break;
+    case kStream2x1: err = launch_stream_mm<2, 1, 4, 2, false>(p, hs); break;
     case kStream2x2: err = launch_stream_mm<2, 2, 4, 2, false>(p, hs); break;
     case kStream4x2: err = launch_stream_mm<4, 2, 4, 2, false>(p, hs); break;
     case kStream4x4: err = launch_stream_mm<4, 4, 4, 1, false>(p, hs); break;
