@@ -63,7 +63,7 @@ def block_scaled_mm(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_s
     """``out [M, N] = (x * x_scale) (w * w_scale)^T``, rounded once to bfloat16.
 
     x ``[M, K]`` float8_e4m3fn with x_scale ``[M, K/128]``; w ``[N, K]`` float8_e4m3fn with w_scale ``[ceil(N/128), K/128]``.
-    N is of any size, K a multiple of 128 up to 65536 (a multiple of 512 is loaded with fewer instructions).  Bit for bit the same from run to run.
+    N is of any size, K a multiple of 128 up to 65536.  Bit for bit the same from run to run.
     """
     return _block_scaled_mm(x, x_scale, w, w_scale)
 

@@ -31,7 +31,7 @@ struct MmParams {
     uint16_t *out;
     int M, N, K, nkb;
     int row_groups, token_groups;   // tiles of the launch
-    int quads;   // 1: a token's scales of four K blocks start at a multiple of 16 bytes, and are loaded together
+    int quads;   // 1: there are four K blocks, whose scales of a token are loaded together
 };
 
 __device__ __forceinline__ int rfl(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -72,19 +72,21 @@ __device__ __forceinline__ lds_v4i lds_tile(const void *p) { return (lds_v4i)(ui
 __device__ __forceinline__ v4i lds_read(const void *p) { return *lds_tile(p); }
 __device__ __forceinline__ float lds_float(const void *p) { return *(lds_f32)(uint32_t)(uintptr_t)p; }
 
-// The scales of a tile's tokens in LDS, loaded four K blocks at a time where they can be (one by one, every scale is a line of its own
-// on the path into the compute unit, half as many again as the data is; 8192 x 4096 x 7168 221 us, by fours 207; 2048 x 4096 x 7168 57.0
-// and 56.0): two places of [token][K block & 3], or eight of [token].
+// The scales of a tile's tokens in LDS, loaded four K blocks at a time if there are four (one by one, every scale is a line of its own
+// on the path into the compute unit, half as many again as the data is; 8192 x 4096 x 7168 221 us, by fours 207, x 7296 229 and 220, 2048 x
+// 4096 x 7168 57.0 and 56.0): two places of [token][four K blocks], or eight of [token].
 struct TokenScales {
-    int quads, tokens;
+    int quads, tokens, last;   // last: the K block at which the last four of a row begin (which a row's last load takes, so that it ends with
+                               // the row; a load of 16 bytes may start at any multiple of four)
     __device__ __forceinline__ bool loads(int kb, bool first) const { return !quads || first || (kb & 3) == 0; }
-    __device__ __forceinline__ int place(int kb) const { return quads ? ((kb >> 2) & 1) * tokens * 16 + (kb & 3) * 4 : (kb & 7) * tokens * 4; }
+    __device__ __forceinline__ int begin(int kb) const { return (kb & ~3) < last ? kb & ~3 : last; }   // of the four with kb
+    __device__ __forceinline__ int place(int kb) const { return quads ? ((kb >> 2) & 1) * tokens * 16 + (kb - begin(kb)) * 4 : (kb & 7) * tokens * 4; }
     __device__ __forceinline__ int stride() const { return quads ? 16 : 4; }   // from token to token
     // lanes [0, count) load the scales of as many tokens, from `token` on, that K block kb is the first to ask for
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t base, unsigned offset, int kb, int token, bool mine, uint8_t *area) const
     {
         if (quads) {
-            if (mine) dma16<0>(base, offset, 4u * (unsigned)(kb & ~3), area + place(kb & ~3) + token * 16);
+            if (mine) dma16<0>(base, offset, 4u * (unsigned)begin(kb), area + ((kb >> 2) & 1) * tokens * 16 + token * 16);
         } else {
             if (mine) dma4(base, offset, 4u * (unsigned)kb, area + place(kb) + token * 4);
         }
@@ -187,7 +189,7 @@ __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(const MmParams p)
 
     uint8_t *ring = lds + w * Ring::kWave;
     uint8_t *ws = ring + D * Ring::kSlot, *xs = ws + Ring::kScales;
-    const TokenScales scales = {p.quads, T * 16};   // (RUN)
+    const TokenScales scales = {p.quads, T * 16, nkb - 4};   // (RUN)
     for (int c = 0; c < count; c += 64)
         if (c + lane < count) dma4(wsbuf, 4u * (unsigned)(first + (c + lane) * STEP), 0u, ws + 4 * c);
     // Load j of a slot for the i-th of this wavefront's K blocks: weights and tokens, the tokens' scales between them, or in front of
@@ -378,7 +380,7 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(co
     const int my_token = lw * T::kScaleLanes + (lane < T::kScaleLanes ? lane : 0);
     const unsigned xs_off = 4u * (unsigned)((m0 + my_token < p.M ? my_token : p.M - 1 - m0) * nkb);
     uint8_t *xs = lds + S * T::kStage, *ws = xs + T::kTokens * 32;
-    const TokenScales scales = {p.quads, T::kTokens};
+    const TokenScales scales = {p.quads, T::kTokens, nkb - 4};
 
     // (a tile's offsets are below 2^25: rows of up to 64 KiB)
     const uint8_t *w_base = p.w + (size_t)c0 * K, *x_base = p.x + (size_t)m0 * K;
@@ -583,7 +585,7 @@ extern "C" int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale,
     MmParams p = {};
     p.x = x, p.x_scale = x_scale, p.w = w, p.w_scale = w_scale, p.out = out;
     p.M = M, p.N = N, p.K = K, p.nkb = K / 128;
-    p.quads = p.nkb % 4 == 0 && (reinterpret_cast<uintptr_t>(x_scale) & 15) == 0;
+    p.quads = p.nkb >= 4;
     hipStream_t hs = static_cast<hipStream_t>(stream);
     hipError_t err = hipErrorInvalidValue;
     switch (plan(M, N)) {
