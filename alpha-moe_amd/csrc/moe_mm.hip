@@ -80,7 +80,10 @@ struct TokenScales {
                                // the row; a load of 16 bytes may start at any multiple of four)
     __device__ __forceinline__ bool loads(int kb, bool first) const { return !quads || first || (kb & 3) == 0; }
     __device__ __forceinline__ int begin(int kb) const { return (kb & ~3) < last ? kb & ~3 : last; }   // of the four with kb
-    __device__ __forceinline__ int place(int kb) const { return quads ? ((kb >> 2) & 1) * tokens * 16 + (kb - begin(kb)) * 4 : (kb & 7) * tokens * 4; }
+    __device__ __forceinline__ int place(int kb) const
+    {
+        return quads ? ((kb >> 2) & 1) * tokens * 16 + (kb - begin(kb)) * 4 : (kb & 7) * tokens * 4;
+    }
     __device__ __forceinline__ int stride() const { return quads ? 16 : 4; }   // from token to token
     // lanes [0, count) load the scales of as many tokens, from `token` on, that K block kb is the first to ask for
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t base, unsigned offset, int kb, int token, bool mine, uint8_t *area) const
@@ -118,6 +121,8 @@ __device__ __forceinline__ void store4(const MmParams &p, int m, int n, v4f v)
 // block, 70 - 100 GB/s) from some thirty on.  MI355X, back to back: 1 x 4096 x 7168 (29 MB) 6.0 us, of which 2.5 are an
 // empty call's, 61 x 2112 x 7168 8.3, 64 x 7168 x 2048 6.0, 256 x 4096 x 7168 15.  Why not the contraction split over workgroups: the
 // partial sums' second launch costs 3 - 4 us, more than the idle compute units it fills (61 x 2112 x 7168 in seven parts 11.6 us).
+// Why through LDS, though no wavefront reads what another has loaded: a load into a matrix operand's registers takes 64 bytes of sixteen
+// lines, and lines are what the path counts (61 x 2112 x 7168 so 15.4 us, 1 x 4096 x 7168 7.8).
 // Weights are loaded non-temporally only with at most eight tokens, where they are read once and there is little else to read
 // (1 x 4096 x 7168 from HBM 6.7 us against 7.5, from the last-level cache 6.4 and 6.6; but 61 x 2112 x 7168 11.9 and 8.3).
 // Deeper rings change nothing (16 x 4096 x 7168 with two, four K blocks 7.0, 7.05 us).  Eight wavefronts where a tile is 16 x 16 or
@@ -316,11 +321,13 @@ hipError_t launch_stream_mm(MmParams p, hipStream_t stream)
 // out one by one between matrix instructions, over the first three eighths of a K block (8192 x 4096 x 7168 in a burst 226, over three
 // eighths 221, over all of it 231; with the tokens' scales four K blocks at a time then 207).
 //
-// What bounds it: matrix instructions and their scaling multiply-adds (19.3 ns a pair on random operands, where the clock gives way:
-// 138 us for 8192 x 4096 x 7168; on equal operands 14.8), and LDS, which takes loads in at 64 bytes a cycle while fragments are
-// read from it (without any loads the same kernel takes 137 us).  MI355X: 8192 x 4096 x 7168 207 us (2.33 PFLOP/s; a library product of
-// the same size without block scales 188), 4096 x 4096 x 7168 99, 1024 x 7168 x 2048 18.7, 256 x 7168 x 2048 9.4.  Also
-// tried, against 221: 128 columns x 64 tokens a wavefront 237; token fragments read two passes ahead 228; all fragments read behind the barrier 239.
+// What bounds it: up to 256 x 128 the path into a compute unit, which takes four cycles for a line of 128 bytes (128 x 64 tile 0.38 us a
+// K block of 192 lines, 128 x 128 0.50, 256 x 128 0.70).  In the largest tile matrix instructions and their scaling multiply-adds
+// (19.3 ns a pair on random operands, where the clock gives way: 138 us for 8192 x 4096 x 7168; on equal operands 14.8), and LDS,
+// which takes loads in at 64 bytes a cycle while fragments are read from it (without any loads the same kernel takes 137 us).
+// MI355X: 8192 x 4096 x 7168 207 - 217 us by card (2.2 - 2.3 PFLOP/s; a library product of the same size without block scales 188),
+// 4096 x 4096 x 7168 99, 1024 x 7168 x 2048 18.7, 256 x 7168 x 2048 9.4.  Also tried, against 221: 128 columns x 64 tokens a wavefront
+// 237; token fragments read two passes ahead 228; all fragments read behind the barrier 239.
 template <int TN, int TM, int WN, int WM, int S, int LOADERS>
 struct Tile {
     static constexpr int kWaves = WN * WM, kLoaders = LOADERS > 0 ? LOADERS : kWaves, kCols = TN * 16 * WN, kTokens = TM * 16 * WM;

@@ -10,6 +10,11 @@
 //
 // A NaN makes its group's scale and codes NaN (the maxima are taken over the bits of |y|, where a NaN is larger than anything), so
 // what was lost upstream stays visible behind the product.
+//
+// Both are bound by memory, or by the launch: MI355X, bf16, 8192 x 7168 with a residual 72.5 us (411 MB, 5.7 TB/s; a copy of a GiB 5.1),
+// 1 x 7168 3.0 us, SwiGLU of 8192 x 2 x 2048 14.0 us (84 MB, some of it from the last-level cache), 7 x 2 x 768 1.9; an empty call 2.2.
+// The norm's rows stay in registers, so that a row is read once; a group's maximum takes a few data-parallel steps in registers
+// (through shuffles, with a second pass over the row for the codes, the two took 76 and 19 us).
 #include "moe_common.hpp"
 
 namespace alpha_moe {
