@@ -327,7 +327,8 @@ hipError_t launch_stream_mm(MmParams p, hipStream_t stream)
 // which takes loads in at 64 bytes a cycle while fragments are read from it (without any loads the same kernel takes 137 us).
 // MI355X: 8192 x 4096 x 7168 207 - 217 us by card (2.2 - 2.3 PFLOP/s; a library product of the same size without block scales 188),
 // 4096 x 4096 x 7168 99, 1024 x 7168 x 2048 18.7, 256 x 7168 x 2048 9.4.  Also tried, against 221: 128 columns x 64 tokens a wavefront
-// 237; token fragments read two passes ahead 228; all fragments read behind the barrier 239.
+// 237; token fragments read two passes ahead 228; all fragments read behind the barrier 239; against 213: weights loaded a K block
+// further ahead, behind a barrier of their own, so that loads go out over all of a K block, 214.
 template <int TN, int TM, int WN, int WM, int S, int LOADERS>
 struct Tile {
     static constexpr int kWaves = WN * WM, kLoaders = LOADERS > 0 ? LOADERS : kWaves, kCols = TN * 16 * WN, kTokens = TM * 16 * WM;
