@@ -96,19 +96,23 @@ struct TokenScales {
     }
 };
 
+// Results at any multiple of their two bytes: a row of an odd N starts at one.  (Memory takes stores of 8 and 16 bytes there as a whole;
+// value by value 8192 x 4095 x 1024 takes 124 us, so 62; 4094 columns 128 and 48, 4096 43.)
+typedef uint32_t any2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
+
 // Columns n .. n + 3 of row m; what is behind the last row or column is not there.
 __device__ __forceinline__ void store4(const MmParams &p, int m, int n, v4f v)
 {
     if (m >= p.M || n >= p.N) return;
     uint16_t *at = p.out + (size_t)m * p.N + n;
-    const uint2 two = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-    if ((p.N & 3) == 0) {   // (then n + 3 is a column too, and the address a multiple of four values)
-        *reinterpret_cast<uint2 *>(at) = two;
+    const any2 two = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    if (n + 3 < p.N) {
+        *reinterpret_cast<any2 *>(at) = two;
     } else {
-        at[0] = (uint16_t)two.x;
-        if (n + 1 < p.N) at[1] = (uint16_t)(two.x >> 16);
-        if (n + 2 < p.N) at[2] = (uint16_t)two.y;
-        if (n + 3 < p.N) at[3] = (uint16_t)(two.y >> 16);
+        at[0] = (uint16_t)two[0];
+        if (n + 1 < p.N) at[1] = (uint16_t)(two[0] >> 16);
+        if (n + 2 < p.N) at[2] = (uint16_t)two[1];
     }
 }
 
@@ -512,14 +516,14 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(co
 #pragma unroll
     for (int t = 0; t < TM; t++) {
         const int m = m0 + (wm * TM + t) * 16 + n;
-        if ((p.N & 7) == 0 && col + 4 * TN <= p.N) {
+        if (col + 4 * TN <= p.N) {
             if (m < p.M) {
-                v4i *to = reinterpret_cast<v4i *>(p.out + (size_t)m * p.N + col);
+                any4 *to = reinterpret_cast<any4 *>(p.out + (size_t)m * p.N + col);
 #pragma unroll
                 for (int k = 0; k < TN; k += 2)
-                    to[k / 2] = (v4i){(int)pack_bf16x2(acc[k][t][0], acc[k][t][1]), (int)pack_bf16x2(acc[k][t][2], acc[k][t][3]),
-                                      (int)pack_bf16x2(acc[k + 1][t][0], acc[k + 1][t][1]),
-                                      (int)pack_bf16x2(acc[k + 1][t][2], acc[k + 1][t][3])};
+                    to[k / 2] = (any4){pack_bf16x2(acc[k][t][0], acc[k][t][1]), pack_bf16x2(acc[k][t][2], acc[k][t][3]),
+                                       pack_bf16x2(acc[k + 1][t][0], acc[k + 1][t][1]),
+                                       pack_bf16x2(acc[k + 1][t][2], acc[k + 1][t][3])};
             }
         } else {
 #pragma unroll
