@@ -128,7 +128,8 @@ __device__ __forceinline__ void store4(const MmParams &p, int m, int n, v4f v)
 // Why through LDS, though no wavefront reads what another has loaded: a load into a matrix operand's registers takes 64 bytes of sixteen
 // lines, and lines are what the path counts (61 x 2112 x 7168 so 15.4 us, 1 x 4096 x 7168 7.8).
 // Weights are loaded non-temporally only with at most eight tokens, where they are read once and there is little else to read
-// (1 x 4096 x 7168 from HBM 6.7 us against 7.5, from the last-level cache 6.4 and 6.6; but 61 x 2112 x 7168 11.9 and 8.3).
+// (1 x 4096 x 7168 from HBM 7.1 us against 7.6, 3 x 1280 x 5120 4.7 and 5.0; but 61 x 2112 x 7168 11.9 and 8.3.  A loop over one small
+// matrix would rather keep it in L2, 3 x 1280 x 5120 4.7 and 3.4 us; a model's layers come back after all the others).
 // Deeper rings change nothing (16 x 4096 x 7168 with two, four K blocks 7.0, 7.05 us).  Eight wavefronts where a tile is 16 x 16 or
 // the tokens are few, four for larger ones, of which two fit a compute unit (17 x 4096 x 7168, 32 x 16 tile, eight 7.7, four 6.9 us; 32 x
 // 4096 x 7168 7.4, 7.1; 32 x 32 tile 61 x 2112 x 7168 8.7, 8.4; 16 x 16 tile, 16 x 4096 x 7168, 6.8 with eight).
