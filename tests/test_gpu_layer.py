@@ -582,3 +582,21 @@ def test_inputs_that_require_gradients_are_refused():
             call()
         with torch.inference_mode():
             call()
+
+
+def test_schemas_and_fakes_say_what_the_operators_do():
+    """no result shares memory with another or with an input; shapes, types and strides are those of the fake implementations"""
+    import alpha_moe_ops  # noqa: F401
+    o = torch.ops.alpha_moe
+    x, w = torch.randn((5, 512), device=DEV).to(torch.bfloat16), torch.ones(512, device=DEV)
+    q, s, mw, ms = (t.to(DEV) for t in mm_problem(5, 130, 512, 0))
+    logits = torch.randn((5, 64), device=DEV)
+    both = ("test_schema", "test_faketensor")
+    for op, args, utils in ((o.rms_norm_quant_fp8.default, (x, w, 1e-6, 128), both),
+                            (o.rms_norm_quant_fp8.keep_norm, (x, w, 1e-6, 128), both),
+                            (o.add_rms_norm_quant_fp8.default, (x, x.clone(), w, 1e-6, 128), both),
+                            (o.add_rms_norm_quant_fp8.keep_norm, (x, x.clone(), w, 1e-6, 128), both),
+                            (o.swiglu_quant_fp8.default, (x, 128), both),
+                            (o.block_scaled_mm.default, (q, s, mw, ms), both[1:]),     # (the schema's check multiplies its inputs)
+                            (o.route_topk.default, (logits, None, 4, False, 1, 1, True, 1, 1.0), both)):
+        torch.library.opcheck(op, args, test_utils=utils)
