@@ -72,6 +72,14 @@ __device__ __forceinline__ float wave_sum(float v)
     return v;
 }
 
+// The sum of f(0) .. f(V - 1), halves first: none of them passes more than log2 V additions.
+template <int V, int FROM = 0, typename F>
+__device__ __forceinline__ float tree_sum(F f)
+{
+    if constexpr (V == 1) return f(FROM);
+    else return tree_sum<V / 2, FROM>(f) + tree_sum<V / 2, FROM + V / 2>(f);
+}
+
 // An unsigned number of the same order; a NaN is -infinity, and the two zeros are one.
 __device__ __forceinline__ uint32_t order_key(float v)
 {
@@ -164,9 +172,15 @@ __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f
 __device__ __forceinline__ float sigmoid_of(float x) { return __builtin_amdgcn_rcpf(1.0f + exp_of(-x)); }
 
 // How far two choices in fp32 have to be from each other for their order to be that in 64 bits, in roundings (2^-24) of 1 + the largest
-// finite bias: a sigmoid is at most 4 off, a softmax 16 (its sum's error counts the score's share), a choice one of its size more,
-// and there are two of them: 12 and 36.  The sum of two choices that a group is worth is off by both and its own rounding, and there
-// are two of these: 24 and 76.  (Equal infinities are never far enough.)
+// finite bias.  A sigmoid is at most 4 off, a choice one of its size more, and there are two of them: 12.  The sum of two choices that a
+// group is worth is off by both and its own rounding, and there are two of these: 24.
+// A softmax score e^x / sum, x <= 0: the subtraction that makes x and the exponential are (2.25 |x| + 2) off, which the score's size turns
+// into less than 2.1; the division is one of its size.  The sum is off by its terms' errors, each with the share p of its term - at
+// most sum p (2.25 |x| + 2), which with the score's own share is below 6 for 4096 experts -, and by log2 V + 6 <= 12 additions, whose
+// parts are none of them larger than the sum (one behind the other V = 64 would be 69, and loses that much where one score is near 1 and
+// the others of its lane are just below 2^-24).  The sum's 18 are common to both scores, whose difference is below 1.  So two choices:
+// 2 (2.1 + 1) + 18 and their own roundings 2, less than 36; two groups, of two scores each that together are below 1: 4 (2.1 + 1) + 18
+// and additions 4 + 4, less than 76.  (Equal infinities are never far enough.)
 struct Margin {
     float choice, group;
     __device__ __forceinline__ Margin(float largest_bias, bool sigmoid)
@@ -365,13 +379,9 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(const RoutePara
 #pragma unroll
             for (int v = 0; v < V; v++) score[v] = sigmoid_of(l[v]);
         } else {
-            float sum = 0.f;
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                score[v] = part(l[v]);
-                sum += l[v] == l[v] ? score[v] : 0.f;   // (a NaN logit has no part in it)
-            }
-            sum = wave_sum(sum);
+            for (int v = 0; v < V; v++) score[v] = part(l[v]);
+            const float sum = wave_sum(tree_sum<V>([&](int v) { return l[v] == l[v] ? score[v] : 0.f; }));   // (a NaN logit has no part in it)
 #pragma unroll
             for (int v = 0; v < V; v++) score[v] = l[v] == -__builtin_inff() ? 0.f : score[v] / sum;
         }
@@ -448,10 +458,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(const RoutePara
         } else {
             w = part(x);
             if (!s.renormalize) {
-                float sum = 0.f;
-#pragma unroll
-                for (int v = 0; v < V; v++) sum += part(l[v]);
-                sum = wave_sum(sum);
+                const float sum = wave_sum(tree_sum<V>([&](int v) { return part(l[v]); }));
                 w = sum != 0.f ? w / sum : 0.f;
             }
         }
