@@ -12,7 +12,9 @@
 // neighbours are closer than fp32 tells in one token of a few thousand, and which expert a token visits is not a rounding.
 //
 // A NaN choice ranks as -infinity.  Every id is a valid one whatever the logits hold; a row with a NaN logit has NaN weights, a row
-// without scores (every chosen logit -infinity) weights of 0.
+// without scores (every chosen logit -infinity) weights of 0.  Scores up to e^-700, which masks make rather than routers, are 0.
+// Above, renormalised weights keep their ratio also where fp32 has no numbers for the scores: where the chosen ones' sum is below 2^-24
+// they are exp(l - the largest chosen l), which is a softmax's ratio exactly and a sigmoid's but for its factor 1 + exp(l) < 1 + 2^-24.
 //
 // One wavefront to a token.  Lane l holds the V experts l V .. l V + V - 1, so that the lowest lane of several with the same value
 // has the lowest expert.  What bounds it is instructions, one dependent chain of them per token, so:
@@ -45,6 +47,7 @@ constexpr int kRouteMaxExperts = 4096;
 constexpr int kRouteMaxTopK = 64;     // a lane each
 constexpr int kRouteMaxGroups = 64;
 constexpr int kRouteWaves = 4;        // most tokens of a workgroup
+constexpr float kNoScore = -700.f;    // a score of its exponential, or less, is 0
 
 // The largest value of the wavefront, in every lane.
 __device__ __forceinline__ uint32_t wave_max(uint32_t v)
@@ -399,7 +402,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(const RoutePara
         const Margin margin(__builtin_bit_cast(float, wave_max(largest)), s.sigmoid);
         auto exact = [&](int e) {
             const double x = (double)logit_at<T>(s.logits, (size_t)token * E + e);
-            return order_key(1.0 / (1.0 + exp(-x)) + (double)s.bias[e]);
+            return order_key((x <= kNoScore ? 0.0 : 1.0 / (1.0 + exp(-x))) + (double)s.bias[e]);
         };
         auto exact_keys = [&](uint64_t (&wide)[V]) {
             double sum = 1.0;
@@ -412,8 +415,9 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(const RoutePara
             }
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                double d = s.sigmoid ? 1.0 / (1.0 + exp(-(double)l[v])) : exp((double)l[v] - (double)top) / sum;
-                if (!s.sigmoid && l[v] == -__builtin_inff()) d = 0.0;
+                const double x = s.sigmoid ? (double)l[v] : (double)l[v] - (double)top;
+                double d = s.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x) / sum;
+                if (x <= kNoScore || l[v] == -__builtin_inff()) d = 0.0;
                 const uint64_t of = order_key(d + (double)bias[v]);
                 wide[v] = e0 + v < E ? of : 0;
             }
@@ -465,7 +469,13 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(const RoutePara
     }
     w = lane < s.top_k ? w : 0.f;
     if (s.renormalize) {
-        const float sum = wave_sum(w);
+        float sum = wave_sum(w);
+        if (sum < 0x1p-24f) {   // (one value in all lanes)
+            const float x = lane < s.top_k ? logit_at<T>(s.logits, (size_t)token * E + my_id) : -__builtin_inff();
+            const float best = from_key(wave_max(order_key(x)));
+            w = x == -__builtin_inff() || (s.sigmoid ? x : x - top) <= kNoScore ? 0.f : exp_of(x - best);
+            sum = wave_sum(w);
+        }
         w = sum != 0.f ? w / sum : 0.f;
     }
     const int kept = s.top_k + s.shared;

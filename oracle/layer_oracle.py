@@ -56,7 +56,7 @@ def route_topk(logits, top_k, scoring="softmax", bias=None, num_groups=1, top_gr
         def score(l):
             if scoring == "sigmoid":
                 return 1.0 / (1.0 + math.exp(-l)) if l > -700 else 0.0
-            return 0.0 if l == -math.inf else math.exp(l - top)
+            return 0.0 if l == -math.inf or l - top <= -700 else math.exp(l - top)     # (so is a sigmoid's score 0 up to e^-700)
 
         scores = [math.nan if l != l else score(l) for l in row]
         if scoring == "softmax":

@@ -30,3 +30,72 @@ def test_softmax_with_a_bias_of_one_loud_expert_and_many_faint_ones(E, small, se
         for groups in (4, 8):
             if E % groups == 0:
                 assert_route(logits, top_k, bias=bias, num_groups=groups, top_groups=2)
+
+
+# ---- scores below fp32's normal numbers --------------------------------------------------------------------
+def assert_far_route(logits, top_k, **kw):
+    """As assert_route, for weights far from 1.  A weight w is exp of some |x| <= -ln w below the largest chosen logit: the
+    subtraction is off by |x| u in the exponent, x log2(e) by 1.25 |x| u, the exponential 2 u; the sum of at most 64 of them by
+    its terms' errors, weighted, (2.25 ln 64 + 2) u < 12 u, and 6 additions; the division u: (2.25 |ln w| + 21) u, and 8 u for
+    the factor 1 + exp(l) that scores below 2^-24 leave out.  A score below 2^-126 may be 0 where the chosen ones' sum is not below 2^-24."""
+    from alpha_moe_python import layer_hip
+    dev = {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+    w, ids = layer_hip.route_topk(logits.to(DEV), top_k, **dev)
+    want, want_ids = L.route_topk(logits, top_k, **kw)
+    assert torch.equal(ids.cpu().long(), want_ids)
+    rel = (2.25 * want.clamp_min(2.0 ** -126).log().abs() + 32) * U
+    assert_within(w, want, rel * want + 2.0 ** -102, "weights")
+    return w
+
+
+FAR = [[-99.0] + [-100.0] * 15, [-88.0, -88.5, -89.0, -90.0] * 4, [-87.0, -88.0] + [-600.0] * 14, [-699.0 + i / 4 for i in range(16)],
+       [-17.0, -30.0, -60.0, -120.0] * 4, [-16.0, -16.5, -17.5, -18.0] * 4, [-650.0] + [-720.0] * 15, [-300.0] * 16,
+       [-103.0, -math.inf] * 8, [-200.0 + 13 * i for i in range(16)], [-15.0, -95.0] * 8]
+
+
+@pytest.mark.parametrize("E", [16, 64, 100, 256, 600, 1100, 4096])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("biased", [False, True])
+def test_sigmoid_weights_of_far_logits_keep_their_ratio(E, dtype, biased):
+    """every chosen logit below -88, where a sigmoid is no fp32 number any more; the weights' ratio is"""
+    print(f"case far sigmoid E={E} {dtype} {biased}", flush=True)
+    g = torch.Generator().manual_seed(E)
+    logits = torch.full((len(FAR), E), -math.inf)
+    for m, row in enumerate(FAR):
+        logits[m, torch.randperm(E, generator=g)[:16]] = torch.tensor(row)
+    logits = logits.to(dtype)
+    bias = 0.1 * torch.randn(E, generator=g) if biased else None
+    groups = dict(num_groups=4, top_groups=2) if E % 4 == 0 else {}
+    for top_k in (1, 4, 8):
+        assert_far_route(logits, top_k, scoring="sigmoid", bias=bias)
+        assert_far_route(logits, top_k, scoring="sigmoid", bias=bias, shared_experts=1, shared_weight=0.4, **groups)
+    if bias is None:
+        w = assert_far_route(logits, 4, scoring="sigmoid")
+        assert bool(((w.sum(1) - 1).abs() < 8 * U).all())
+
+
+@pytest.mark.parametrize("E", [16, 64, 100, 256, 600, 1100, 4096])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_softmax_weights_of_experts_far_below_the_largest_keep_their_ratio(E, dtype):
+    """a bias keeps the row's largest logit out: what is chosen lies further below it than fp32 reaches"""
+    print(f"case far softmax E={E} {dtype}", flush=True)
+    g = torch.Generator().manual_seed(E)
+    logits = torch.full((len(FAR), E), -math.inf)
+    bias = torch.full((E,), -2.0)
+    for m, row in enumerate(FAR):
+        at = torch.randperm(E - 1, generator=g)[:15] + 1
+        logits[m, at] = torch.tensor(row[:15]) + 3.0
+    logits[:, 0] = 3.0
+    logits = logits.to(dtype)
+    bias[0] = -math.inf
+    bias[1:] += torch.randperm(E - 1, generator=g) / E
+    for top_k in (1, 4, 8):
+        assert_far_route(logits, top_k, bias=bias)
+        if E % 4 == 0:
+            assert_far_route(logits, top_k, bias=bias, num_groups=4, top_groups=3)
+    best = logits.float()[:, 1:].amax(1)             # the experts with the largest logits behind it, and nobody else
+    for m in range(len(FAR)):
+        one = torch.full((E,), -math.inf)
+        which = (logits[m].float() == best[m]).nonzero().flatten()
+        one[which] = 0.5
+        assert_far_route(logits[m:m + 1], min(8, which.numel()), bias=one)
