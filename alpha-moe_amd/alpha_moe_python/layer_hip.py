@@ -80,9 +80,10 @@ def route_topk(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias:
     name the experts E, E + 1, ... fused behind the routed ones, with ``shared_weight`` (1 / routed scaling factor
     where the fused operator scales everything).  E is at most 4096, top_k and num_groups at most 64.
 
-    A NaN ranks last and makes its row's weights NaN; a row whose chosen scores are all 0 (every logit -inf) has weights of 0.  Ids
-    are valid whatever the logits hold.  Scores up to e^-700 are 0; above, renormalised weights keep their ratio where all chosen
-    scores are too small for fp32 (beside larger ones, and with ``renormalize=False``, one below 2^-126 may count as 0).
+    A NaN ranks last and makes its row's weights NaN (and so does +inf in a softmax); a row whose chosen scores are all 0 (every
+    logit -inf) has weights of 0.  Ids are valid whatever the logits hold.  Scores up to e^-700 are 0; above, renormalised weights
+    keep their ratio where all chosen scores are too small for fp32 (beside larger ones, and with ``renormalize=False``, one below
+    2^-126 may count as 0).
     """
     if scoring not in ("softmax", "sigmoid"):
         raise ValueError(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")

@@ -11,8 +11,8 @@
 // Of equal choices, and of equal groups, the lower index comes first.  The order is decided in 64 bits: of 256 experts' scores two
 // neighbours are closer than fp32 tells in one token of a few thousand, and which expert a token visits is not a rounding.
 //
-// A NaN choice ranks as -infinity.  Every id is a valid one whatever the logits hold; a row with a NaN logit has NaN weights, a row
-// without scores (every chosen logit -infinity) weights of 0.  Scores up to e^-700, which masks make rather than routers, are 0.
+// A NaN choice ranks as -infinity.  Every id is a valid one whatever the logits hold; a row with a NaN logit, or with +infinity in a
+// softmax, has NaN weights, a row without scores (every chosen logit -infinity) weights of 0.  Scores up to e^-700, which masks make rather than routers, are 0.
 // Above, renormalised weights keep their ratio also where fp32 has no numbers for the scores: where the chosen ones' sum is below 2^-24
 // they are exp(l - the largest chosen l), which is a softmax's ratio exactly and a sigmoid's but for its factor 1 + exp(l) < 1 + 2^-24.
 //
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(const RoutePara
     bool nan = false;
 #pragma unroll
     for (int v = 0; v < V; v++) nan |= l[v] != l[v];
-    const bool any_nan = __ballot(nan) != 0;
+    bool lost = __ballot(nan) != 0;   // whether the row has no weights
 
     float top = 0.f;   // the softmax's largest logit
     if (!s.sigmoid) {
@@ -370,6 +370,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(const RoutePara
 #pragma unroll
         for (int v = 0; v < V; v++) m = max(m, order_key(l[v]));
         top = from_key(wave_max(m));
+        lost |= top == __builtin_inff();
     }
     auto part = [&](float x) { return x == -__builtin_inff() ? 0.f : exp_of(x - top); };
     int my_id;
@@ -481,7 +482,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(const RoutePara
     const int kept = s.top_k + s.shared;
     const size_t out = (size_t)token * kept;
     if (lane < s.top_k) {
-        s.weights[out + lane] = any_nan ? __builtin_nanf("") : w;
+        s.weights[out + lane] = lost ? __builtin_nanf("") : w;
         s.ids[out + lane] = my_id;
     }
     for (int i = lane; i < s.shared; i += 64) {

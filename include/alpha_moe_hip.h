@@ -270,9 +270,10 @@ int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale, const uint
  *   with num_groups > 1 only experts of the top_groups best of num_groups equal runs of experts stay, a run being worth the sum of its
  *   two largest choices (its largest if bias is NULL); then the top_k largest choices, descending, equal ones by ascending index.
  *   weights s, divided by their sum if renormalize != 0; the last shared_experts columns are E, E + 1, ... with shared_weight.
- * A NaN choice ranks as -infinity and every id is valid; a row that holds a NaN logit has NaN weights; a row whose chosen scores
- * are all 0 has weights of 0.  Scores up to e^-700 are 0.  Above, renormalised weights keep their ratio where all chosen scores are
- * below fp32's numbers; beside larger ones, and without renormalisation, a score below 2^-126 may count as 0.
+ * A NaN choice ranks as -infinity and every id is valid; a row that holds a NaN logit, or +infinity in a softmax, has NaN weights;
+ * a row whose chosen scores are all 0 has weights of 0.  Scores up to e^-700 are 0.  Above, renormalised weights keep their ratio
+ * where all chosen scores are below fp32's numbers; beside larger ones, and without renormalisation, a score below 2^-126 may
+ * count as 0.
  * M < 2^26, E <= 4096, top_k <= 64, num_groups <= 64, top_k <= top_groups * E / num_groups.
  */
 int alpha_moe_route_topk(const void *logits, int is_f32, const float *bias, float *topk_weights, int32_t *topk_ids, int M, int E,

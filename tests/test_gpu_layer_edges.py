@@ -99,3 +99,23 @@ def test_softmax_weights_of_experts_far_below_the_largest_keep_their_ratio(E, dt
         which = (logits[m].float() == best[m]).nonzero().flatten()
         one[which] = 0.5
         assert_far_route(logits[m:m + 1], min(8, which.numel()), bias=one)
+
+
+# ---- infinities --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("E", [16, 64, 256, 1100])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_softmax_rows_with_an_infinite_logit_have_no_weights(E, renormalize):
+    """infinity minus infinity: the row's weights are NaN, whichever experts a bias or the masked others make it visit"""
+    from alpha_moe_python import layer_hip
+    logits = torch.randn((4, E), generator=torch.Generator().manual_seed(E))
+    logits[0, 2:] = -math.inf
+    logits[0, 1] = math.inf
+    logits[1, 5] = math.inf
+    logits[2, 3:] = -math.inf
+    bias = 0.1 * torch.randn(E, generator=torch.Generator().manual_seed(E + 1))
+    for b in (None, bias.to(DEV)):
+        for top_k in (1, 8):
+            w, ids = layer_hip.route_topk(logits.to(DEV), top_k, bias=b, renormalize=renormalize, shared_experts=1, shared_weight=0.5)
+            assert bool(w[:2, :top_k].isnan().all()) and bool(w[2:].isfinite().all()) and bool((w[:, top_k] == 0.5).all())
+            ids = ids.cpu()
+            assert bool(((ids[:, :top_k] >= 0) & (ids[:, :top_k] < E)).all()) and all(len(set(r.tolist())) == top_k + 1 for r in ids)
