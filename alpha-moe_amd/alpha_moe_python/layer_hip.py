@@ -8,7 +8,7 @@ products of its dense layers.  Callers of the reference take these from their se
 
 HIP kernels on the current stream of the inputs' device; nothing is kept between calls, so they may be captured into HIP graphs
 and run on several streams at once.  Inputs are contiguous.  Inference only: inputs that require gradients are refused while
-gradients are recorded.
+gradients are recorded, and inputs that carry a forward-mode tangent wherever tangents are, in a trace too.
 """
 from typing import NamedTuple, Optional, Tuple
 

@@ -8,10 +8,12 @@
 //   * the device guard is installed before the stream is fetched;
 //   * a refused launch or an unsupported knob raises instead of printing or doing nothing.
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <torch/library.h>
 
 #include "../../include/alpha_moe_hip.h"
@@ -19,8 +21,10 @@
 #include <hip/hip_runtime_api.h>
 
 #include <algorithm>
+#include <cstring>
 #include <map>
 #include <mutex>
+#include <string>
 #include <tuple>
 #include <utility>
 #include <vector>
@@ -420,13 +424,6 @@ int is_f32_or_bf16(const at::Tensor &t, const char *name)
     return t.scalar_type() == at::kFloat;
 }
 
-// These operators have no backward pass; a gradient that somebody waits for would be missing without a word.
-void check_inference(const at::Tensor &t, const char *name)
-{
-    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name, " requires a gradient, and this operator has none: call it "
-                "under torch.no_grad() or torch.inference_mode()");
-}
-
 // y = rms_norm(x + residual) * weight quantised as above, and - where they are asked for, otherwise undefined - the sum and y in x's
 // type.
 struct NormQuant {
@@ -446,9 +443,7 @@ NormQuant run_norm(const at::Tensor &x, const at::Tensor *residual, const at::Te
     TORCH_CHECK(M <= INT32_MAX, "too many rows");
     check_tensor(weight, "weight", weight.scalar_type(), dev);
     TORCH_CHECK(weight.dim() == 1 && weight.size(0) == K, "weight must be [K]");
-    check_inference(x, "x"), check_inference(weight, "weight");
     if (residual) {
-        check_inference(*residual, "residual");
         check_tensor(*residual, "residual", x.scalar_type(), dev);
         TORCH_CHECK(residual->sizes() == x.sizes(), "residual must have the shape of x");
     }
@@ -502,7 +497,6 @@ std::tuple<at::Tensor, at::Tensor> swiglu_quant_fp8(const at::Tensor &gate_up, i
     const int is_f32 = is_f32_or_bf16(gate_up, "gate_up");
     check_tensor(gate_up, "gate_up", gate_up.scalar_type(), dev);
     TORCH_CHECK(gate_up.dim() == 2 && gate_up.size(1) > 0 && gate_up.size(1) % 256 == 0, "gate_up must be [M, 2 I] with I % 128 == 0");
-    check_inference(gate_up, "gate_up");
     const int64_t M = gate_up.size(0), I = gate_up.size(1) / 2;
     TORCH_CHECK(M <= INT32_MAX && I <= INT32_MAX / 2, "sizes exceed int32");
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
@@ -533,7 +527,6 @@ at::Tensor block_scaled_mm(const at::Tensor &x, const at::Tensor &x_scale, const
     TORCH_CHECK(x_scale.dim() == 2 && x_scale.size(0) == M && x_scale.size(1) == K / 128, "x_scale must be [M, K/128]");
     TORCH_CHECK(w_scale.dim() == 2 && w_scale.size(0) == (N + 127) / 128 && w_scale.size(1) == K / 128,
                 "w_scale must be [ceil(N/128), K/128]");
-    check_inference(x, "x"), check_inference(x_scale, "x_scale"), check_inference(w, "w"), check_inference(w_scale, "w_scale");
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
     at::Tensor out = empty_on(dev, {M, N}, at::kBFloat16);
@@ -561,9 +554,7 @@ std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor &logits, const c1
     if (bias.has_value()) {
         check_tensor(*bias, "bias", at::kFloat, dev);
         TORCH_CHECK(bias->dim() == 1 && bias->size(0) == E, "bias must be [E]");
-        check_inference(*bias, "bias");
     }
-    check_inference(logits, "logits");
     TORCH_CHECK(top_k > 0 && top_k <= 64 && top_k <= E, "top_k must be in [1, min(E, 64)]");
     TORCH_CHECK(num_groups > 0 && num_groups <= 64 && E % num_groups == 0, "num_groups must divide the experts, at most 64");
     TORCH_CHECK(top_groups > 0 && top_groups <= num_groups, "top_groups must be in [1, num_groups]");
@@ -581,6 +572,54 @@ std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor &logits, const c1
     return {weights, ids};
 }
 
+// These operators have no derivatives; a gradient or a tangent that somebody waits for would be missing without a word.  They are
+// refused at the dispatcher's Autograd key: below it a transform's inputs (torch.func) are ordinary tensors, and there tracing with
+// fake tensors is refused as well.
+void refuse_derivatives(const at::Tensor &t, const c10::Argument &arg)
+{
+    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), arg.name(), " requires a gradient, and this operator has none: call "
+                "it under torch.no_grad() or torch.inference_mode()");
+    TORCH_CHECK(!(t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()), arg.name(),
+                " carries a tangent, and this operator has no derivative: call it on torch.autograd.forward_ad.unpack_dual(", arg.name(),
+                ").primal");
+}
+void refuse_derivatives(const c10::optional<at::Tensor> &t, const c10::Argument &arg)
+{
+    if (t.has_value()) refuse_derivatives(*t, arg);
+}
+template <typename T>
+void refuse_derivatives(const T &, const c10::Argument &)
+{
+}
+
+template <auto Op, typename Signature = decltype(Op)>
+struct InferenceOnly;
+template <auto Op, typename R, typename... Args>
+struct InferenceOnly<Op, R (*)(Args...)> {
+    static c10::OperatorName &name()   // (made at its first use: define() runs among the library's static initialisers)
+    {
+        static c10::OperatorName n{"", ""};
+        return n;
+    }
+    static R call(c10::DispatchKeySet keys, Args... args)
+    {
+        static const auto handle = c10::Dispatcher::singleton().findSchemaOrThrow(name().name.c_str(), name().overload_name.c_str());
+        static const auto op = handle.template typed<R(Args...)>();
+        size_t i = 0;
+        (refuse_derivatives(args, handle.schema().arguments()[i++]), ...);
+        return op.redispatch(keys & c10::after_autograd_keyset, std::forward<Args>(args)...);
+    }
+    static void define(torch::Library &m, const char *schema)
+    {
+        const std::string full(schema, std::strchr(schema, '('));
+        const size_t dot = full.find('.');
+        name() = {"alpha_moe::" + full.substr(0, dot), dot == std::string::npos ? "" : full.substr(dot + 1)};
+        m.def(schema);
+        m.impl(full.c_str(), c10::DispatchKey::CUDA, Op);
+        m.impl(full.c_str(), c10::DispatchKey::Autograd, TORCH_FN(call));
+    }
+};
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(alpha_moe, m)
@@ -595,23 +634,19 @@ TORCH_LIBRARY_FRAGMENT(alpha_moe, m)
     m.def("fused_experts(Tensor(a!) hidden_states, Tensor topk_ids, Tensor w, Tensor w_scale, Tensor w2, Tensor w2_scale, "
           "Tensor topk_weights, int group_size, int block_m, int block_n, int warp_n, int stages, float scaling_factor) -> ()");
     m.impl("fused_experts", c10::DispatchKey::CUDA, &fused_experts);
-    m.def("rms_norm_quant_fp8(Tensor x, Tensor weight, float eps, int group_size) -> (Tensor, Tensor)");
-    m.impl("rms_norm_quant_fp8", c10::DispatchKey::CUDA, &rms_norm_quant_fp8);
-    m.def("rms_norm_quant_fp8.keep_norm(Tensor x, Tensor weight, float eps, int group_size) -> (Tensor, Tensor, Tensor)");
-    m.impl("rms_norm_quant_fp8.keep_norm", c10::DispatchKey::CUDA, &rms_norm_quant_fp8_keep);
-    m.def("add_rms_norm_quant_fp8(Tensor x, Tensor residual, Tensor weight, float eps, int group_size) -> "
-          "(Tensor, Tensor, Tensor)");
-    m.impl("add_rms_norm_quant_fp8", c10::DispatchKey::CUDA, &add_rms_norm_quant_fp8);
-    m.def("add_rms_norm_quant_fp8.keep_norm(Tensor x, Tensor residual, Tensor weight, float eps, int group_size) -> "
-          "(Tensor, Tensor, Tensor, Tensor)");
-    m.impl("add_rms_norm_quant_fp8.keep_norm", c10::DispatchKey::CUDA, &add_rms_norm_quant_fp8_keep);
-    m.def("swiglu_quant_fp8(Tensor gate_up, int group_size) -> (Tensor, Tensor)");
-    m.impl("swiglu_quant_fp8", c10::DispatchKey::CUDA, &swiglu_quant_fp8);
-    m.def("block_scaled_mm(Tensor x, Tensor x_scale, Tensor w, Tensor w_scale) -> Tensor");
-    m.impl("block_scaled_mm", c10::DispatchKey::CUDA, &block_scaled_mm);
-    m.def("route_topk(Tensor logits, Tensor? bias, int top_k, bool sigmoid, int num_groups, int top_groups, bool renormalize, "
-          "int shared_experts, float shared_weight) -> (Tensor, Tensor)");
-    m.impl("route_topk", c10::DispatchKey::CUDA, &route_topk);
+    InferenceOnly<&rms_norm_quant_fp8>::define(m, "rms_norm_quant_fp8(Tensor x, Tensor weight, float eps, int group_size) -> (Tensor, Tensor)");
+    InferenceOnly<&rms_norm_quant_fp8_keep>::define(
+        m, "rms_norm_quant_fp8.keep_norm(Tensor x, Tensor weight, float eps, int group_size) -> (Tensor, Tensor, Tensor)");
+    InferenceOnly<&add_rms_norm_quant_fp8>::define(
+        m, "add_rms_norm_quant_fp8(Tensor x, Tensor residual, Tensor weight, float eps, int group_size) -> (Tensor, Tensor, Tensor)");
+    InferenceOnly<&add_rms_norm_quant_fp8_keep>::define(
+        m, "add_rms_norm_quant_fp8.keep_norm(Tensor x, Tensor residual, Tensor weight, float eps, int group_size) -> "
+           "(Tensor, Tensor, Tensor, Tensor)");
+    InferenceOnly<&swiglu_quant_fp8>::define(m, "swiglu_quant_fp8(Tensor gate_up, int group_size) -> (Tensor, Tensor)");
+    InferenceOnly<&block_scaled_mm>::define(m, "block_scaled_mm(Tensor x, Tensor x_scale, Tensor w, Tensor w_scale) -> Tensor");
+    InferenceOnly<&route_topk>::define(
+        m, "route_topk(Tensor logits, Tensor? bias, int top_k, bool sigmoid, int num_groups, int top_groups, bool renormalize, "
+           "int shared_experts, float shared_weight) -> (Tensor, Tensor)");
     m.def("reserve_workspace(Tensor like, int bytes) -> ()");
     m.impl("reserve_workspace", c10::DispatchKey::CUDA, &reserve_workspace);
     m.def("scratch_buffers(Tensor like) -> int[]");

@@ -104,6 +104,65 @@ def test_fake_implementations_give_the_shapes():
     assert w.shape == ids.shape == (3, 7) and w.dtype == torch.float32 and ids.dtype == torch.int32
 
 
+def inference_calls(make, grad):
+    """``(what, call)`` of every operator, with one input at a time put through ``grad``."""
+    x, w = make((3, 512), torch.bfloat16), make((512,), torch.float32)
+    q, s = make((3, 512), torch.float8_e4m3fn), make((3, 4), torch.float32)
+    mw, ms = make((100, 512), torch.float8_e4m3fn), make((1, 4), torch.float32)
+    logits, bias = make((3, 64), torch.float32), make((64,), torch.float32)
+    H = layer_hip
+    for keep in (False, True):
+        yield "x", lambda: H.rms_norm_quant_fp8(grad(x), w, keep_norm=keep)
+        yield "weight", lambda: H.rms_norm_quant_fp8(x, grad(w), keep_norm=keep)
+        yield "x", lambda: H.rms_norm_quant_fp8(grad(x), w, residual=x, keep_norm=keep)
+        yield "residual", lambda: H.rms_norm_quant_fp8(x, w, residual=grad(x), keep_norm=keep)
+        yield "weight", lambda: H.rms_norm_quant_fp8(x, grad(w), residual=x, keep_norm=keep)
+    yield "gate_up", lambda: H.swiglu_quant_fp8(grad(x))
+    yield "x_scale", lambda: H.block_scaled_mm(q, grad(s), mw, ms)
+    yield "w_scale", lambda: H.block_scaled_mm(q, s, mw, grad(ms))
+    yield "logits", lambda: H.route_topk(grad(logits), 4, bias=bias)
+    yield "logits", lambda: H.route_topk(grad(logits), 4)
+    yield "bias", lambda: H.route_topk(logits, 4, bias=grad(bias))
+
+
+def on_meta(shape, dtype):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+def test_inputs_that_require_gradients_are_refused_while_tracing_too():
+    for name, call in inference_calls(on_meta, lambda t: t.detach().requires_grad_()):
+        with pytest.raises(RuntimeError, match=f"{name} requires a gradient"):
+            call()
+        with torch.no_grad():
+            call()
+        with torch.inference_mode():
+            call()
+    for _, call in inference_calls(on_meta, lambda t: t):
+        call()
+
+
+def test_inputs_with_a_forward_mode_tangent_are_refused():
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        for name, call in inference_calls(on_meta, lambda t: fwd.make_dual(t, torch.empty_like(t))):
+            with pytest.raises(RuntimeError, match=f"{name} carries a tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):    # (which stops gradients, not tangents)
+                call()
+        for _, call in inference_calls(on_meta, lambda t: t):
+            call()
+
+
+def test_transformed_functions_are_refused():
+    x, w = on_meta((3, 512), torch.float32), on_meta((512,), torch.float32)
+    with pytest.raises(RuntimeError, match="weight carries a tangent"):
+        torch.func.jvp(lambda v: layer_hip.rms_norm_quant_fp8(x, v).scale, (w,), (w,))
+    with pytest.raises(RuntimeError, match="weight requires a gradient"):
+        torch.func.grad(lambda v: layer_hip.rms_norm_quant_fp8(x, v).scale.sum())(w)
+    with pytest.raises(RuntimeError, match="logits requires a gradient"):
+        torch.func.vjp(lambda v: layer_hip.route_topk(v, 4)[0], x)
+
+
 # ---- the oracle itself -------------------------------------------------------------------------------------
 def test_oracle_norm_and_swiglu_by_hand():
     x = torch.zeros((1, 128))
