@@ -407,6 +407,7 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(const RoutePara
         };
         auto exact_keys = [&](uint64_t (&wide)[V]) {
             double sum = 1.0;
+            const float lowest = s.sigmoid ? kNoScore : top < __builtin_inff() ? top + kNoScore : -__builtin_inff();
             if (!s.sigmoid) {
                 sum = 0.0;
 #pragma unroll
@@ -416,9 +417,8 @@ __global__ __launch_bounds__(64 * kRouteWaves) void route_kernel(const RoutePara
             }
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const double x = s.sigmoid ? (double)l[v] : (double)l[v] - (double)top;
-                double d = s.sigmoid ? 1.0 / (1.0 + exp(-x)) : exp(x) / sum;
-                if (x <= kNoScore || l[v] == -__builtin_inff()) d = 0.0;
+                double d = s.sigmoid ? 1.0 / (1.0 + exp(-(double)l[v])) : exp((double)l[v] - (double)top) / sum;
+                if (l[v] <= lowest) d = 0.0;
                 const uint64_t of = order_key(d + (double)bias[v]);
                 wide[v] = e0 + v < E ? of : 0;
             }

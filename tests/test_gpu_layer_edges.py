@@ -101,6 +101,19 @@ def test_softmax_weights_of_experts_far_below_the_largest_keep_their_ratio(E, dt
         assert_far_route(logits[m:m + 1], min(8, which.numel()), bias=one)
 
 
+@pytest.mark.parametrize("E", [16, 256, 1100])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_scores_up_to_e_to_the_minus_700_are_equal(E, scoring):
+    """a bias of zeros, so that the scores alone decide, in 64 bits: down to e^-700 the larger one is first, below the lower index"""
+    logits = torch.full((3, E), -math.inf)
+    logits[:, :16] = torch.tensor([-720.0, -701, -650, -699, -698, -710, -600, -705] * 2)
+    logits[1] = logits[1].flip(0)
+    if scoring == "softmax":
+        logits[2, 8] = 0.0                           # (in the rows before, the largest is -600 itself)
+    for top_k in (1, 8, 16):
+        assert_far_route(logits, top_k, scoring=scoring, bias=torch.zeros(E))
+
+
 # ---- infinities --------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("E", [16, 64, 256, 1100])
 @pytest.mark.parametrize("renormalize", [True, False])
