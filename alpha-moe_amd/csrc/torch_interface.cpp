@@ -577,6 +577,7 @@ std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor &logits, const c1
 // fake tensors is refused as well.
 void refuse_derivatives(const at::Tensor &t, const c10::Argument &arg)
 {
+    if (t.unsafeGetTensorImpl()->autograd_meta() == nullptr) return;   // (nobody has asked for either)
     TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), arg.name(), " requires a gradient, and this operator has none: call "
                 "it under torch.no_grad() or torch.inference_mode()");
     TORCH_CHECK(!(t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()), arg.name(),
