@@ -132,3 +132,26 @@ def test_softmax_rows_with_an_infinite_logit_have_no_weights(E, renormalize):
             assert bool(w[:2, :top_k].isnan().all()) and bool(w[2:].isfinite().all()) and bool((w[:, top_k] == 0.5).all())
             ids = ids.cpu()
             assert bool(((ids[:, :top_k] >= 0) & (ids[:, :top_k] < E)).all()) and all(len(set(r.tolist())) == top_k + 1 for r in ids)
+
+
+# ---- norm --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [512, 4224])
+def test_norm_of_an_ordinary_row_beside_lost_ones(K, dtype):
+    """a NaN in one group of the weight, and rows that hold NaN, infinities and values whose squares pass fp32: the other groups of an
+    ordinary row are those of the whole row"""
+    from alpha_moe_python import layer_hip
+    x = activations(5, K, 3, dtype)
+    x[0, 5], x[1, 200], x[3, 300] = float("nan"), float("inf"), 2.0 ** 100
+    w = 1 + 0.3 * torch.randn(K, generator=torch.Generator().manual_seed(K))
+    w[130] = float("nan")
+    r = layer_hip.rms_norm_quant_fp8(x.to(DEV), w.to(DEV), keep_norm=True)
+    plain = w.clone()
+    plain[130] = 1.0                                 # (the row's length does not depend on the weight)
+    rows, cols = [2, 4], [c for c in range(K) if not 128 <= c < 256]
+    y, _ = L.rms_norm(x[rows], plain, 1e-6)
+    assert_codes(r.q[rows][:, cols], r.scale[rows][:, [0] + list(range(2, K // 128))], y[:, cols], NORM)
+    cols += [c for c in range(128, 256) if c != 130]
+    assert_within(r.norm[rows][:, cols], y[:, cols], (half_step(dtype) + NORM) * y[:, cols].abs(), "norm")
+    lost = r.q.float().cpu()[rows][:, 128:256]
+    assert bool(lost.isnan().all()) and bool(r.scale.cpu()[rows][:, 1].isnan().all()) and bool(r.norm[rows][:, 130].isnan().all())
