@@ -14,7 +14,10 @@
 // Both are bound by memory, or by the launch: MI355X, bf16, 8192 x 7168 with a residual 72.5 us (411 MB, 5.7 TB/s; a copy of a GiB 5.1),
 // 1 x 7168 3.0 us, SwiGLU of 8192 x 2 x 2048 14.0 us (84 MB, some of it from the last-level cache), 7 x 2 x 768 1.9; an empty call 2.2.
 // The norm's rows stay in registers, so that a row is read once; a group's maximum takes a few data-parallel steps in registers
-// (through shuffles, with a second pass over the row for the codes, the two took 76 and 19 us).
+// (through shuffles, with a second pass over the row for the codes, the two took 76 and 19 us).  Above 32768 columns this holds for bf16
+// rows and weights only: a lane of 1024 threads has 128 registers, and what fp32 rows (or fp32 weights of bf16 rows) need beyond
+// goes to scratch memory, 348 to 476 (136) bytes a lane.  1024 rows with a residual: bf16 of 32768, 65536 columns 42, 107 us, with a fp32
+// weight 144; fp32 98, 337 (5.6, 4.4, 3.3, 4.5, 2.6 TB/s).
 #include "moe_common.hpp"
 
 namespace alpha_moe {
@@ -136,8 +139,8 @@ struct NormParams {
     int M, K;
 };
 
-// One workgroup to a row, which stays in registers between its sum of squares and its codes: P pieces of 16 bytes a thread, all
-// loads of them in flight at once (pieces behind the row's end: its last one again, and not used).
+// One workgroup to a row, which stays in registers between its sum of squares and its codes (for the longest rows see above): P
+// pieces of 16 bytes a thread, all loads of them in flight at once (pieces behind the row's end: its last one again, and not used).
 template <typename T, typename W, int P>
 __global__ __launch_bounds__(1024) void rms_norm_kernel(const NormParams s)
 {
@@ -234,8 +237,8 @@ hipError_t launch_norm(const NormParams &s, hipStream_t stream)
     if (pieces <= 512) fn = rms_norm_kernel<T, W, 1>, per = 1;
     else if (pieces <= 2048) fn = rms_norm_kernel<T, W, 2>, per = 2;
     else if (pieces <= 4096) fn = rms_norm_kernel<T, W, 4>, per = 4;
-    else if (pieces <= 8192) fn = rms_norm_kernel<T, W, 8>, per = 8;
-    else fn = rms_norm_kernel<T, W, 16>, per = 16;
+    else if (sizeof(T) == 2 || pieces <= 8192) fn = rms_norm_kernel<T, W, 8>, per = 8;   // (K is 65536 at most)
+    else if constexpr (sizeof(T) == 4) fn = rms_norm_kernel<T, W, 16>, per = 16;
     const int threads = ((pieces + per - 1) / per + 63) & ~63;
     void *args[] = {const_cast<NormParams *>(&s)};
     return hipLaunchKernel(reinterpret_cast<const void *>(fn), dim3((unsigned)s.M), dim3((unsigned)threads), args, 0, stream);
