@@ -40,8 +40,9 @@ def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
 
     x ``[M, K]`` bf16 or fp32, K a multiple of 128 up to 65536; weight ``[K]`` bf16 or fp32; residual None or like x.  Returns
     ``q [M, K]`` float8_e4m3fn and ``scale [M, K/128]`` float32 of ``y`` (as ``per_token_group_quant_fp8`` defines them, but NaN
-    in a group that holds one; a row whose squares add up to more than fp32 holds becomes 0), ``residual`` = ``h`` in x's
-    dtype (a new tensor), and with ``keep_norm`` ``norm`` = ``y`` in x's dtype, which a router or a bf16 product reads.
+    in a group that holds one; a row whose squares add up to more than fp32 holds becomes 0, one whose squares are all below its
+    numbers is not a number if ``eps`` is 0), ``residual`` = ``h`` in x's dtype (a new tensor), and with ``keep_norm`` ``norm`` =
+    ``y`` in x's dtype, which a router or a bf16 product reads.
     """
     if residual is None:
         if not keep_norm:
@@ -55,7 +56,8 @@ def rms_norm_quant_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
 
 def swiglu_quant_fp8(gate_up: torch.Tensor, group_size: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
     """``gate_up [M, 2 I]`` bf16 or fp32, the gate in the first half of the columns (checkpoint order, not interleaved) ->
-    ``(q [M, I] float8_e4m3fn, scale [M, I/128] float32)`` of ``silu(gate) * up``, computed in fp32."""
+    ``(q [M, I] float8_e4m3fn, scale [M, I/128] float32)`` of ``silu(gate) * up``, computed in fp32 (where the silu of a gate below
+    -88.7 is -0)."""
     return _swiglu_quant_fp8(gate_up, group_size)
 
 
@@ -63,7 +65,8 @@ def block_scaled_mm(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_s
     """``out [M, N] = (x * x_scale) (w * w_scale)^T``, rounded once to bfloat16.
 
     x ``[M, K]`` float8_e4m3fn with x_scale ``[M, K/128]``; w ``[N, K]`` float8_e4m3fn with w_scale ``[ceil(N/128), K/128]``.
-    N is of any size, K a multiple of 128 up to 65536.  Bit for bit the same from run to run.
+    N is of any size, K a multiple of 128 up to 65536.  The product of two scales is taken first, in fp32, and has to be one of its
+    normal numbers or 0.  Bit for bit the same from run to run.
     """
     return _block_scaled_mm(x, x_scale, w, w_scale)
 

@@ -72,7 +72,8 @@ def norm_moe(hidden_states: torch.Tensor, residual: torch.Tensor, norm_weight: t
     product in ``gate_weight``'s type, ``[E_routed, K]``), the router picks ``top_k`` experts (``route_topk``), and the fused
     operator reads the codes.  ``w13 [E, N, K]`` and its scales are interleaved as for :func:`fused_experts`.  Experts that
     ``w13`` has beyond the gate's are shared ones: every token visits them, with a weight of 1 after the operator's
-    ``routed_scaling_factor``."""
+    ``routed_scaling_factor``.  The aligner is a launch of its own at any number of tokens (:func:`fused_experts`
+    does without up to 16), and a ``correction_bias`` that is not fp32 is converted in every call."""
     from .layer_hip import rms_norm_quant_fp8, route_topk
     from .prep_hip import moe_align_block_size
 

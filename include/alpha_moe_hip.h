@@ -250,7 +250,8 @@ int alpha_moe_rms_norm_quant_fp8(const void *x, const void *residual, const void
 
 /*
  * gate_up [M, 2 I] bf16 or (is_f32 != 0) fp32, the gate in the first I columns (not interleaved): q [M, I] and scale [M, I/128]
- * are the codes and scales of gate / (1 + exp(-gate)) * up, computed in fp32.  I % 128 == 0.
+ * are the codes and scales of gate / (1 + exp(-gate)) * up, computed in fp32 (so for gates below -88.7, where exp(-gate) is infinite, of
+ * -0 * up).  I % 128 == 0.
  */
 int alpha_moe_swiglu_quant_fp8(const void *gate_up, int is_f32, uint8_t *q, float *scale, int M, int I,
                                void *stream /* hipStream_t */);
@@ -259,6 +260,7 @@ int alpha_moe_swiglu_quant_fp8(const void *gate_up, int is_f32, uint8_t *q, floa
  * out[m, n] = sum over blocks kb of 128 columns of x_scale[m, kb] * w_scale[n / 128, kb] * (x[m, kb] . w[n, kb]), rounded once.
  *   x [M, K] fp8, x_scale [M, K/128] f32, w [N, K] fp8, w_scale [ceil(N / 128), K/128] f32, out [M, N] bf16.  K % 128 == 0,
  *   K <= 65536; any N (what takes more than 2^32 threads is refused).  Sums are taken in an order that depends on M, N and K only.
+ *   x_scale * w_scale is taken first, in fp32, and has to be one of its normal numbers or 0.
  */
 int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale, const uint8_t *w, const float *w_scale,
                               uint16_t *out, int M, int N, int K, void *stream /* hipStream_t */);
