@@ -91,6 +91,28 @@ def _route_topk_fake(logits, bias, top_k, sigmoid, num_groups, top_groups, renor
     return logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int32)
 
 
+@torch.library.register_fake("alpha_moe::sort_tokens")
+def _sort_tokens_fake(x, topk_ids, num_experts):
+    return (x.new_empty((topk_ids.numel(), x.shape[1])), topk_ids.new_empty((num_experts + 1,)), torch.empty_like(topk_ids))
+
+
+@torch.library.register_fake("alpha_moe::sort_tokens.scaled")
+def _sort_tokens_scaled_fake(x, x_scale, topk_ids, num_experts):
+    rows, offsets, row_of_slot = _sort_tokens_fake(x, topk_ids, num_experts)
+    return rows, x_scale.new_empty((topk_ids.numel(), x_scale.shape[1])), offsets, row_of_slot
+
+
+@torch.library.register_fake("alpha_moe::combine_tokens")
+def _combine_tokens_fake(rows, row_of_slot, topk_weights, scaling_factor):
+    return rows.new_empty((row_of_slot.shape[0], rows.shape[1]))
+
+
+@torch.library.register_fake("alpha_moe::combine_tokens_grad")
+def _combine_tokens_grad_fake(grad, rows, row_of_slot, topk_weights, scaling_factor, for_rows):
+    return (grad.new_empty((row_of_slot.numel() if for_rows else 0, grad.shape[1])),
+            grad.new_empty((0 if rows is None else row_of_slot.shape[0], row_of_slot.shape[1]), dtype=torch.float32))
+
+
 def fused_moe_w8a8_up_down(
     x: torch.Tensor,
     x_scale: torch.Tensor,

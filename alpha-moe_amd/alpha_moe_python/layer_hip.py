@@ -24,6 +24,9 @@ _add_norm_keep = torch.ops.alpha_moe.add_rms_norm_quant_fp8.keep_norm
 _swiglu_quant_fp8 = torch.ops.alpha_moe.swiglu_quant_fp8.default
 _block_scaled_mm = torch.ops.alpha_moe.block_scaled_mm.default
 _route_topk = torch.ops.alpha_moe.route_topk.default
+_sort_tokens = torch.ops.alpha_moe.sort_tokens.default
+_sort_tokens_scaled = torch.ops.alpha_moe.sort_tokens.scaled
+_combine_tokens = torch.ops.alpha_moe.combine_tokens.default
 
 
 class NormQuant(NamedTuple):
@@ -92,3 +95,44 @@ def route_topk(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias:
         raise ValueError(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
     return _route_topk(logits, bias, top_k, scoring == "sigmoid", num_groups, top_groups, renormalize, shared_experts,
                        shared_weight)
+
+
+class SortedTokens(NamedTuple):
+    """Result of :func:`sort_tokens`; ``scale`` is None where there were no scales."""
+    rows: torch.Tensor
+    scale: Optional[torch.Tensor]
+    offsets: torch.Tensor
+    row_of_slot: torch.Tensor
+
+
+def sort_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, x_scale: Optional[torch.Tensor] = None) -> SortedTokens:
+    """The tokens of all routing slots, sorted by expert: what a product with each expert's weights reads.
+
+    x ``[M, K]`` bf16, fp32 or float8_e4m3fn codes (K a multiple of 128) with or without ``x_scale [M, K/128]`` float32; topk_ids
+    ``[M, top_k]`` int32, top_k at most 64, at most 4096 experts.  Returns ``rows [M * top_k, K]``: x's row of every slot by ascending
+    expert, equal experts by ascending slot, and behind them a row of zeros for each slot whose id is outside ``[0, num_experts)`` (a padded
+    batch, experts of another GPU); ``scale`` in the same order; ``offsets [num_experts + 1]`` int32, the first row of each expert, the
+    last one the number of slots that have one; ``row_of_slot [M, top_k]`` int32, the slot's row r, or ``~r`` (negative) where that is one of
+    the zeros.  Nothing of it depends on anything but the inputs.
+
+    Differentiable in x where there is no x_scale: a token's gradient is its slots' sum, in fp32, rounded once; what the rows of
+    zeros are given counts for nothing.
+    """
+    if x_scale is None:
+        rows, offsets, row_of_slot = _sort_tokens(x, topk_ids, num_experts)
+        return SortedTokens(rows, None, offsets, row_of_slot)
+    return SortedTokens(*_sort_tokens_scaled(x, x_scale, topk_ids, num_experts))
+
+
+def combine_tokens(rows: torch.Tensor, row_of_slot: torch.Tensor, topk_weights: Optional[torch.Tensor] = None,
+                   scaling_factor: float = 1.0) -> torch.Tensor:
+    """``out[t] = scaling_factor * sum over s of topk_weights[t, s] * rows[row_of_slot[t, s]]``, the way back from :func:`sort_tokens`.
+
+    rows ``[M * top_k, K]`` bf16 or fp32, row_of_slot as :func:`sort_tokens` returns it, topk_weights ``[M, top_k]`` float32 or None (all 1).
+    Summed in fp32 by ascending s and rounded once, to rows' dtype.  Slots with a negative entry take no part, whatever their row and
+    weight hold; a token without any others is 0.
+
+    Differentiable in rows and topk_weights.  (row_of_slot names every row once; if it does not, sums are as written above, and
+    gradients of rows that it names twice or not at all are undefined.)
+    """
+    return _combine_tokens(rows, row_of_slot, topk_weights, scaling_factor)

@@ -37,6 +37,7 @@ HIP_SOURCES = {
     "moe_reduce.hip": [],
     "moe_prep.hip": [],
     "moe_norm.hip": [],
+    "moe_sort.hip": [],
     "moe_route.hip": [],
     "moe_mm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }

@@ -14,6 +14,7 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/AutogradState.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include "../../include/alpha_moe_hip.h"
@@ -572,17 +573,154 @@ std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor &logits, const c1
     return {weights, ids};
 }
 
-// These operators have no derivatives; a gradient or a tangent that somebody waits for would be missing without a word.  They are
+// ---- tokens sorted by expert and back --------------------------------------------------------------------------
+// (rows, scale, offsets, row_of_slot); without x_scale there is no scale.
+struct Sorted {
+    at::Tensor rows, scale, offsets, row_of_slot;
+};
+Sorted run_sort(const at::Tensor &x, const at::Tensor *x_scale, const at::Tensor &topk_ids, int64_t num_experts)
+{
+    TORCH_CHECK(x.is_cuda(), "x must be a GPU tensor");
+    const at::Device dev = x.device();
+    const bool codes = x.scalar_type() == at::kFloat8_e4m3fn;
+    TORCH_CHECK(codes || x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat,
+                "x must be bfloat16, float32 or float8_e4m3fn");
+    check_tensor(x, "x", x.scalar_type(), dev);
+    TORCH_CHECK(x.dim() == 2 && x.size(1) > 0, "x must be [M, K]");
+    const int64_t M = x.size(0), K = x.size(1);
+    TORCH_CHECK(!codes || K % 128 == 0, "the columns of codes must be a multiple of 128");
+    check_tensor(topk_ids, "topk_ids", at::kInt, dev);
+    TORCH_CHECK(topk_ids.dim() == 2 && topk_ids.size(0) == M, "topk_ids must be [M, top_k] with the M of x");
+    const int64_t top_k = topk_ids.size(1);
+    TORCH_CHECK(top_k > 0 && top_k <= 64, "top_k must be in [1, 64]");
+    TORCH_CHECK(num_experts > 0 && num_experts <= 4096, "num_experts must be in [1, 4096]");
+    TORCH_CHECK(M <= INT32_MAX && K <= INT32_MAX && M * top_k <= INT32_MAX, "sizes exceed int32");
+    if (x_scale) {
+        check_tensor(*x_scale, "x_scale", at::kFloat, dev);
+        TORCH_CHECK(codes, "x_scale goes with codes (float8_e4m3fn)");
+        TORCH_CHECK(x_scale->dim() == 2 && x_scale->size(0) == M && x_scale->size(1) == K / 128, "x_scale must be [M, K/128]");
+    }
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    Sorted r;
+    r.rows = empty_on(dev, {M * top_k, K}, x.scalar_type());
+    if (x_scale) r.scale = empty_on(dev, {M * top_k, K / 128}, at::kFloat);
+    r.offsets = empty_on(dev, {num_experts + 1}, at::kInt);
+    r.row_of_slot = empty_on(dev, {M, top_k}, at::kInt);
+    const size_t ws_bytes = alpha_moe_sort_workspace_bytes(static_cast<int>(M * top_k), static_cast<int>(num_experts));
+    at::Tensor ws;
+    if (ws_bytes > 0) ws = empty_on(dev, {static_cast<int64_t>(ws_bytes)}, at::kByte);
+    const int rc = alpha_moe_sort_tokens(
+        x.const_data_ptr(), static_cast<int>(x.element_size()), x_scale ? x_scale->const_data_ptr<float>() : nullptr,
+        topk_ids.const_data_ptr<int32_t>(), r.rows.data_ptr(), x_scale ? r.scale.data_ptr<float>() : nullptr,
+        r.offsets.data_ptr<int32_t>(), r.row_of_slot.data_ptr<int32_t>(), static_cast<int>(M), static_cast<int>(K),
+        static_cast<int>(top_k), static_cast<int>(num_experts), ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes,
+        static_cast<void *>(stream));
+    TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_sort_tokens failed: ", alpha_moe_status_string(rc));
+    return r;
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> sort_tokens(const at::Tensor &x, const at::Tensor &topk_ids, int64_t num_experts)
+{
+    Sorted r = run_sort(x, nullptr, topk_ids, num_experts);
+    return {std::move(r.rows), std::move(r.offsets), std::move(r.row_of_slot)};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> sort_tokens_scaled(const at::Tensor &x, const at::Tensor &x_scale,
+                                                                              const at::Tensor &topk_ids, int64_t num_experts)
+{
+    Sorted r = run_sort(x, &x_scale, topk_ids, num_experts);
+    return {std::move(r.rows), std::move(r.scale), std::move(r.offsets), std::move(r.row_of_slot)};
+}
+
+// What combine_tokens checks of rows and the map, and its gradient of what it reads; returns (M, top_k).
+std::pair<int64_t, int64_t> check_map(const at::Tensor &row_of_slot, const c10::optional<at::Tensor> &topk_weights, const at::Device &dev)
+{
+    check_tensor(row_of_slot, "row_of_slot", at::kInt, dev);
+    TORCH_CHECK(row_of_slot.dim() == 2 && row_of_slot.size(1) > 0 && row_of_slot.size(1) <= 64,
+                "row_of_slot must be [M, top_k] with top_k in [1, 64]");
+    TORCH_CHECK(row_of_slot.numel() <= INT32_MAX, "sizes exceed int32");
+    if (topk_weights.has_value()) {
+        check_tensor(*topk_weights, "topk_weights", at::kFloat, dev);
+        TORCH_CHECK(topk_weights->sizes() == row_of_slot.sizes(), "topk_weights must have the shape of row_of_slot");
+    }
+    return {row_of_slot.size(0), row_of_slot.size(1)};
+}
+void check_rows(const at::Tensor &rows, const at::Tensor &row_of_slot, const at::Device &dev, at::ScalarType dtype)
+{
+    check_tensor(rows, "rows", dtype, dev);
+    TORCH_CHECK(rows.dim() == 2 && rows.size(1) > 0 && rows.size(0) == row_of_slot.numel(),
+                "rows must be [M * top_k, K], one row for each entry of row_of_slot");
+    TORCH_CHECK(rows.size(1) <= INT32_MAX, "sizes exceed int32");
+}
+
+at::Tensor combine_tokens(const at::Tensor &rows, const at::Tensor &row_of_slot, const c10::optional<at::Tensor> &topk_weights,
+                          double scaling_factor)
+{
+    TORCH_CHECK(rows.is_cuda(), "rows must be a GPU tensor");
+    const at::Device dev = rows.device();
+    const int is_f32 = is_f32_or_bf16(rows, "rows");
+    const auto [M, top_k] = check_map(row_of_slot, topk_weights, dev);
+    check_rows(rows, row_of_slot, dev, rows.scalar_type());
+    const int64_t K = rows.size(1);
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    at::Tensor out = empty_on(dev, {M, K}, rows.scalar_type());
+    const int rc = alpha_moe_combine_tokens(
+        rows.const_data_ptr(), is_f32, row_of_slot.const_data_ptr<int32_t>(),
+        topk_weights.has_value() ? topk_weights->const_data_ptr<float>() : nullptr, out.data_ptr(), static_cast<int>(M),
+        static_cast<int>(K), static_cast<int>(top_k), static_cast<float>(scaling_factor), static_cast<void *>(stream));
+    TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_combine_tokens failed: ", alpha_moe_status_string(rc));
+    return out;
+}
+
+// (grad_rows, grad_weights) of combine_tokens: the weights' if there are rows, which only they need; what is not asked for has no
+// elements.
+std::tuple<at::Tensor, at::Tensor> combine_tokens_grad(const at::Tensor &grad, const c10::optional<at::Tensor> &rows,
+                                                       const at::Tensor &row_of_slot, const c10::optional<at::Tensor> &topk_weights,
+                                                       double scaling_factor, bool for_rows)
+{
+    TORCH_CHECK(grad.is_cuda(), "grad must be a GPU tensor");
+    const at::Device dev = grad.device();
+    const int is_f32 = is_f32_or_bf16(grad, "grad");
+    const auto [M, top_k] = check_map(row_of_slot, topk_weights, dev);
+    check_tensor(grad, "grad", grad.scalar_type(), dev);
+    TORCH_CHECK(grad.dim() == 2 && grad.size(0) == M && grad.size(1) > 0 && grad.size(1) <= INT32_MAX, "grad must be [M, K]");
+    const int64_t K = grad.size(1);
+    if (rows.has_value()) {
+        check_rows(*rows, row_of_slot, dev, grad.scalar_type());
+        TORCH_CHECK(rows->size(1) == K, "rows must have the columns of grad");
+    }
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    at::Tensor grad_rows = empty_on(dev, {for_rows ? M * top_k : 0, K}, grad.scalar_type());
+    at::Tensor grad_weights = empty_on(dev, {rows.has_value() ? M : 0, top_k}, at::kFloat);
+    const int rc = alpha_moe_combine_tokens_grad(
+        grad.const_data_ptr(), rows.has_value() ? rows->const_data_ptr() : nullptr, is_f32, row_of_slot.const_data_ptr<int32_t>(),
+        topk_weights.has_value() ? topk_weights->const_data_ptr<float>() : nullptr, for_rows ? grad_rows.data_ptr() : nullptr,
+        rows.has_value() ? grad_weights.data_ptr<float>() : nullptr, static_cast<int>(M), static_cast<int>(K), static_cast<int>(top_k),
+        static_cast<float>(scaling_factor), static_cast<void *>(stream));
+    TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_combine_tokens_grad failed: ", alpha_moe_status_string(rc));
+    return {grad_rows, grad_weights};
+}
+
+// Operators without derivatives; a gradient or a tangent that somebody waits for would be missing without a word.  They are
 // refused at the dispatcher's Autograd key: below it a transform's inputs (torch.func) are ordinary tensors, and there tracing with
 // fake tensors is refused as well.
+void refuse_tangent(const at::Tensor &t, const char *name)
+{
+    TORCH_CHECK(!(t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()), name,
+                " carries a tangent, and this operator has no derivative: call it on torch.autograd.forward_ad.unpack_dual(", name,
+                ").primal");
+}
+void refuse_gradient(const at::Tensor &t, const char *name)
+{
+    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name, " requires a gradient, and this operator has none: call "
+                "it under torch.no_grad() or torch.inference_mode()");
+}
 void refuse_derivatives(const at::Tensor &t, const c10::Argument &arg)
 {
     if (t.unsafeGetTensorImpl()->autograd_meta() == nullptr) return;   // (nobody has asked for either)
-    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), arg.name(), " requires a gradient, and this operator has none: call "
-                "it under torch.no_grad() or torch.inference_mode()");
-    TORCH_CHECK(!(t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode()), arg.name(),
-                " carries a tangent, and this operator has no derivative: call it on torch.autograd.forward_ad.unpack_dual(", arg.name(),
-                ").primal");
+    refuse_gradient(t, arg.name().c_str());
+    refuse_tangent(t, arg.name().c_str());
 }
 void refuse_derivatives(const c10::optional<at::Tensor> &t, const c10::Argument &arg)
 {
@@ -621,6 +759,92 @@ struct InferenceOnly<Op, R (*)(Args...)> {
     }
 };
 
+// ---- gradients of the sort and the combination -----------------------------------------------------------------
+// Each is the other's adjoint: a row's gradient goes to its token as a combination without weights, a token's to its rows with the
+// weights.  Saved are the map and, for the combination, rows and weights.  The functions below stand at the dispatcher's Autograd key;
+// where nobody waits for a gradient they are a redispatch.
+template <typename Fn>
+auto &typed_op(const char *name, const char *overload = "")
+{
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(name, overload).template typed<Fn>();
+    return op;
+}
+
+bool wants_gradient(const at::Tensor &t, const char *name)
+{
+    if (t.unsafeGetTensorImpl()->autograd_meta() == nullptr) return false;
+    refuse_tangent(t, name);
+    return t.requires_grad() && at::GradMode::is_enabled();
+}
+
+at::Tensor combine_through_dispatcher(const at::Tensor &rows, const at::Tensor &row_of_slot, const c10::optional<at::Tensor> &topk_weights,
+                                      double scaling_factor)
+{
+    return typed_op<decltype(combine_tokens)>("alpha_moe::combine_tokens").call(rows, row_of_slot, topk_weights, scaling_factor);
+}
+
+struct SortTokens : public torch::autograd::Function<SortTokens> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &topk_ids,
+                                                  int64_t num_experts)
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        const auto [rows, offsets, row_of_slot] =
+            typed_op<decltype(sort_tokens)>("alpha_moe::sort_tokens").call(x, topk_ids, num_experts);
+        ctx->save_for_backward({row_of_slot});
+        ctx->mark_non_differentiable({offsets, row_of_slot});
+        return {rows, offsets, row_of_slot};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads)
+    {
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
+        return {combine_through_dispatcher(grads[0].contiguous(), ctx->get_saved_variables()[0], c10::nullopt, 1.0), at::Tensor(),
+                at::Tensor()};
+    }
+};
+std::tuple<at::Tensor, at::Tensor, at::Tensor> sort_tokens_autograd(c10::DispatchKeySet keys, const at::Tensor &x,
+                                                                    const at::Tensor &topk_ids, int64_t num_experts)
+{
+    const bool wanted = wants_gradient(x, "x");
+    if (wanted && at::isFloat8Type(x.scalar_type())) refuse_gradient(x, "x");   // (of codes)
+    if (!wanted)
+        return typed_op<decltype(sort_tokens)>("alpha_moe::sort_tokens").redispatch(keys & c10::after_autograd_keyset, x, topk_ids, num_experts);
+    auto r = SortTokens::apply(x, topk_ids, num_experts);
+    return {r[0], r[1], r[2]};
+}
+
+struct CombineTokens : public torch::autograd::Function<CombineTokens> {
+    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &rows, const at::Tensor &row_of_slot,
+                              const c10::optional<at::Tensor> &topk_weights, double scaling_factor)
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        const bool weighted = topk_weights.has_value(), for_weights = weighted && topk_weights->requires_grad();
+        ctx->save_for_backward({for_weights ? rows : at::Tensor(), row_of_slot, weighted ? *topk_weights : at::Tensor()});
+        ctx->saved_data["scaling"] = scaling_factor;
+        return combine_through_dispatcher(rows, row_of_slot, topk_weights, scaling_factor);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads)
+    {
+        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+        const auto saved = ctx->get_saved_variables();
+        auto optional = [](const at::Tensor &t, bool there) { return there && t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
+        const bool for_rows = ctx->needs_input_grad(0), for_weights = saved[0].defined() && ctx->needs_input_grad(2);
+        const auto [rows, weights] = typed_op<decltype(combine_tokens_grad)>("alpha_moe::combine_tokens_grad")
+            .call(grads[0].contiguous(), optional(saved[0], for_weights), saved[1], optional(saved[2], true),
+                  ctx->saved_data["scaling"].toDouble(), for_rows);
+        return {for_rows ? rows : at::Tensor(), at::Tensor(), for_weights ? weights : at::Tensor(), at::Tensor()};
+    }
+};
+at::Tensor combine_tokens_autograd(c10::DispatchKeySet keys, const at::Tensor &rows, const at::Tensor &row_of_slot,
+                                   const c10::optional<at::Tensor> &topk_weights, double scaling_factor)
+{
+    const bool for_rows = wants_gradient(rows, "rows");
+    const bool for_weights = topk_weights.has_value() && wants_gradient(*topk_weights, "topk_weights");
+    if (!for_rows && !for_weights)
+        return typed_op<decltype(combine_tokens)>("alpha_moe::combine_tokens")
+            .redispatch(keys & c10::after_autograd_keyset, rows, row_of_slot, topk_weights, scaling_factor);
+    return CombineTokens::apply(rows, row_of_slot, topk_weights, scaling_factor);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(alpha_moe, m)
@@ -648,6 +872,17 @@ TORCH_LIBRARY_FRAGMENT(alpha_moe, m)
     InferenceOnly<&route_topk>::define(
         m, "route_topk(Tensor logits, Tensor? bias, int top_k, bool sigmoid, int num_groups, int top_groups, bool renormalize, "
            "int shared_experts, float shared_weight) -> (Tensor, Tensor)");
+    m.def("sort_tokens(Tensor x, Tensor topk_ids, int num_experts) -> (Tensor, Tensor, Tensor)");
+    m.impl("sort_tokens", c10::DispatchKey::CUDA, &sort_tokens);
+    m.impl("sort_tokens", c10::DispatchKey::Autograd, TORCH_FN(sort_tokens_autograd));
+    InferenceOnly<&sort_tokens_scaled>::define(
+        m, "sort_tokens.scaled(Tensor x, Tensor x_scale, Tensor topk_ids, int num_experts) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("combine_tokens(Tensor rows, Tensor row_of_slot, Tensor? topk_weights, float scaling_factor) -> Tensor");
+    m.impl("combine_tokens", c10::DispatchKey::CUDA, &combine_tokens);
+    m.impl("combine_tokens", c10::DispatchKey::Autograd, TORCH_FN(combine_tokens_autograd));
+    InferenceOnly<&combine_tokens_grad>::define(
+        m, "combine_tokens_grad(Tensor grad, Tensor? rows, Tensor row_of_slot, Tensor? topk_weights, float scaling_factor, bool for_rows) "
+           "-> (Tensor, Tensor)");
     m.def("reserve_workspace(Tensor like, int bytes) -> ()");
     m.impl("reserve_workspace", c10::DispatchKey::CUDA, &reserve_workspace);
     m.def("scratch_buffers(Tensor like) -> int[]");

@@ -282,6 +282,38 @@ int alpha_moe_route_topk(const void *logits, int is_f32, const float *bias, floa
                          int top_k, int sigmoid, int num_groups, int top_groups, int renormalize, int shared_experts,
                          float shared_weight, void *stream /* hipStream_t */);
 
+/*
+ * Tokens sorted by expert and back.  Slot t * top_k + s is expert topk_ids[t, s] of token t, top_k <= 64, num_experts <= 4096.
+ *
+ * alpha_moe_sort_tokens: x [M, K] of values of value_bytes bytes (1: FP8 codes, K % 128 == 0, with x_scale [M, K/128] or NULL; 2; 4) ->
+ *   rows [M * top_k, K]  the tokens of the slots, by ascending expert, equal experts by ascending slot; behind them a row of zeros for each
+ *                        slot whose id is outside [0, num_experts)
+ *   scale                x_scale's rows in the same order, zeros behind them (NULL exactly if x_scale is)
+ *   offsets [num_experts + 1]  the first row of each expert; the last one is the number of slots that have one
+ *   row_of_slot [M, top_k]     the slot's row r, or ~r (negative) where the row is one of the zeros
+ * More than a few thousand slots need alpha_moe_sort_workspace_bytes(M * top_k, num_experts) bytes of workspace (any contents; 0: none).
+ * M = 0 writes offsets.
+ *
+ * alpha_moe_combine_tokens: out[t] = scaling_factor * sum over s of topk_weights[t, s] * rows[row_of_slot[t, s]], summed in fp32 by ascending
+ * s, rounded once; negative entries take no part, whatever the row and the weight hold.  rows [M * top_k, K] and out [M, K] bf16 or
+ * (is_f32 != 0) fp32, topk_weights fp32 or NULL (all 1).  With NULL and a factor of 1 it is also the gradient of the sort.
+ *
+ * alpha_moe_combine_tokens_grad: from grad [M, K], of rows' type, grad_rows[row_of_slot[t, s]] = scaling_factor * topk_weights[t, s] * grad[t], 0
+ * where the entry is negative (row ~r), and grad_weights[t, s] = scaling_factor * (grad[t] . rows[row_of_slot[t, s]]), 0 for a negative entry.
+ * Either may be NULL.  row_of_slot has to name every row once, as alpha_moe_sort_tokens writes it; a row outside
+ * [0, M * top_k) is neither read nor written.
+ * M < 2^24 - 1, a row has at most 2^27 bytes.
+ */
+size_t alpha_moe_sort_workspace_bytes(int numel, int num_experts);
+int alpha_moe_sort_tokens(const void *x, int value_bytes, const float *x_scale, const int32_t *topk_ids, void *rows, float *scale,
+                          int32_t *offsets, int32_t *row_of_slot, int M, int K, int top_k, int num_experts, void *workspace,
+                          size_t workspace_bytes, void *stream /* hipStream_t */);
+int alpha_moe_combine_tokens(const void *rows, int is_f32, const int32_t *row_of_slot, const float *topk_weights, void *out, int M,
+                             int K, int top_k, float scaling_factor, void *stream /* hipStream_t */);
+int alpha_moe_combine_tokens_grad(const void *grad, const void *rows, int is_f32, const int32_t *row_of_slot,
+                                  const float *topk_weights, void *grad_rows, float *grad_weights, int M, int K, int top_k,
+                                  float scaling_factor, void *stream /* hipStream_t */);
+
 /* Human-readable text for a status code (static storage). */
 const char *alpha_moe_status_string(int status);
 

@@ -1,4 +1,4 @@
-"""The operators around the fused experts (norm, SwiGLU, block-scaled product, router) from their definitions in float64, on the
+"""The operators around the fused experts (norm, SwiGLU, block-scaled product, router, tokens sorted by expert and back) from their definitions in float64, on the
 CPU: what the tests of the HIP kernels compare with.  Written with loops where that is plainer."""
 import math
 
@@ -82,3 +82,49 @@ def route_topk(logits, top_k, scoring="softmax", bias=None, num_groups=1, top_gr
         all_ids.append(ids + list(range(E, E + shared_experts)))
     shape = (M, top_k + shared_experts)
     return torch.tensor(all_w, dtype=torch.float64).reshape(shape), torch.tensor(all_ids, dtype=torch.int64).reshape(shape)
+
+
+def sort_slots(topk_ids, num_experts):
+    """``(slots, offsets, row_of_slot)``: the slot of every row, those without an expert last; slot by slot."""
+    ids = topk_ids.flatten().tolist()
+    expert = [i if 0 <= i < num_experts else num_experts for i in ids]
+    slots = sorted(range(len(ids)), key=lambda s: (expert[s], s))
+    count = [0] * (num_experts + 1)
+    for e in expert:
+        count[e] += 1
+    offsets = [sum(count[:e]) for e in range(num_experts + 1)]
+    row = [0] * len(ids)
+    for r, s in enumerate(slots):
+        row[s] = r if expert[s] < num_experts else ~r
+    return (torch.tensor(slots, dtype=torch.int64), torch.tensor(offsets, dtype=torch.int32),
+            torch.tensor(row, dtype=torch.int32).reshape(topk_ids.shape))
+
+
+def combine_tokens(rows, row_of_slot, weights=None, scaling=1.0):
+    """``(out, size)`` in float64: the sums, and the same sums over magnitudes."""
+    M, top_k = row_of_slot.shape
+    out = torch.zeros((M, rows.shape[1]), dtype=torch.float64)
+    size = torch.zeros_like(out)
+    for s in range(top_k):
+        t = (row_of_slot[:, s] >= 0).nonzero().flatten()
+        part = rows[row_of_slot[t, s].long()].double() * scaling
+        if weights is not None:
+            part = part * weights[t, s].double()[:, None]
+        out[t] += part
+        size[t] += part.abs()
+    return out, size
+
+
+def combine_tokens_grad(grad, rows, row_of_slot, weights=None, scaling=1.0):
+    """``(grad_rows, grad_weights, size of grad_weights)`` in float64."""
+    M, top_k = row_of_slot.shape
+    grad_rows = torch.zeros(rows.shape, dtype=torch.float64)
+    grad_weights = torch.zeros((M, top_k), dtype=torch.float64)
+    size = torch.zeros_like(grad_weights)
+    for s in range(top_k):
+        t = (row_of_slot[:, s] >= 0).nonzero().flatten()
+        at, g = row_of_slot[t, s].long(), grad[t].double() * scaling
+        grad_rows[at] = g if weights is None else g * weights[t, s].double()[:, None]
+        grad_weights[t, s] = (g * rows[at].double()).sum(1)
+        size[t, s] = (g * rows[at].double()).abs().sum(1)
+    return grad_rows, grad_weights, size

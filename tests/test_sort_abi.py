@@ -1,0 +1,112 @@
+"""Tokens sorted by expert and back without a GPU: what the C ABI refuses, the fake implementations with their gradients, and the
+oracle by hand."""
+import pytest
+import torch
+
+import alpha_moe
+import alpha_moe_ops  # noqa: F401  (fake implementations)
+from alpha_moe_python import layer_hip
+from oracle import layer_oracle as L
+
+OK, NULL, SHAPE, WORKSPACE, ALIGN = 0, 1, 2, 7, 10
+A = alpha_moe.c_abi
+
+
+def sort(x=4096, size=2, scale_in=None, ids=4096, rows=4096, scale=None, offsets=4096, row_of_slot=4096, M=4, K=8, top_k=2, E=8, ws=None, nws=0):
+    return A.alpha_moe_sort_tokens(x, size, scale_in, ids, rows, scale, offsets, row_of_slot, M, K, top_k, E, ws, nws, None)
+
+
+def test_sort_refusals():
+    for kw in (dict(size=3), dict(size=8), dict(M=-1), dict(M=2 ** 24), dict(K=0), dict(top_k=0), dict(top_k=65), dict(E=0), dict(E=4097),
+               dict(size=1, K=64), dict(K=2 ** 27),
+               dict(size=2, scale_in=4096, scale=4096)):
+        assert sort(**kw) == SHAPE, kw
+    for name in ("x", "ids", "rows", "offsets", "row_of_slot"):
+        assert sort(**{name: None}) == NULL, name
+    assert sort(size=1, K=128, scale_in=4096) == NULL and sort(size=1, K=128, scale=4096) == NULL      # both or neither
+    assert sort(x=4104) == ALIGN and sort(rows=4098) == ALIGN
+    big = dict(M=40000, top_k=8, E=256)
+    need = A.alpha_moe_sort_workspace_bytes(320000, 256)
+    assert need > 0 and sort(**big) == WORKSPACE and sort(**big, ws=4096, nws=need - 1) == WORKSPACE and sort(**big, nws=need) == WORKSPACE
+    assert A.alpha_moe_sort_workspace_bytes(64, 256) == 0 and A.alpha_moe_sort_workspace_bytes(-1, 8) == 0
+    assert A.alpha_moe_sort_workspace_bytes(320000, 0) == 0
+
+
+def test_combine_refusals():
+    def call(rows=4096, at=4096, weights=4096, out=4096, M=4, K=8, top_k=2):
+        return A.alpha_moe_combine_tokens(rows, 0, at, weights, out, M, K, top_k, 1.0, None)
+    assert call(M=0) == OK and call(M=-1) == SHAPE and call(K=0) == SHAPE and call(top_k=0) == SHAPE and call(top_k=65) == SHAPE
+    assert call(M=2 ** 24) == SHAPE and call(K=2 ** 26 + 1) == SHAPE
+    assert call(rows=None) == NULL and call(at=None) == NULL and call(out=None) == NULL
+    assert call(rows=4104) == ALIGN and call(out=4104) == ALIGN
+
+    def grad(g=4096, rows=4096, at=4096, weights=4096, grad_rows=4096, grad_weights=4096, M=4, K=8, top_k=2):
+        return A.alpha_moe_combine_tokens_grad(g, rows, 0, at, weights, grad_rows, grad_weights, M, K, top_k, 1.0, None)
+    assert grad(M=0) == OK and grad(grad_rows=None, grad_weights=None) == OK
+    assert grad(M=-1) == SHAPE and grad(K=0) == SHAPE and grad(top_k=65) == SHAPE
+    assert grad(g=None) == NULL and grad(at=None) == NULL and grad(rows=None) == NULL
+    for name in ("g", "rows", "grad_rows"):
+        assert grad(**{name: 4104}) == ALIGN, name
+
+
+def meta(shape, dtype=torch.float32):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+def test_fake_implementations_and_their_gradients():
+    ids = meta((3, 2), torch.int32)
+    s = layer_hip.sort_tokens(meta((3, 256), torch.float8_e4m3fn), ids, 9, x_scale=meta((3, 2)))
+    assert s.rows.shape == (6, 256) and s.rows.dtype == torch.float8_e4m3fn and s.scale.shape == (6, 2)
+    assert s.offsets.shape == (10,) and s.row_of_slot.shape == (3, 2) and s.offsets.dtype == s.row_of_slot.dtype == torch.int32
+    x, w = meta((3, 7), torch.bfloat16).requires_grad_(), meta((3, 2)).requires_grad_()
+    s = layer_hip.sort_tokens(x, ids, 9)
+    assert s.scale is None and s.rows.requires_grad and not s.offsets.requires_grad and not s.row_of_slot.requires_grad
+    out = layer_hip.combine_tokens(s.rows, s.row_of_slot, w, 2.0)
+    assert out.shape == (3, 7) and out.dtype == torch.bfloat16
+    gx, gw = torch.autograd.grad(out, (x, w), meta((3, 7), torch.bfloat16))
+    assert gx.shape == (3, 7) and gx.dtype == torch.bfloat16 and gw.shape == (3, 2) and gw.dtype == torch.float32
+    with torch.no_grad():
+        assert not layer_hip.combine_tokens(layer_hip.sort_tokens(x, ids, 9).rows, s.row_of_slot, w).requires_grad
+
+
+def test_derivatives_that_do_not_exist_are_refused():
+    import torch.autograd.forward_ad as fwd
+    ids, at = meta((3, 2), torch.int32), meta((3, 2), torch.int32)
+    x, rows, w = meta((3, 8)), meta((6, 8)), meta((3, 2))
+    codes, scale = meta((3, 128), torch.float8_e4m3fn), meta((3, 1))
+    with pytest.raises(RuntimeError, match="x requires a gradient"):
+        layer_hip.sort_tokens(codes.detach().requires_grad_(), ids, 4)
+    with pytest.raises(RuntimeError, match="x_scale requires a gradient"):
+        layer_hip.sort_tokens(codes, ids, 4, x_scale=scale.detach().requires_grad_())
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.empty_like(t))
+        for call, name in ((lambda: layer_hip.sort_tokens(dual(x), ids, 4), "x"),
+                           (lambda: layer_hip.combine_tokens(dual(rows), at, w), "rows"),
+                           (lambda: layer_hip.combine_tokens(rows, at, dual(w)), "topk_weights")):
+            with pytest.raises(RuntimeError, match=f"{name} carries a tangent"):
+                call()
+    r, v = rows.detach().requires_grad_(), w.detach().requires_grad_()
+    out = layer_hip.combine_tokens(r, at, v)
+    with pytest.raises(RuntimeError, match="requires a gradient"):
+        torch.autograd.grad(out, (r, v), meta((3, 8)).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: layer_hip.combine_tokens(t, at, w).sum())(rows)
+
+
+def test_cpu_tensors_are_refused():
+    x, ids = torch.zeros((2, 8)), torch.zeros((2, 2), dtype=torch.int32)
+    for call in (lambda: layer_hip.sort_tokens(x, ids, 4), lambda: layer_hip.combine_tokens(torch.zeros((4, 8)), ids)):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call()
+
+
+def test_oracle_by_hand():
+    ids = torch.tensor([[2, 0], [-1, 2], [0, 3]], dtype=torch.int32)
+    slots, offsets, at = L.sort_slots(ids, 3)
+    assert slots.tolist() == [1, 4, 0, 3, 2, 5] and offsets.tolist() == [0, 2, 2, 4] and at.tolist() == [[2, 0], [~4, 3], [1, ~5]]
+    rows = torch.arange(1.0, 7.0)[:, None]
+    w = torch.tensor([[1.0, 2.0], [float("nan"), 3.0], [4.0, float("nan")]])
+    out, size = L.combine_tokens(rows, at, w, 2.0)
+    assert out.flatten().tolist() == [10.0, 24.0, 16.0] == size.flatten().tolist()
+    gr, gw, _ = L.combine_tokens_grad(torch.tensor([[1.0], [-1.0], [0.5]]), rows, at, w, 2.0)
+    assert gr.flatten().tolist() == [4.0, 4.0, 2.0, -6.0, 0.0, 0.0] and gw.tolist() == [[6.0, 2.0], [0.0, -8.0], [2.0, 0.0]]
