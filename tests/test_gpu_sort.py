@@ -320,7 +320,7 @@ def test_refusals():
             (lambda: H.sort_tokens(q[:, :64].contiguous(), ids, 4), "128"), (lambda: H.sort_tokens(q, ids, 4, x_scale=sc.half()), "dtype"),
             (lambda: H.sort_tokens(torch.zeros((4 * 128 + 1,), device=DEV)[1:].view(4, 128), ids, 4), "multiple of 16"),
             (lambda: H.combine_tokens(rows.half(), at), "bfloat16 or float32"), (lambda: H.combine_tokens(rows[:7], at), "one row for each"),
-            (lambda: H.combine_tokens(rows, at, w[:, :1]), "shape"), (lambda: H.combine_tokens(rows, at, w.bfloat16()), "dtype"),
+            (lambda: H.combine_tokens(rows, at, w[:, :1]), "contiguous"), (lambda: H.combine_tokens(rows, at, w[:3]), "shape"), (lambda: H.combine_tokens(rows, at, w.bfloat16()), "dtype"),
             (lambda: H.combine_tokens(rows, at.long()), "dtype"), (lambda: H.combine_tokens(rows, at, w.cpu()), "must be on"),
             (lambda: H.sort_tokens(q.requires_grad_(), ids, 4), "requires a gradient")):
         with pytest.raises(RuntimeError, match=message):
