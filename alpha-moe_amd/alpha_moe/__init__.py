@@ -94,6 +94,8 @@ c_abi.alpha_moe_combine_tokens.argtypes = (
 c_abi.alpha_moe_combine_tokens_grad.restype = ctypes.c_int
 c_abi.alpha_moe_combine_tokens_grad.argtypes = (
     [ctypes.c_void_p] * 2 + [ctypes.c_int] + [ctypes.c_void_p] * 4 + [ctypes.c_int] * 3 + [ctypes.c_float, ctypes.c_void_p])
+c_abi.alpha_moe_grouped_block_scaled_mm.restype = ctypes.c_int
+c_abi.alpha_moe_grouped_block_scaled_mm.argtypes = [ctypes.c_void_p] * 6 + [ctypes.c_int] * 4 + [ctypes.c_void_p]
 
 __version__ = c_abi.alpha_moe_version().decode()
 

@@ -113,6 +113,11 @@ def _combine_tokens_grad_fake(grad, rows, row_of_slot, topk_weights, scaling_fac
             grad.new_empty((0 if rows is None else row_of_slot.shape[0], row_of_slot.shape[1]), dtype=torch.float32))
 
 
+@torch.library.register_fake("alpha_moe::grouped_block_scaled_mm")
+def _grouped_block_scaled_mm_fake(x, x_scale, offsets, w, w_scale):
+    return x.new_empty((x.shape[0], w.shape[1]), dtype=torch.bfloat16)
+
+
 def fused_moe_w8a8_up_down(
     x: torch.Tensor,
     x_scale: torch.Tensor,

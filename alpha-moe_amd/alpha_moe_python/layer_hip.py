@@ -27,6 +27,7 @@ _route_topk = torch.ops.alpha_moe.route_topk.default
 _sort_tokens = torch.ops.alpha_moe.sort_tokens.default
 _sort_tokens_scaled = torch.ops.alpha_moe.sort_tokens.scaled
 _combine_tokens = torch.ops.alpha_moe.combine_tokens.default
+_grouped_block_scaled_mm = torch.ops.alpha_moe.grouped_block_scaled_mm.default
 
 
 class NormQuant(NamedTuple):
@@ -136,3 +137,15 @@ def combine_tokens(rows: torch.Tensor, row_of_slot: torch.Tensor, topk_weights: 
     gradients of rows that it names twice or not at all are undefined.)
     """
     return _combine_tokens(rows, row_of_slot, topk_weights, scaling_factor)
+
+
+def grouped_block_scaled_mm(x: torch.Tensor, x_scale: torch.Tensor, offsets: torch.Tensor, w: torch.Tensor,
+                            w_scale: torch.Tensor) -> torch.Tensor:
+    """The product of :func:`block_scaled_mm` for tokens sorted by expert: ``out[r] = (x[r] * x_scale[r]) (w[e] * w_scale[e])^T`` for the rows
+    ``offsets[e] <= r < offsets[e + 1]``, rounded once to bfloat16.
+
+    x ``[R, K]`` float8_e4m3fn, x_scale ``[R, K/128]`` and offsets ``[E + 1]`` int32 as :func:`sort_tokens` returns them (ascending, from 0
+    on; rows behind the last become 0); w ``[E, N, K]`` float8_e4m3fn in checkpoint order, w_scale ``[E, ceil(N/128), K/128]``.  N is of
+    any size, K a multiple of 128 up to 65536, E at most 4096.  Bit for bit the same from run to run.
+    """
+    return _grouped_block_scaled_mm(x, x_scale, offsets, w, w_scale)

@@ -34,6 +34,8 @@ struct MmParams {
     int M, N, K, nkb;
     int row_groups, token_groups;   // tiles of the launch
     int quads;   // 1: there are four K blocks, whose scales of a token are loaded together
+    const int32_t *offsets;   // grouped: rows [offsets[e], offsets[e + 1]) of x belong to expert e, whose weights are the e-th [N, K]
+    int E;
 };
 
 __device__ __forceinline__ int rfl(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -118,6 +120,97 @@ __device__ __forceinline__ void store4(const MmParams &p, int m, int n, v4f v)
     }
 }
 
+// ---- groups of tokens with weights of their own ---------------------------------------------------------------
+// A tile of a grouped launch: rows [lo, lo + rows) of x, `token_tile` of the group's `token_tiles`, and a group of columns; expert E
+// stands for the rows behind the last expert's, which become 0.
+struct GroupTile {
+    int expert, lo, rows, token_tile, row_group;
+};
+
+__device__ __forceinline__ int wave_scan(int v)   // inclusive sums over the wavefront
+{
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // from 1, 2, 4, 8 lanes below in the row
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // lane 15 of rows 0 and 2 to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // lane 31 to rows 2 and 3
+    return v;
+}
+
+// The tile of this workgroup, if there is one.  How many there are, only the device knows: each wavefront counts the experts' tiles,
+// a run of experts to a lane, and looks for its own.  An expert's tiles follow each other, its tiles of tokens in groups of HIGH next to each
+// other; each XCD gets a run of tiles.  Offsets are taken into [0, M], and where they do not ascend then, nobody has a tile.
+template <int TOKENS, int HIGH>
+__device__ __forceinline__ bool find_tile(const MmParams &p, GroupTile &g)
+{
+    const int lane = threadIdx.x & 63, groups = p.E + 1;
+    const int per = (groups + 63) >> 6, first = lane * per;
+    auto bound = [&](int e) { return e == 0 ? 0 : e > p.E ? p.M : min(max(p.offsets[e], 0), p.M); };
+    auto tiles_of_rows = [](int rows) { return rows > 0 ? (rows + TOKENS - 1) / TOKENS : 0; };
+    int sum = 0, from = first < groups ? bound(first) : 0;
+    bool ascend = true;
+    for (int e = first; e < min(first + per, groups); e++) {
+        const int to = bound(e + 1);
+        ascend &= to >= from;
+        sum += tiles_of_rows(to - from);
+        from = to;
+    }
+    if (!__all(ascend)) return false;
+    const int incl = wave_scan(sum);
+    const int total = __builtin_amdgcn_readlane(incl, 63) * p.row_groups, run = (total + 7) >> 3;
+    const int in_run = (int)(blockIdx.x >> 3), tile = (int)(blockIdx.x & 7) * run + in_run;
+    if (in_run >= run || tile >= total) return false;
+    const int at = tile / p.row_groups;   // among the tiles of tokens
+    const int owner = (int)__builtin_ctzll(__ballot(incl > at));
+    int before = incl - sum, e = first, rows = 0;
+    from = first < groups ? bound(first) : 0;
+    for (; e < min(first + per, groups); e++) {
+        const int to = bound(e + 1);
+        rows = to - from;
+        if (before + tiles_of_rows(rows) > at) break;
+        before += tiles_of_rows(rows);
+        from = to;
+    }
+    g.expert = __builtin_amdgcn_readlane(e, owner);
+    g.lo = __builtin_amdgcn_readlane(from, owner);
+    g.rows = __builtin_amdgcn_readlane(rows, owner);
+    const int token_tiles = tiles_of_rows(g.rows), inside = tile - __builtin_amdgcn_readlane(before, owner) * p.row_groups;
+    const int per_group = HIGH * p.row_groups, group = inside / per_group, in_group = inside - group * per_group;
+    const int high = min(token_tiles - group * HIGH, HIGH);
+    g.row_group = in_group / high;
+    g.token_tile = group * HIGH + in_group - g.row_group * high;
+    return true;
+}
+
+// What a workgroup multiplies, of a grouped launch: p becomes the expert's own product, rows [m0, p.M) and columns from c0 on.  Returns
+// false where there is nothing to multiply.
+template <int COLS, int TOKENS, int HIGH, int THREADS>
+__device__ __forceinline__ bool enter_group(MmParams &p, int &c0, int &m0)
+{
+    GroupTile g;
+    if (!find_tile<TOKENS, HIGH>(p, g)) return false;
+    c0 = g.row_group * COLS, m0 = g.token_tile * TOKENS;
+    p.M = min(g.rows, m0 + TOKENS);
+    p.out += (size_t)g.lo * p.N;
+    if (g.expert == p.E) {
+        for (int i = threadIdx.x; i < TOKENS * (COLS / 8); i += THREADS) {
+            const int m = m0 + i / (COLS / 8), n = c0 + i % (COLS / 8) * 8;
+            if (m >= p.M) break;
+            uint16_t *at = p.out + (size_t)m * p.N + n;
+            if (n + 8 <= p.N) *reinterpret_cast<any4 *>(at) = (any4){0, 0, 0, 0};
+            else
+                for (int j = 0; n + j < p.N; j++) at[j] = 0;
+        }
+        return false;
+    }
+    p.x += (size_t)g.lo * p.K;
+    p.x_scale += (size_t)g.lo * p.nkb;
+    p.w += (size_t)g.expert * p.N * p.K;
+    p.w_scale += (size_t)g.expert * ((p.N + 127) >> 7) * p.nkb;
+    return true;
+}
+
 // Few tokens: a workgroup multiplies R * 16 rows of w with T * 16 tokens, its wavefronts taking K blocks in turn, each through a
 // ring of its own in LDS (D K blocks of weights, tokens and scales), so that nobody waits for anybody until the sums over the
 // wavefronts at the end.  HALF: at most eight tokens, whose second eight places in a tile are left as they are - a matrix
@@ -149,8 +242,8 @@ struct StreamRing {
     static_assert(kBytes <= 160 * 1024, "");
 };
 
-template <int R, int T, int WAVES, int D, bool HALF>
-__global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(const MmParams p)
+template <int R, int T, int WAVES, int D, bool HALF, bool GROUPED>
+__global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(MmParams p)
 {
     typedef StreamRing<R, T, WAVES, D, HALF> Ring;
     constexpr int L = Ring::kLoads, DATA = Ring::kData;
@@ -159,11 +252,16 @@ __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(const MmParams p)
     const int n = lane & 15, q = lane >> 4;
 
     // workgroups are dealt to the eight XCDs in turn: each gets a run of tiles, token groups of one row group next to each other
-    const int tiles = p.row_groups * p.token_groups, run = (tiles + 7) >> 3;
-    const int tile = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
-    if (tile >= tiles) return;
-    const int rg = tile / p.token_groups, tg = tile - rg * p.token_groups;
-    const int c0 = rg * (R * 16), m0 = tg * (T * 16);
+    int c0, m0;
+    if constexpr (GROUPED) {
+        if (!enter_group<R * 16, HALF ? 8 : T * 16, 1 << 24, WAVES * 64>(p, c0, m0)) return;
+    } else {
+        const int tiles = p.row_groups * p.token_groups, run = (tiles + 7) >> 3;
+        const int tile = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
+        if (tile >= tiles) return;
+        const int rg = tile / p.token_groups, tg = tile - rg * p.token_groups;
+        c0 = rg * (R * 16), m0 = tg * (T * 16);
+    }
     const int K = p.K, nkb = p.nkb;
     // This wavefront's K blocks: every WAVES-th one, so that a workgroup reads on along its rows; with four tiles of tokens a run of
     // them, for the sake of the tokens' scales.  61 tokens, 2112 columns, K = 7168: with four tiles 14.4 us as a run against 16.5 in turn,
@@ -304,16 +402,30 @@ int64_t tiles_of(int M, int N, int cols, int tokens)
 // A launch has less than 2^32 threads.
 bool grid_fits(int64_t tiles, int threads) { return (tiles + 7) * threads < (int64_t(1) << 32); }
 
-template <int R, int T, int WAVES, int D, bool HALF>
-hipError_t launch_stream_mm(MmParams p, hipStream_t stream)
+// The most tiles of `tokens` rows that M rows in E groups and what is behind them have: each group that has rows may end in a short one.
+int64_t most_token_tiles(int M, int E, int tokens)
 {
-    if (!grid_fits(tiles_of(p.M, p.N, R * 16, T * 16), WAVES * 64)) return hipErrorInvalidConfiguration;
-    p.row_groups = (p.N + R * 16 - 1) / (R * 16);
-    p.token_groups = (p.M + T * 16 - 1) / (T * 16);
-    const int run = (p.row_groups * p.token_groups + 7) / 8;
+    const int64_t groups = E + 1 < M ? E + 1 : M;
+    return ((int64_t)M + groups * (tokens - 1)) / tokens;
+}
+
+template <typename Kernel>
+hipError_t launch_tiles(Kernel kernel, MmParams p, int cols, int tokens, int threads, bool grouped, hipStream_t stream)
+{
+    const int64_t token_groups = grouped ? most_token_tiles(p.M, p.E, tokens) : (p.M + (int64_t)tokens - 1) / tokens;
+    const int64_t tiles = ((int64_t)p.N + cols - 1) / cols * token_groups;
+    if (!grid_fits(tiles, threads)) return hipErrorInvalidConfiguration;
+    p.row_groups = (p.N + cols - 1) / cols;
+    p.token_groups = (int)token_groups;
+    const unsigned run = (unsigned)((tiles + 7) / 8);
     void *args[] = {&p};
-    return hipLaunchKernel(reinterpret_cast<const void *>(mm_stream_kernel<R, T, WAVES, D, HALF>), dim3((unsigned)run * 8),
-                           dim3(WAVES * 64), args, 0, stream);
+    return hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3(run * 8), dim3(threads), args, 0, stream);
+}
+
+template <int R, int T, int WAVES, int D, bool HALF, bool GROUPED = false>
+hipError_t launch_stream_mm(const MmParams &p, hipStream_t stream)
+{
+    return launch_tiles(mm_stream_kernel<R, T, WAVES, D, HALF, GROUPED>, p, R * 16, GROUPED && HALF ? 8 : T * 16, WAVES * 64, GROUPED, stream);
 }
 
 // Many tokens: WN x WM wavefronts, each with TN * 16 columns x TM * 16 tokens of a workgroup's tile, through S stages of one K
@@ -353,8 +465,8 @@ struct Tile {
     static_assert(kCols >= 128 ? (TN * 16) <= 128 : 128 % kCols == 0, "a wavefront's columns share their scales");
 };
 
-template <int TN, int TM, int WN, int WM, int S, int LOADERS>
-__global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(const MmParams p)
+template <int TN, int TM, int WN, int WM, int S, int LOADERS, bool GROUPED>
+__global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(MmParams p)
 {
     typedef Tile<TN, TM, WN, WM, S, LOADERS> T;
     __shared__ __attribute__((aligned(128))) uint8_t lds[T::kBytes];
@@ -365,14 +477,19 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(co
     const int n = lane & 15, q = lane >> 4;
 
     // each XCD gets a run of tiles, in groups of eight tiles of tokens, so that those at work at a time share rows and columns
-    const int tiles = p.row_groups * p.token_groups, run = (tiles + 7) >> 3;
-    const int tile = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
-    if (tile >= tiles) return;
     constexpr int kGroup = 8;
-    const int per_group = kGroup * p.row_groups, group = tile / per_group, in_group = tile - group * per_group;
-    const int high = p.token_groups - group * kGroup < kGroup ? p.token_groups - group * kGroup : kGroup;
-    const int rg = in_group / high, tg = group * kGroup + in_group - rg * high;
-    const int c0 = rg * T::kCols, m0 = tg * T::kTokens;
+    int c0, m0;
+    if constexpr (GROUPED) {
+        if (!enter_group<T::kCols, T::kTokens, kGroup, (T::kWaves + LOADERS) * 64>(p, c0, m0)) return;
+    } else {
+        const int tiles = p.row_groups * p.token_groups, run = (tiles + 7) >> 3;
+        const int tile = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
+        if (tile >= tiles) return;
+        const int per_group = kGroup * p.row_groups, group = tile / per_group, in_group = tile - group * per_group;
+        const int high = p.token_groups - group * kGroup < kGroup ? p.token_groups - group * kGroup : kGroup;
+        const int rg = in_group / high, tg = group * kGroup + in_group - rg * high;
+        c0 = rg * T::kCols, m0 = tg * T::kTokens;
+    }
     const int K = p.K, nkb = p.nkb;
 
     // Matrix row r of a wavefront's weight tile k is its column 4 TN (r / 4) + 4 k + r % 4, so a lane's results of all tiles are 4 TN
@@ -536,17 +653,11 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(co
     }
 }
 
-template <int TN, int TM, int WN, int WM, int S, int LOADERS>
-hipError_t launch_tile_mm(MmParams p, hipStream_t stream)
+template <int TN, int TM, int WN, int WM, int S, int LOADERS, bool GROUPED = false>
+hipError_t launch_tile_mm(const MmParams &p, hipStream_t stream)
 {
     typedef Tile<TN, TM, WN, WM, S, LOADERS> T;
-    if (!grid_fits(tiles_of(p.M, p.N, T::kCols, T::kTokens), (T::kWaves + LOADERS) * 64)) return hipErrorInvalidConfiguration;
-    p.row_groups = (p.N + T::kCols - 1) / T::kCols;
-    p.token_groups = (p.M + T::kTokens - 1) / T::kTokens;
-    const int run = (p.row_groups * p.token_groups + 7) / 8;
-    void *args[] = {&p};
-    return hipLaunchKernel(reinterpret_cast<const void *>(mm_tile_kernel<TN, TM, WN, WM, S, LOADERS>), dim3((unsigned)run * 8),
-                           dim3((T::kWaves + LOADERS) * 64), args, 0, stream);
+    return launch_tiles(mm_tile_kernel<TN, TM, WN, WM, S, LOADERS, GROUPED>, p, T::kCols, T::kTokens, (T::kWaves + LOADERS) * 64, GROUPED, stream);
 }
 
 // What a call takes.  Few tiles: the largest tile of the streaming kernel of which there are more than half as many as compute
@@ -585,6 +696,33 @@ Plan plan(int M, int N)
     return best;
 }
 
+// Of a grouped call: by the rows that an expert has on average.
+Plan grouped_plan(int M, int N, int E)
+{
+    const int mean = M / E;
+    return mean <= 4 ? kStreamHalf2 : mean <= 12 ? kStream2x1 : mean <= 24 ? kStream2x2 : mean <= 48 ? kTile128x64 : mean <= 128 ? kTile128x128 : kTile256x256;
+}
+
+template <bool G>
+int launch_plan(Plan plan, const MmParams &p, hipStream_t hs)
+{
+    hipError_t err = hipErrorInvalidValue;
+    switch (plan) {
+    case kStreamHalf1: err = launch_stream_mm<1, 1, 8, 2, true, G>(p, hs); break;
+    case kStreamHalf2: err = launch_stream_mm<2, 1, 8, 2, true, G>(p, hs); break;
+    case kStream1x1: err = launch_stream_mm<1, 1, 8, 2, false, G>(p, hs); break;
+    case kStream2x1: err = launch_stream_mm<2, 1, 4, 2, false, G>(p, hs); break;
+    case kStream2x2: err = launch_stream_mm<2, 2, 4, 2, false, G>(p, hs); break;
+    case kStream4x2: err = launch_stream_mm<4, 2, 4, 2, false, G>(p, hs); break;
+    case kStream4x4: err = launch_stream_mm<4, 4, 4, 1, false, G>(p, hs); break;
+    case kTile128x64: err = launch_tile_mm<4, 2, 2, 2, 3, 4, G>(p, hs); break;
+    case kTile128x128: err = launch_tile_mm<4, 4, 2, 2, 4, 4, G>(p, hs); break;
+    case kTile256x128: err = launch_tile_mm<4, 4, 4, 2, 3, 4, G>(p, hs); break;
+    case kTile256x256: err = launch_tile_mm<4, 8, 4, 2, 2, 0, G>(p, hs); break;
+    }
+    return err == hipSuccess ? ALPHA_MOE_OK : err == hipErrorInvalidConfiguration ? ALPHA_MOE_ERR_SHAPE : ALPHA_MOE_ERR_LAUNCH;
+}
+
 }  // namespace
 }  // namespace alpha_moe
 
@@ -602,20 +740,24 @@ extern "C" int alpha_moe_block_scaled_mm(const uint8_t *x, const float *x_scale,
     p.x = x, p.x_scale = x_scale, p.w = w, p.w_scale = w_scale, p.out = out;
     p.M = M, p.N = N, p.K = K, p.nkb = K / 128;
     p.quads = p.nkb >= 4;
-    hipStream_t hs = static_cast<hipStream_t>(stream);
-    hipError_t err = hipErrorInvalidValue;
-    switch (plan(M, N)) {
-    case kStreamHalf1: err = launch_stream_mm<1, 1, 8, 2, true>(p, hs); break;
-    case kStreamHalf2: err = launch_stream_mm<2, 1, 8, 2, true>(p, hs); break;
-    case kStream1x1: err = launch_stream_mm<1, 1, 8, 2, false>(p, hs); break;
-    case kStream2x1: err = launch_stream_mm<2, 1, 4, 2, false>(p, hs); break;
-    case kStream2x2: err = launch_stream_mm<2, 2, 4, 2, false>(p, hs); break;
-    case kStream4x2: err = launch_stream_mm<4, 2, 4, 2, false>(p, hs); break;
-    case kStream4x4: err = launch_stream_mm<4, 4, 4, 1, false>(p, hs); break;
-    case kTile128x64: err = launch_tile_mm<4, 2, 2, 2, 3, 4>(p, hs); break;
-    case kTile128x128: err = launch_tile_mm<4, 4, 2, 2, 4, 4>(p, hs); break;
-    case kTile256x128: err = launch_tile_mm<4, 4, 4, 2, 3, 4>(p, hs); break;
-    case kTile256x256: err = launch_tile_mm<4, 8, 4, 2, 2, 0>(p, hs); break;
-    }
-    return err == hipSuccess ? ALPHA_MOE_OK : err == hipErrorInvalidConfiguration ? ALPHA_MOE_ERR_SHAPE : ALPHA_MOE_ERR_LAUNCH;
+    return launch_plan<false>(plan(M, N), p, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int alpha_moe_grouped_block_scaled_mm(const uint8_t *x, const float *x_scale, const int32_t *offsets, const uint8_t *w,
+                                                 const float *w_scale, uint16_t *out, int M, int N, int K, int num_experts, void *stream)
+{
+    using namespace alpha_moe;
+    if (M < 0 || N <= 0 || K <= 0 || K % 128 != 0 || K > 128 * kMaxKBlocks || M > INT32_MAX - 255 || N > INT32_MAX - 255 ||
+        num_experts <= 0 || num_experts > 4096)
+        return ALPHA_MOE_ERR_SHAPE;
+    if (M == 0) return ALPHA_MOE_OK;
+    if (!x || !x_scale || !offsets || !w || !w_scale || !out) return ALPHA_MOE_ERR_NULL_POINTER;
+    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
+        return ALPHA_MOE_ERR_ALIGNMENT;
+    MmParams p = {};
+    p.x = x, p.x_scale = x_scale, p.w = w, p.w_scale = w_scale, p.out = out;
+    p.M = M, p.N = N, p.K = K, p.nkb = K / 128;
+    p.quads = p.nkb >= 4;
+    p.offsets = offsets, p.E = num_experts;
+    return launch_plan<true>(grouped_plan(M, N, num_experts), p, static_cast<hipStream_t>(stream));
 }

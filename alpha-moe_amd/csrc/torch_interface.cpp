@@ -540,6 +540,39 @@ at::Tensor block_scaled_mm(const at::Tensor &x, const at::Tensor &x_scale, const
     return out;
 }
 
+// out [R, N]: the block-scaled product of rows [offsets[e], offsets[e + 1]) of x [R, K] with w[e] of w [E, N, K].
+at::Tensor grouped_block_scaled_mm(const at::Tensor &x, const at::Tensor &x_scale, const at::Tensor &offsets, const at::Tensor &w,
+                                   const at::Tensor &w_scale)
+{
+    TORCH_CHECK(x.is_cuda(), "x must be a GPU tensor");
+    const at::Device dev = x.device();
+    check_tensor(x, "x", at::kFloat8_e4m3fn, dev);
+    check_tensor(x_scale, "x_scale", at::kFloat, dev);
+    check_tensor(offsets, "offsets", at::kInt, dev);
+    check_tensor(w, "w", at::kFloat8_e4m3fn, dev);
+    check_tensor(w_scale, "w_scale", at::kFloat, dev);
+    TORCH_CHECK(x.dim() == 2 && x.size(1) > 0 && x.size(1) % 128 == 0 && x.size(1) <= 65536,
+                "x must be [R, K] with K % 128 == 0 and K <= 65536");
+    const int64_t R = x.size(0), K = x.size(1);
+    TORCH_CHECK(w.dim() == 3 && w.size(2) == K && w.size(1) > 0, "w must be [E, N, K] with the K of x");
+    const int64_t E = w.size(0), N = w.size(1);
+    TORCH_CHECK(E > 0 && E <= 4096, "w must hold 1 to 4096 experts");
+    TORCH_CHECK(R <= INT32_MAX && N <= INT32_MAX, "sizes exceed int32");
+    TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) == E + 1, "offsets must be [E + 1]");
+    TORCH_CHECK(x_scale.dim() == 2 && x_scale.size(0) == R && x_scale.size(1) == K / 128, "x_scale must be [R, K/128]");
+    TORCH_CHECK(w_scale.dim() == 3 && w_scale.size(0) == E && w_scale.size(1) == (N + 127) / 128 && w_scale.size(2) == K / 128,
+                "w_scale must be [E, ceil(N/128), K/128]");
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    at::Tensor out = empty_on(dev, {R, N}, at::kBFloat16);
+    const int rc = alpha_moe_grouped_block_scaled_mm(
+        static_cast<const uint8_t *>(x.const_data_ptr()), x_scale.const_data_ptr<float>(), offsets.const_data_ptr<int32_t>(),
+        static_cast<const uint8_t *>(w.const_data_ptr()), w_scale.const_data_ptr<float>(), static_cast<uint16_t *>(out.data_ptr()),
+        static_cast<int>(R), static_cast<int>(N), static_cast<int>(K), static_cast<int>(E), static_cast<void *>(stream));
+    TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_grouped_block_scaled_mm failed: ", alpha_moe_status_string(rc));
+    return out;
+}
+
 // (topk_weights f32, topk_ids i32), both [M, top_k + shared_experts].
 std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor &logits, const c10::optional<at::Tensor> &bias, int64_t top_k,
                                               bool sigmoid, int64_t num_groups, int64_t top_groups, bool renormalize,
@@ -883,6 +916,8 @@ TORCH_LIBRARY_FRAGMENT(alpha_moe, m)
     InferenceOnly<&combine_tokens_grad>::define(
         m, "combine_tokens_grad(Tensor grad, Tensor? rows, Tensor row_of_slot, Tensor? topk_weights, float scaling_factor, bool for_rows) "
            "-> (Tensor, Tensor)");
+    InferenceOnly<&grouped_block_scaled_mm>::define(
+        m, "grouped_block_scaled_mm(Tensor x, Tensor x_scale, Tensor offsets, Tensor w, Tensor w_scale) -> Tensor");
     m.def("reserve_workspace(Tensor like, int bytes) -> ()");
     m.impl("reserve_workspace", c10::DispatchKey::CUDA, &reserve_workspace);
     m.def("scratch_buffers(Tensor like) -> int[]");

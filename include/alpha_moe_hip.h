@@ -314,6 +314,17 @@ int alpha_moe_combine_tokens_grad(const void *grad, const void *rows, int is_f32
                                   const float *topk_weights, void *grad_rows, float *grad_weights, int M, int K, int top_k,
                                   float scaling_factor, void *stream /* hipStream_t */);
 
+/*
+ * The block-scaled product of tokens sorted by expert with each expert's weights: rows [offsets[e], offsets[e + 1]) of x [M, K] with
+ * w [num_experts, N, K] and w_scale [num_experts, ceil(N / 128), K/128] -> out [M, N], otherwise as alpha_moe_block_scaled_mm.  offsets
+ * [num_experts + 1] as alpha_moe_sort_tokens writes them: ascending, from 0 to at most M (rows behind the last one become 0).  Others give
+ * rows that may be wrong or not written, but nothing is read or written outside the arrays.  Experts without rows cost nothing but the look at
+ * their offsets.  num_experts <= 4096.
+ */
+int alpha_moe_grouped_block_scaled_mm(const uint8_t *x, const float *x_scale, const int32_t *offsets, const uint8_t *w,
+                                      const float *w_scale, uint16_t *out, int M, int N, int K, int num_experts,
+                                      void *stream /* hipStream_t */);
+
 /* Human-readable text for a status code (static storage). */
 const char *alpha_moe_status_string(int status);
 

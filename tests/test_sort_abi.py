@@ -110,3 +110,21 @@ def test_oracle_by_hand():
     assert out.flatten().tolist() == [10.0, 24.0, 16.0] == size.flatten().tolist()
     gr, gw, _ = L.combine_tokens_grad(torch.tensor([[1.0], [-1.0], [0.5]]), rows, at, w, 2.0)
     assert gr.flatten().tolist() == [4.0, 4.0, 2.0, -6.0, 0.0, 0.0] and gw.tolist() == [[6.0, 2.0], [0.0, -8.0], [2.0, 0.0]]
+
+
+def test_grouped_refusals_and_shapes():
+    def call(x=4096, xs=4096, off=4096, w=4096, ws=4096, out=4096, M=4, N=100, K=256, E=8):
+        return A.alpha_moe_grouped_block_scaled_mm(x, xs, off, w, ws, out, M, N, K, E, None)
+    assert call(M=0) == OK and call(M=-1) == SHAPE and call(N=0) == SHAPE and call(K=0) == SHAPE and call(K=64) == SHAPE
+    assert call(K=65536 + 128) == SHAPE and call(E=0) == SHAPE and call(E=4097) == SHAPE
+    for name in ("x", "xs", "off", "w", "ws", "out"):
+        assert call(**{name: None}) == NULL, name
+    for name in ("x", "w", "out"):
+        assert call(**{name: 4104}) == ALIGN, name
+    for M, N, E in ((2 ** 31 - 1, 8, 8), (8, 2 ** 31 - 1, 8), (2 ** 30, 2 ** 30, 4096), (2 ** 31 - 300, 40, 1), (8, 2 ** 31 - 300, 8)):
+        assert call(M=M, N=N, E=E) == SHAPE, (M, N, E)
+    x, xs = meta((6, 256), torch.float8_e4m3fn), meta((6, 2))
+    out = layer_hip.grouped_block_scaled_mm(x, xs, meta((5,), torch.int32), meta((4, 100, 256), torch.float8_e4m3fn), meta((4, 1, 2)))
+    assert out.shape == (6, 100) and out.dtype == torch.bfloat16
+    with pytest.raises(RuntimeError, match="x_scale requires a gradient"):
+        layer_hip.grouped_block_scaled_mm(x, xs.requires_grad_(), meta((5,), torch.int32), meta((4, 100, 256), torch.float8_e4m3fn), meta((4, 1, 2)))
