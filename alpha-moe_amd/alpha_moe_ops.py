@@ -118,6 +118,11 @@ def _grouped_block_scaled_mm_fake(x, x_scale, offsets, w, w_scale):
     return x.new_empty((x.shape[0], w.shape[1]), dtype=torch.bfloat16)
 
 
+@torch.library.register_fake("alpha_moe::add_adapters")
+def _add_adapters_fake(base, x, x_scale, a, b, adapter_ids, scale):
+    return torch.empty_like(base)
+
+
 def fused_moe_w8a8_up_down(
     x: torch.Tensor,
     x_scale: torch.Tensor,

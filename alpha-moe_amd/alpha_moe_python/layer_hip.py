@@ -27,6 +27,7 @@ _route_topk = torch.ops.alpha_moe.route_topk.default
 _sort_tokens = torch.ops.alpha_moe.sort_tokens.default
 _sort_tokens_scaled = torch.ops.alpha_moe.sort_tokens.scaled
 _combine_tokens = torch.ops.alpha_moe.combine_tokens.default
+_add_adapters = torch.ops.alpha_moe.add_adapters.default
 _grouped_block_scaled_mm = torch.ops.alpha_moe.grouped_block_scaled_mm.default
 
 
@@ -149,3 +150,20 @@ def grouped_block_scaled_mm(x: torch.Tensor, x_scale: torch.Tensor, offsets: tor
     any size, K a multiple of 128 up to 65536, E at most 4096.  Bit for bit the same from run to run.
     """
     return _grouped_block_scaled_mm(x, x_scale, offsets, w, w_scale)
+
+
+def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor,
+                 scale: Optional[torch.Tensor] = None, x_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Low-rank adapters of many requests beside a shared projection: ``base[m] + scale[l] * (x[m] a[l]^T) b[l]^T`` with
+    ``l = adapter_ids[m]``; ``base[m]`` where l is outside ``[0, L)``.  A new tensor like base.
+
+    base ``[M, N]`` bf16 is the projection's result (of :func:`block_scaled_mm`, say), x ``[M, K]`` its input: bf16, or float8_e4m3fn codes
+    with ``x_scale [M, K/128]`` float32.  a ``[L, rank, K]`` and b ``[L, N, rank]`` bf16 (adapters of smaller rank padded with zeros),
+    scale ``[L]`` float32 or None (all 1), adapter_ids ``[M]`` int32 in any order (neighbours of one adapter share its reading).  K a multiple of
+    128 up to 65536, N of any size, rank a multiple of 8 up to 128, M at most 1048560.
+
+    Sums are fp32, in an order that depends on the sizes alone; the ``rank`` values between the two products are good to 2^-16; one
+    rounding at the end.  Another request's adapter or activations, whatever they hold, change nothing of a token's result.
+    What an infinity in b meets is infinite or NaN.
+    """
+    return _add_adapters(base, x, x_scale, a, b, adapter_ids, scale)

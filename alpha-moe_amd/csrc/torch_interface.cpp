@@ -573,6 +573,54 @@ at::Tensor grouped_block_scaled_mm(const at::Tensor &x, const at::Tensor &x_scal
     return out;
 }
 
+// out [M, N] = base + each token's adapter on x.
+at::Tensor add_adapters(const at::Tensor &base, const at::Tensor &x, const c10::optional<at::Tensor> &x_scale, const at::Tensor &a,
+                        const at::Tensor &b, const at::Tensor &adapter_ids, const c10::optional<at::Tensor> &scale)
+{
+    TORCH_CHECK(base.is_cuda(), "base must be a GPU tensor");
+    const at::Device dev = base.device();
+    check_tensor(base, "base", at::kBFloat16, dev);
+    check_tensor(x, "x", x_scale.has_value() ? at::kFloat8_e4m3fn : at::kBFloat16, dev);
+    check_tensor(a, "a", at::kBFloat16, dev);
+    check_tensor(b, "b", at::kBFloat16, dev);
+    check_tensor(adapter_ids, "adapter_ids", at::kInt, dev);
+    TORCH_CHECK(base.dim() == 2 && base.size(1) > 0, "base must be [M, N]");
+    const int64_t M = base.size(0), N = base.size(1);
+    TORCH_CHECK(x.dim() == 2 && x.size(0) == M && x.size(1) > 0 && x.size(1) % 128 == 0 && x.size(1) <= 65536,
+                "x must be [M, K] with the M of base, K % 128 == 0 and K <= 65536");
+    const int64_t K = x.size(1);
+    TORCH_CHECK(a.dim() == 3 && a.size(0) > 0 && a.size(2) == K, "a must be [L, rank, K] with the K of x");
+    const int64_t L = a.size(0), rank = a.size(1);
+    TORCH_CHECK(rank > 0 && rank % 8 == 0 && rank <= 128, "rank must be a multiple of 8 in [8, 128]");
+    TORCH_CHECK(b.dim() == 3 && b.size(0) == L && b.size(1) == N && b.size(2) == rank, "b must be [L, N, rank]");
+    TORCH_CHECK(adapter_ids.dim() == 1 && adapter_ids.size(0) == M, "adapter_ids must be [M]");
+    TORCH_CHECK(M <= 1048560, "at most 1048560 rows");
+    TORCH_CHECK(N <= INT32_MAX && L <= INT32_MAX, "sizes exceed int32");
+    if (x_scale.has_value()) {
+        check_tensor(*x_scale, "x_scale", at::kFloat, dev);
+        TORCH_CHECK(x_scale->dim() == 2 && x_scale->size(0) == M && x_scale->size(1) == K / 128, "x_scale must be [M, K/128]");
+    }
+    if (scale.has_value()) {
+        check_tensor(*scale, "scale", at::kFloat, dev);
+        TORCH_CHECK(scale->dim() == 1 && scale->size(0) == L, "scale must be [L]");
+    }
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
+    at::Tensor out = empty_on(dev, {M, N}, at::kBFloat16);
+    const size_t ws_bytes = alpha_moe_adapters_workspace_bytes(static_cast<int>(M), static_cast<int>(K), static_cast<int>(rank),
+                                                               static_cast<int>(L));
+    at::Tensor ws = empty_on(dev, {static_cast<int64_t>(ws_bytes)}, at::kByte);
+    const int rc = alpha_moe_add_adapters(
+        static_cast<const uint16_t *>(base.const_data_ptr()), x.const_data_ptr(),
+        x_scale.has_value() ? x_scale->const_data_ptr<float>() : nullptr, static_cast<const uint16_t *>(a.const_data_ptr()),
+        static_cast<const uint16_t *>(b.const_data_ptr()), adapter_ids.const_data_ptr<int32_t>(),
+        scale.has_value() ? scale->const_data_ptr<float>() : nullptr, static_cast<uint16_t *>(out.data_ptr()), static_cast<int>(M),
+        static_cast<int>(N), static_cast<int>(K), static_cast<int>(rank), static_cast<int>(L), ws.data_ptr(), ws_bytes,
+        static_cast<void *>(stream));
+    TORCH_CHECK(rc == ALPHA_MOE_OK, "alpha_moe_add_adapters failed: ", alpha_moe_status_string(rc));
+    return out;
+}
+
 // (topk_weights f32, topk_ids i32), both [M, top_k + shared_experts].
 std::tuple<at::Tensor, at::Tensor> route_topk(const at::Tensor &logits, const c10::optional<at::Tensor> &bias, int64_t top_k,
                                               bool sigmoid, int64_t num_groups, int64_t top_groups, bool renormalize,
@@ -918,6 +966,8 @@ TORCH_LIBRARY_FRAGMENT(alpha_moe, m)
            "-> (Tensor, Tensor)");
     InferenceOnly<&grouped_block_scaled_mm>::define(
         m, "grouped_block_scaled_mm(Tensor x, Tensor x_scale, Tensor offsets, Tensor w, Tensor w_scale) -> Tensor");
+    InferenceOnly<&add_adapters>::define(
+        m, "add_adapters(Tensor base, Tensor x, Tensor? x_scale, Tensor a, Tensor b, Tensor adapter_ids, Tensor? scale) -> Tensor");
     m.def("reserve_workspace(Tensor like, int bytes) -> ()");
     m.impl("reserve_workspace", c10::DispatchKey::CUDA, &reserve_workspace);
     m.def("scratch_buffers(Tensor like) -> int[]");

@@ -1,4 +1,4 @@
-"""The operators around the fused experts (norm, SwiGLU, block-scaled product, router, tokens sorted by expert and back) from their definitions in float64, on the
+"""The operators around the fused experts (norm, SwiGLU, block-scaled product, router, tokens sorted by expert and back, adapters) from their definitions in float64, on the
 CPU: what the tests of the HIP kernels compare with.  Written with loops where that is plainer."""
 import math
 
@@ -128,3 +128,22 @@ def combine_tokens_grad(grad, rows, row_of_slot, weights=None, scaling=1.0):
         grad_weights[t, s] = (g * rows[at].double()).sum(1)
         size[t, s] = (g * rows[at].double()).abs().sum(1)
     return grad_rows, grad_weights, size
+
+
+def add_adapters(base, x, a, b, ids, scale=None, x_scale=None):
+    """``(out, inner, outer)`` in float64: the result; the adapters' part with magnitudes all the way through (what rounding errors of the
+    first product's additions go by); and the second product's sums over magnitudes."""
+    out = base.double().clone()
+    inner, outer = torch.zeros_like(out), torch.zeros_like(out)
+    xd = x.double()
+    if x_scale is not None:
+        xd = xd * x_scale.double().repeat_interleave(GROUP, 1)
+    for m, l in enumerate(ids.tolist()):
+        if 0 <= l < a.shape[0]:
+            s = 1.0 if scale is None else scale[l].item()
+            al, bl = a[l].double(), b[l].double()
+            v = al @ xd[m] * s
+            out[m] += bl @ v
+            inner[m] = bl.abs() @ (al.abs() @ xd[m].abs()) * abs(s)
+            outer[m] = bl.abs() @ v.abs()
+    return out, inner, outer

@@ -128,3 +128,39 @@ def test_grouped_refusals_and_shapes():
     assert out.shape == (6, 100) and out.dtype == torch.bfloat16
     with pytest.raises(RuntimeError, match="x_scale requires a gradient"):
         layer_hip.grouped_block_scaled_mm(x, xs.requires_grad_(), meta((5,), torch.int32), meta((4, 100, 256), torch.float8_e4m3fn), meta((4, 1, 2)))
+
+
+def test_adapter_refusals_and_shapes():
+    def call(base=4096, x=4096, xs=None, a=4096, b=4096, ids=4096, scale=None, out=4096, M=4, N=100, K=256, rank=16, L=8, ws=4096, nws=1 << 40):
+        return A.alpha_moe_add_adapters(base, x, xs, a, b, ids, scale, out, M, N, K, rank, L, ws, nws, None)
+    assert call(M=0) == OK and call(M=-1) == SHAPE and call(N=0) == SHAPE and call(K=0) == SHAPE and call(K=64) == SHAPE
+    assert call(K=65536 + 128) == SHAPE and call(L=0) == SHAPE and call(M=1048561) == SHAPE and call(N=2 ** 31 - 1) == SHAPE
+    for rank in (0, -8, 4, 12, 136):
+        assert call(rank=rank) == SHAPE, rank
+    for name in ("base", "x", "a", "b", "ids", "out"):
+        assert call(**{name: None}) == NULL, name
+    for name in ("base", "x", "a", "b", "out"):
+        assert call(**{name: 4104}) == ALIGN, name
+    need = A.alpha_moe_adapters_workspace_bytes(4, 256, 16, 8)
+    assert need >= 4 * 16 * 4 and call(ws=None) == WORKSPACE and call(ws=4104) == WORKSPACE and call(nws=need - 1) == WORKSPACE
+    assert A.alpha_moe_adapters_workspace_bytes(0, 256, 16, 8) == 0 and A.alpha_moe_adapters_workspace_bytes(4, 256, 15, 8) == 0
+    base, x, ids = meta((6, 100), torch.bfloat16), meta((6, 256), torch.bfloat16), meta((6,), torch.int32)
+    a, b = meta((3, 16, 256), torch.bfloat16), meta((3, 100, 16), torch.bfloat16)
+    out = layer_hip.add_adapters(base, x, a, b, ids, scale=meta((3,)))
+    assert out.shape == (6, 100) and out.dtype == torch.bfloat16
+    for i, name in enumerate(("base", "x", "a", "b")):
+        args = [base, x, a, b]
+        args[i] = args[i].detach().requires_grad_()
+        with pytest.raises(RuntimeError, match=f"{name} requires a gradient"):
+            layer_hip.add_adapters(*args, ids)
+
+
+def test_oracle_of_adapters_by_hand():
+    base, x = torch.ones((3, 2)), torch.zeros((3, 128))
+    x[:, 0] = torch.tensor([1.0, 2.0, -3.0])
+    a, b = torch.zeros((2, 8, 128)), torch.zeros((2, 2, 8))
+    a[0, 0, 0], a[1, 3, 0] = 2.0, 1.0
+    b[0, :, 0], b[1, :, 3] = torch.tensor([1.0, -1.0]), torch.tensor([0.5, 4.0])
+    out, inner, outer = L.add_adapters(base, x, a, b, torch.tensor([0, 5, 1]), torch.tensor([10.0, -1.0]))
+    assert out.tolist() == [[21.0, -19.0], [1.0, 1.0], [2.5, 13.0]]
+    assert inner.tolist() == [[20.0, 20.0], [0.0, 0.0], [1.5, 12.0]] == outer.tolist()
