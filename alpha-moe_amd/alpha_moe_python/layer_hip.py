@@ -160,7 +160,7 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     base ``[M, N]`` bf16 is the projection's result (of :func:`block_scaled_mm`, say), x ``[M, K]`` its input: bf16, or float8_e4m3fn codes
     with ``x_scale [M, K/128]`` float32.  a ``[L, rank, K]`` and b ``[L, N, rank]`` bf16 (adapters of smaller rank padded with zeros),
     scale ``[L]`` float32 or None (all 1), adapter_ids ``[M]`` int32 in any order (neighbours of one adapter share its reading).  K a multiple of
-    128 up to 65536, N of any size, rank a multiple of 8 up to 128, M at most 1048560.
+    128 up to 65536, N at most 2^24, rank a multiple of 8 up to 128, M at most 1048560.
 
     Sums are fp32, in an order that depends on the sizes alone; the ``rank`` values between the two products are good to 2^-16; one
     rounding at the end.  Another request's adapter or activations, whatever they hold, change nothing of a token's result.

@@ -38,7 +38,7 @@ HIP_SOURCES = {
     "moe_prep.hip": [],
     "moe_norm.hip": [],
     "moe_sort.hip": [],
-    "moe_adapt.hip": [],
+    "moe_adapt.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "moe_route.hip": [],
     "moe_mm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }

@@ -19,7 +19,7 @@ namespace alpha_moe {
 namespace {
 
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));   // rows of an odd N start at any multiple of two bytes
+typedef uint32_t v4w __attribute__((ext_vector_type(4)));
 
 constexpr int kMaxRank = 128;
 
@@ -30,8 +30,42 @@ struct AdaptParams {
     const int32_t *ids;
     uint16_t *out;
     float *part;               // [splits][M][rank]
-    int M, N, K, rank, adapters, nkb, splits, sharers;
+    int M, N, K, rank, adapters, nkb, splits, sharers, run, tiles, pieces;
 };
+
+// LDS accesses of one wavefront complete in order; this keeps the compiler to the written order
+__device__ __forceinline__ void lds_order()
+{
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Workgroups are dealt to the eight XCDs in turn: each gets a run of tiles, so that an adapter's a and b are read into few of their L2s
+//.  A tile's workgroups: `pieces` times `sharers`.
+struct Place {
+    int tile, piece, turn;
+};
+__device__ __forceinline__ bool find_place(int tiles, int pieces, Place &at)
+{
+    // (the sharers behind each other: most of a tile's have nothing to do, and every so-many-th workgroup is the same few compute units')
+    const int all = tiles * pieces, run = (all + 7) >> 3, in_run = (int)(blockIdx.x >> 3);
+    at.turn = in_run / run;
+    const int i = (int)(blockIdx.x & 7) * run + in_run - at.turn * run;
+    if (i >= all) return false;
+    at.tile = i / pieces;
+    at.piece = i - at.tile * pieces;
+    return true;
+}
+
+// A buffer at a wavefront-uniform base: loads behind its end give 0.  (Rows of an odd N start at any multiple of two bytes, and memory
+// takes 16 bytes there as a whole.)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void *uniform_base, uint32_t bytes)
+{
+    const uint64_t v = reinterpret_cast<uint64_t>(uniform_base);
+    const uint64_t u = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32)) << 32) |
+                       (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(u), 0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
+}
 
 // The distinct adapters of a tile of tokens, in the order of their first tokens: f(adapter, tokens that have it), every `sharers`-th one.
 template <typename F>
@@ -70,40 +104,43 @@ __global__ __launch_bounds__(256) void adapt_in_kernel(const AdaptParams p)
     __shared__ v4f sums[4][RT * T][64];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, q = lane >> 4;
-    const int m0 = blockIdx.x * (16 * T), split = blockIdx.y;
+    Place place;
+    if (!find_place(p.tiles, p.splits, place)) return;
+    const int m0 = place.tile * (16 * T), split = place.piece;
     const int first = (int)((int64_t)split * p.nkb / p.splits), last = (int)((int64_t)(split + 1) * p.nkb / p.splits);
     const int id = lane < 16 * T && m0 + lane < p.M ? p.ids[m0 + lane] : -1;
     const int K = p.K;
     int token[T];
 #pragma unroll
     for (int t = 0; t < T; t++) token[t] = min(m0 + 16 * t + n, p.M - 1);
-    for_each_adapter(id, p.adapters, blockIdx.z, p.sharers, [&](int adapter, unsigned long long same) {
+    for_each_adapter(id, p.adapters, place.turn, p.sharers, [&](int adapter, unsigned long long same) {
         const uint16_t *a = p.a + (size_t)adapter * p.rank * K;
         v4f acc[RT][T] = {};
         for (int kb = first + w; kb < last; kb += 4) {
-            // lane (n, q) has the 32 columns [32 q, 32 q + 32) of the block, of rank n's row and of token n's
+            // lane (n, q) has columns [16 q, 16 q + 16) of either half of the block, of rank n's row and of token n's: a load of all lanes
+            // is sixteen lines (any other share of the columns made it thirty-two, and lines are what the path into a compute unit counts)
             v8bf av[RT][4], xv[T][4];
 #pragma unroll
             for (int r = 0; r < RT; r++) {
-                const v8bf *at = reinterpret_cast<const v8bf *>(a + (size_t)min(16 * r + n, p.rank - 1) * K + kb * 128 + q * 32);
+                const v8bf *at = reinterpret_cast<const v8bf *>(a + (size_t)min(16 * r + n, p.rank - 1) * K + kb * 128 + q * 16);
 #pragma unroll
-                for (int i = 0; i < 4; i++) av[r][i] = at[i];
+                for (int i = 0; i < 4; i++) av[r][i] = at[8 * (i / 2) + i % 2];
             }
             float f[T];
 #pragma unroll
             for (int t = 0; t < T; t++) {
                 if constexpr (FP8) {
-                    const v4i *at = reinterpret_cast<const v4i *>(p.x + (size_t)token[t] * K + kb * 128 + q * 32);
+                    const v4i *at = reinterpret_cast<const v4i *>(p.x + (size_t)token[t] * K + kb * 128 + q * 16);
                     v8bf two[2];
                     widen(at[0], two);
                     xv[t][0] = two[0], xv[t][1] = two[1];
-                    widen(at[1], two);
+                    widen(at[4], two);
                     xv[t][2] = two[0], xv[t][3] = two[1];
                     f[t] = p.x_scale[(size_t)token[t] * p.nkb + kb];
                 } else {
-                    const v8bf *at = reinterpret_cast<const v8bf *>(p.x + 2 * ((size_t)token[t] * K + kb * 128 + q * 32));
+                    const v8bf *at = reinterpret_cast<const v8bf *>(p.x + 2 * ((size_t)token[t] * K + kb * 128 + q * 16));
 #pragma unroll
-                    for (int i = 0; i < 4; i++) xv[t][i] = at[i];
+                    for (int i = 0; i < 4; i++) xv[t][i] = at[8 * (i / 2) + i % 2];
                 }
             }
 #pragma unroll
@@ -132,94 +169,181 @@ __global__ __launch_bounds__(256) void adapt_in_kernel(const AdaptParams p)
     });
 }
 
-// out: each wavefront 64 columns of T tiles of 16 tokens; STEPS matrix instructions of 32 along the two parts of the ranks.
-template <int STEPS, int T>
-__global__ __launch_bounds__(256) void adapt_out_kernel(const AdaptParams p)
+// out: each wavefront 64 columns of T tiles of 16 tokens.  Up to 16 ranks (RT = 1) their high and low parts lie behind each other in one
+// matrix instruction, and b's values twice; beyond, b's values of 32 ranks are multiplied with both.
+template <int RT, int T>
+__global__ __launch_bounds__(256, RT == 8 ? 3 : 4) void adapt_out_kernel(const AdaptParams p)
 {
-    constexpr int kRow = STEPS * 64 + 16;   // bytes of a token's parts in LDS, and 16 so that tokens' rows begin at other banks
+    constexpr int S = RT == 1 ? 1 : RT / 2, PARTS = RT == 1 ? 1 : 2;   // matrix instructions along the ranks, and for each of them
+    constexpr int kLow = RT == 1 ? 0 : 64 * S;                         // RT > 1: where the low parts of a token begin
+    constexpr int kRow = 64 * S * PARTS + 16;   // bytes of a token's parts in LDS, and 16 so that tokens' rows begin at other banks
     __shared__ __attribute__((aligned(16))) uint8_t parts[16 * T * kRow];
+    __shared__ __attribute__((aligned(16))) float turned[4][16][68];   // of each wavefront: 64 columns of 16 tokens, from columns to rows
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, q = lane >> 4;
-    const int m0 = blockIdx.y * (16 * T), c0 = (blockIdx.x * 4 + w) * 64, rank = p.rank;
+    Place place;
+    if (!find_place(p.tiles, p.pieces, place)) return;
+    const int m0 = place.tile * (16 * T), rank = p.rank, chunks = rank / 8;
+    // this wavefront's columns: 64 of every 256, `run` times
+    const int c_begin = place.piece * p.run * 256 + 64 * w, c_end = min((place.piece + 1) * p.run * 256, p.N);
     const int id = lane < 16 * T && m0 + lane < p.M ? p.ids[m0 + lane] : -1;
     const unsigned long long there = __ballot(lane < 16 * T && m0 + lane < p.M);
-    // matrix row r of column tile k is column 16 (r / 4) + 4 k + r % 4: a lane's results are the 16 columns from 16 q on
-    const int col = c0 + 16 * q;
-    auto finish = [&](int t, const v4f (&acc)[4]) {
-        const size_t at = (size_t)(m0 + 16 * t + n) * p.N + col;
-        if (col + 16 <= p.N) {
-            const any4 *from = reinterpret_cast<const any4 *>(p.base + at);
-            any4 *to = reinterpret_cast<any4 *>(p.out + at);
+    // base and out go by rows, eight tokens' 128 bytes at a time (as the matrix instructions' results lie, sixteen tokens' 64, a load
+    // or store takes twice the lines): lane l has eight columns of tokens l / 8 and 8 + l / 8 of a tile
+    const int row = lane >> 3, col = 8 * (lane & 7);
+    // (a tile has at most 64 rows of 2^24 columns; what is behind the last row is not there: a row's part of an offset is in the register
+    // that is compared with the buffer's size, whether or not the uniform part, a column of the first row, is added before)
+    const uint32_t tile_bytes = (uint32_t)min(16 * T, p.M - m0) * (uint32_t)p.N * 2u;
+    const __amdgpu_buffer_rsrc_t base_tile = buffer(p.base + (size_t)m0 * p.N, tile_bytes), out_tile = buffer(p.out + (size_t)m0 * p.N, tile_bytes);
+    const uint32_t at = ((uint32_t)row * (uint32_t)p.N + (uint32_t)col) * 2u, eight_rows = 16u * (uint32_t)p.N;
+    auto load_base = [&](int c0, int t, int h) {   // of a whole 64 columns
+        return __builtin_bit_cast(v4w, __builtin_amdgcn_raw_buffer_load_b128(base_tile, (int)(at + (2 * t + h) * eight_rows), 2 * c0, 0));
+    };
+    auto store = [&](int c0, int t, int h, v4w v) {
+        __builtin_amdgcn_raw_buffer_store_b128(v, out_tile, (int)(at + (2 * t + h) * eight_rows), 2 * c0, 0);
+    };
+    auto add = [](v4w base, v4f lo, v4f hi) {
+        auto two = [](uint32_t b, float x, float y) {
+            return pack_bf16x2(__builtin_bit_cast(float, b << 16) + x, __builtin_bit_cast(float, b & 0xffff0000u) + y);
+        };
+        return (v4w){two(base[0], lo[0], lo[1]), two(base[1], lo[2], lo[3]), two(base[2], hi[0], hi[1]), two(base[3], hi[2], hi[3])};
+    };
+    // The tokens of `tokens` in tile t: base plus lo, hi (of either half).
+    auto finish = [&](int c0, int t, unsigned long long tokens, const v4w (&base)[2], const v4f (&lo)[2], const v4f (&hi)[2]) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                any4 v = from[h];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const v4f s = acc[2 * h + i / 2];
-                    const float lo = __builtin_bit_cast(float, v[i] << 16), hi = __builtin_bit_cast(float, v[i] & 0xffff0000u);
-                    v[i] = i % 2 == 0 ? pack_bf16x2(lo + s[0], hi + s[1]) : pack_bf16x2(lo + s[2], hi + s[3]);
-                }
-                to[h] = v;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (col + i < p.N)
-                    p.out[at + i] = (uint16_t)pack_bf16x2(__builtin_bit_cast(float, (uint32_t)p.base[at + i] << 16) + acc[i / 4][i % 4], 0.f);
+        for (int h = 0; h < 2; h++) {
+            const v4w sum = add(base[h], lo[h], hi[h]);
+            if ((tokens >> (16 * t + 8 * h + row)) & 1) store(c0, t, h, sum);
         }
     };
-    if (blockIdx.z == 0) {   // tokens without an adapter
-        const unsigned long long none = there & ~__ballot((unsigned)id < (unsigned)p.adapters);
+    // The same behind the last whole 64 columns, as far as there are any.
+    auto finish_ragged = [&](int c0, int t, unsigned long long tokens, const v4f (&lo)[2], const v4f (&hi)[2]) {
+        for (int h = 0; h < 2; h++) {
+            const int token = 16 * t + 8 * h + row;
+            if (!((tokens >> token) & 1)) continue;
+            const size_t from = (size_t)(m0 + token) * p.N + c0 + col;
 #pragma unroll
-        for (int t = 0; t < T; t++)
-            if ((none >> (16 * t + n)) & 1) {
-                const v4f zero[4] = {};
-                finish(t, zero);
-            }
+            for (int i = 0; i < 8; i++)
+                if (c0 + col + i < p.N)
+                    p.out[from + i] = (uint16_t)pack_bf16x2(__builtin_bit_cast(float, (uint32_t)p.base[from + i] << 16) + (i < 4 ? lo[h][i % 4] : hi[h][i % 4]), 0.f);
+        }
+    };
+    const unsigned long long with = __ballot((unsigned)id < (unsigned)p.adapters);
+    if (place.turn == 0 && with != there) {   // tokens without an adapter
+        const v4f zero[2] = {};
+#pragma unroll 1
+        for (int c0 = c_begin; c0 < c_end; c0 += 256)
+#pragma unroll 1
+            for (int t = 0; t < T; t++)
+                if (c0 + 64 <= p.N) {
+                    const v4w base[2] = {load_base(c0, t, 0), load_base(c0, t, 1)};
+                    finish(c0, t, there & ~with, base, zero, zero);
+                } else {
+                    finish_ragged(c0, t, there & ~with, zero, zero);
+                }
     }
-    for_each_adapter(id, p.adapters, blockIdx.z, p.sharers, [&](int adapter, unsigned long long same) {
+    // eight values of a chunk of b: the ranks' chunks one behind the other (RT == 1: twice), 0 behind the last one
+    struct Weights {
+        v8bf v[S][4];
+    };
+    uint32_t b_at[S];
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        const bool some = RT == 1 ? q < 2 * chunks : 4 * s + q < chunks;
+        const int chunk = RT == 1 && q >= chunks ? q - chunks : 4 * s + q;
+        b_at[s] = some ? 2u * (uint32_t)(n * rank + 8 * chunk) : 0x40000000u;
+    }
+    // (the parts' places behind the last rank; what is multiplied there is 0 on both sides)
+    for (int i = tid; i < 16 * T * kRow / 16; i += 256) reinterpret_cast<v4i *>(parts)[i] = (v4i){0, 0, 0, 0};
+    for_each_adapter(id, p.adapters, place.turn, p.sharers, [&](int adapter, unsigned long long same) {
+        const uint16_t *b = p.b + (size_t)adapter * p.N * rank;
+        auto load_weights = [&](int c0, Weights &bv) {
+            const int cols = min(64, p.N - c0);
+            const __amdgpu_buffer_rsrc_t from = buffer(b + (size_t)c0 * rank, cols > 0 ? 2u * (uint32_t)(cols * rank) : 0u);
+#pragma unroll
+            for (int s = 0; s < S; s++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    bv.v[s][k] = __builtin_bit_cast(v8bf, __builtin_amdgcn_raw_buffer_load_b128(from, (int)(b_at[s] + 32u * (uint32_t)(k * rank)), 0, 0));
+        };
+        Weights bv;
+        load_weights(c_begin, bv);   // (in front of the parts' loads)
         const float scale = p.scale ? p.scale[adapter] : 1.f;
         __syncthreads();   // (the parts of the adapter before have been read)
-        for (int i = tid; i < 16 * T * rank; i += 256) {
-            const int t = i / rank, r = i - t * rank;
+        for (int i = tid; i < 16 * T * rank / 4; i += 256) {   // four ranks of a token
+            const int t = i / (rank / 4), r = 4 * (i - t * (rank / 4));
             if (!((same >> t) & 1)) continue;
             const float *from = p.part + (size_t)(m0 + t) * rank + r;
-            float v = 0.f;
-            for (int s = 0; s < p.splits; s++) v += from[(size_t)s * p.M * rank];
-            v *= scale;
-            const uint32_t high = __builtin_bit_cast(uint32_t, v) & 0xffff0000u;
-            const float low = fabsf(v) == __builtin_inff() ? 0.f : v - __builtin_bit_cast(float, high);
-            uint16_t *to = reinterpret_cast<uint16_t *>(parts + t * kRow) + r;
-            to[0] = (uint16_t)(high >> 16);
-            to[rank] = (uint16_t)pack_bf16x2(low, 0.f);
+            const size_t step = (size_t)p.M * rank;
+            v4f v = {0.f, 0.f, 0.f, 0.f};
+            constexpr int F = T == 1 ? 8 : 2;   // loads in flight
+            for (int s0 = 0; s0 < p.splits; s0 += F) {
+                v4f in[F];
+#pragma unroll
+                for (int s = 0; s < F; s++) in[s] = *reinterpret_cast<const v4f *>(from + (size_t)min(s0 + s, p.splits - 1) * step);
+#pragma unroll
+                for (int s = 0; s < F; s++)
+                    if (s0 + s < p.splits) v += in[s];
+            }
+            uint32_t high[4];
+            float low[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float f = v[j] * scale;
+                high[j] = __builtin_bit_cast(uint32_t, f) & 0xffff0000u;
+                low[j] = fabsf(f) == __builtin_inff() ? 0.f : f - __builtin_bit_cast(float, high[j]);
+            }
+            uint8_t *to = parts + t * kRow + 2 * r;
+            *reinterpret_cast<uint2 *>(to) = make_uint2(high[0] >> 16 | high[1], high[2] >> 16 | high[3]);
+            *reinterpret_cast<uint2 *>(to + (RT == 1 ? 2 * rank : kLow)) = make_uint2(pack_bf16x2(low[0], low[1]), pack_bf16x2(low[2], low[3]));
         }
         __syncthreads();
-        const uint16_t *b = p.b + (size_t)adapter * p.N * rank;
-        v4f acc[T][4] = {};
-        if (c0 < p.N) {
-            const int chunks = rank / 8;
+        // Tile t: matrix row r of column tile k is column 16 k + r; the results go through LDS into rows.
+        auto multiply = [&](int t, const Weights &bv, v4f (&lo)[2], v4f (&hi)[2]) {
+            v4f acc[4] = {};
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                const int chunk = 4 * s + q;   // eight values of the high parts, then of the low ones; nothing behind them
-                const bool some = chunk < 2 * chunks;
-                v8bf bv[4], vv[T];
+            for (int s = 0; s < S; s++) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int c = min(c0 + 16 * (n >> 2) + 4 * k + (n & 3), p.N - 1);
-                    bv[k] = some ? *reinterpret_cast<const v8bf *>(b + (size_t)c * rank + (chunk < chunks ? chunk : chunk - chunks) * 8) : (v8bf){};
+                for (int h = 0; h < PARTS; h++) {
+                    const v8bf v = *reinterpret_cast<const v8bf *>(parts + (16 * t + n) * kRow + h * kLow + 64 * s + 16 * q);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv.v[s][k], v, acc[k], 0, 0, 0);
                 }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) *reinterpret_cast<v4f *>(&turned[w][n][16 * k + 4 * q]) = acc[k];
+            lds_order();   // (of one wavefront: its LDS accesses complete in order)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                lo[h] = *reinterpret_cast<const v4f *>(&turned[w][8 * h + row][col]);
+                hi[h] = *reinterpret_cast<const v4f *>(&turned[w][8 * h + row][col + 4]);
+            }
+            lds_order();
+        };
+#pragma unroll 1
+        for (int c0 = c_begin; c0 < c_end; c0 += 256) {
+            if (c0 > c_begin) load_weights(c0, bv);
+            v4f lo[2], hi[2];
+            if (c0 + 64 <= p.N) {
+                v4w base[T][2];
 #pragma unroll
                 for (int t = 0; t < T; t++)
-                    vv[t] = some ? *reinterpret_cast<const v8bf *>(parts + (16 * t + n) * kRow + chunk * 16) : (v8bf){};
 #pragma unroll
-                for (int t = 0; t < T; t++)
+                    for (int h = 0; h < 2; h++) base[t][h] = load_base(c0, t, h);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) acc[t][k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[k], vv[t], acc[t][k], 0, 0, 0);
+                for (int t = 0; t < T; t++) {
+                    multiply(t, bv, lo, hi);
+                    finish(c0, t, same, base[t], lo, hi);
+                    __builtin_amdgcn_sched_barrier(0);   // (one tile's registers at a time)
+                }
+            } else {
+#pragma unroll 1
+                for (int t = 0; t < T; t++) {
+                    multiply(t, bv, lo, hi);
+                    finish_ragged(c0, t, same, lo, hi);
+                }
             }
         }
-#pragma unroll
-        for (int t = 0; t < T; t++)
-            if ((same >> (16 * t + n)) & 1) finish(t, acc[t]);
     });
 }
 
@@ -231,13 +355,13 @@ struct AdaptPlan {
     AdaptPlan(int M, int K, int rank, int adapters)
     {
         const int nkb = K / 128;
-        T = M <= 1024 || rank > 64 ? 1 : rank > 32 ? 2 : 4;
+        T = M <= 1024 ? 1 : rank > 64 ? 2 : 4;
         const int64_t tiles = ceil_div(M, 16 * T);
         const int most = adapters < 16 * T ? adapters : 16 * T;
-        sharers = (int)ceil_div(256, tiles);
+        sharers = tiles < 32 ? (int)ceil_div(128, tiles) : 4;
         sharers = sharers > most ? most : sharers;
         sharers = sharers > M ? M : sharers;
-        const int64_t want = ceil_div(512, tiles * sharers), can = ceil_div(nkb, 4);
+        const int64_t want = ceil_div(1024, tiles * sharers), can = ceil_div(nkb, 4);
         splits = (int)(want > can ? can : want);
     }
 };
@@ -250,19 +374,21 @@ hipError_t launch(void (*kernel)(Args...), dim3 grid, dim3 block, hipStream_t st
 }
 
 template <int RT, int T>
-hipError_t adapt(const AdaptParams &p, hipStream_t hs)
+hipError_t adapt(AdaptParams p, hipStream_t hs)
 {
-    const unsigned tiles = (unsigned)ceil_div(p.M, 16 * T);
+    p.tiles = (int)ceil_div(p.M, 16 * T);
+    p.pieces = (int)ceil_div(p.N, 256 * (int64_t)p.run);
+    auto grid = [&](int pieces) { return dim3((unsigned)(8 * ceil_div((int64_t)p.tiles * pieces, 8) * p.sharers)); };
     const auto in = p.x_scale ? adapt_in_kernel<RT, T, true> : adapt_in_kernel<RT, T, false>;
-    const hipError_t err = launch(in, dim3(tiles, p.splits, p.sharers), dim3(256), hs, p);
+    const hipError_t err = launch(in, grid(p.splits), dim3(256), hs, p);
     if (err != hipSuccess) return err;
-    return launch(adapt_out_kernel<RT, T>, dim3((unsigned)ceil_div(p.N, 256), tiles, p.sharers), dim3(256), hs, p);
+    return launch(adapt_out_kernel<RT, T>, grid(p.pieces), dim3(256), hs, p);
 }
 
 bool sizes_fit(int M, int N, int K, int rank, int adapters)
 {
     return M >= 0 && N > 0 && K > 0 && K % 128 == 0 && K <= 128 * kMaxKBlocks && rank > 0 && rank % 8 == 0 && rank <= kMaxRank &&
-           adapters > 0 && M <= 16 * 65535 && N <= INT32_MAX - 255;
+           adapters > 0 && M <= 16 * 65535 && N <= (1 << 24);
 }
 
 }  // namespace
@@ -297,11 +423,13 @@ extern "C" int alpha_moe_add_adapters(const uint16_t *base, const void *x, const
     p.ids = adapter_ids, p.out = out, p.part = static_cast<float *>(workspace);
     p.M = M, p.N = N, p.K = K, p.rank = rank, p.adapters = num_adapters, p.nkb = K / 128;
     p.splits = plan.splits, p.sharers = plan.sharers;
+    const int64_t pieces = ceil_div(N, 256) * ceil_div(M, 16 * plan.T) / 1536;   // 256 columns of a tile
+    p.run = pieces < 1 ? 1 : pieces > 4 ? 4 : (int)pieces;
     hipStream_t hs = static_cast<hipStream_t>(stream);
     const int T = plan.T;
     const hipError_t err = rank <= 16   ? (T == 1 ? adapt<1, 1>(p, hs) : adapt<1, 4>(p, hs))
                            : rank <= 32 ? (T == 1 ? adapt<2, 1>(p, hs) : adapt<2, 4>(p, hs))
-                           : rank <= 64 ? (T == 1 ? adapt<4, 1>(p, hs) : adapt<4, 2>(p, hs))
-                                        : adapt<8, 1>(p, hs);
+                           : rank <= 64 ? (T == 1 ? adapt<4, 1>(p, hs) : adapt<4, 4>(p, hs))
+                                        : (T == 1 ? adapt<8, 1>(p, hs) : adapt<8, 2>(p, hs));
     return err == hipSuccess ? ALPHA_MOE_OK : ALPHA_MOE_ERR_LAUNCH;
 }

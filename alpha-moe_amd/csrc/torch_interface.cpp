@@ -595,7 +595,8 @@ at::Tensor add_adapters(const at::Tensor &base, const at::Tensor &x, const c10::
     TORCH_CHECK(b.dim() == 3 && b.size(0) == L && b.size(1) == N && b.size(2) == rank, "b must be [L, N, rank]");
     TORCH_CHECK(adapter_ids.dim() == 1 && adapter_ids.size(0) == M, "adapter_ids must be [M]");
     TORCH_CHECK(M <= 1048560, "at most 1048560 rows");
-    TORCH_CHECK(N <= INT32_MAX && L <= INT32_MAX, "sizes exceed int32");
+    TORCH_CHECK(N <= 16777216, "at most 2^24 columns");
+    TORCH_CHECK(L <= INT32_MAX, "sizes exceed int32");
     if (x_scale.has_value()) {
         check_tensor(*x_scale, "x_scale", at::kFloat, dev);
         TORCH_CHECK(x_scale->dim() == 2 && x_scale->size(0) == M && x_scale->size(1) == K / 128, "x_scale must be [M, K/128]");
