@@ -378,6 +378,8 @@ hipError_t adapt(AdaptParams p, hipStream_t hs)
 {
     p.tiles = (int)ceil_div(p.M, 16 * T);
     p.pieces = (int)ceil_div(p.N, 256 * (int64_t)p.run);
+    if (8 * (ceil_div((int64_t)p.tiles * (p.pieces > p.splits ? p.pieces : p.splits), 8)) * p.sharers * 256 >= (int64_t(1) << 32))
+        return hipErrorInvalidConfiguration;   // (a launch has less than 2^32 threads)
     auto grid = [&](int pieces) { return dim3((unsigned)(8 * ceil_div((int64_t)p.tiles * pieces, 8) * p.sharers)); };
     const auto in = p.x_scale ? adapt_in_kernel<RT, T, true> : adapt_in_kernel<RT, T, false>;
     const hipError_t err = launch(in, grid(p.splits), dim3(256), hs, p);
@@ -431,5 +433,5 @@ extern "C" int alpha_moe_add_adapters(const uint16_t *base, const void *x, const
                            : rank <= 32 ? (T == 1 ? adapt<2, 1>(p, hs) : adapt<2, 4>(p, hs))
                            : rank <= 64 ? (T == 1 ? adapt<4, 1>(p, hs) : adapt<4, 4>(p, hs))
                                         : (T == 1 ? adapt<8, 1>(p, hs) : adapt<8, 2>(p, hs));
-    return err == hipSuccess ? ALPHA_MOE_OK : ALPHA_MOE_ERR_LAUNCH;
+    return err == hipSuccess ? ALPHA_MOE_OK : err == hipErrorInvalidConfiguration ? ALPHA_MOE_ERR_SHAPE : ALPHA_MOE_ERR_LAUNCH;
 }

@@ -139,8 +139,8 @@ __device__ __forceinline__ int wave_scan(int v)   // inclusive sums over the wav
 }
 
 // The tile of this workgroup, if there is one.  How many there are, only the device knows: each wavefront counts the experts' tiles,
-// a run of experts to a lane, and looks for its own.  An expert's tiles follow each other, its tiles of tokens in groups of HIGH next to each
-// other; each XCD gets a run of tiles.  Offsets are taken into [0, M], and where they do not ascend then, nobody has a tile.
+// a run of experts to a lane, and looks for its own.  An expert's tiles follow each other, its tiles of tokens in groups of HIGH (0: all of
+// them) next to each other; each XCD gets a run of tiles.  Offsets are taken into [0, M], and where they do not ascend then, nobody has a tile.
 template <int TOKENS, int HIGH>
 __device__ __forceinline__ bool find_tile(const MmParams &p, GroupTile &g)
 {
@@ -176,8 +176,9 @@ __device__ __forceinline__ bool find_tile(const MmParams &p, GroupTile &g)
     g.lo = __builtin_amdgcn_readlane(from, owner);
     g.rows = __builtin_amdgcn_readlane(rows, owner);
     const int token_tiles = tiles_of_rows(g.rows), inside = tile - __builtin_amdgcn_readlane(before, owner) * p.row_groups;
-    const int per_group = HIGH * p.row_groups, group = inside / per_group, in_group = inside - group * per_group;
-    const int high = min(token_tiles - group * HIGH, HIGH);
+    // (a launch has fewer than 2^24 tiles, so HIGH, which is 8, times the groups of columns is an int)
+    const int per_group = HIGH * p.row_groups, group = HIGH > 0 ? inside / per_group : 0, in_group = inside - group * per_group;
+    const int high = HIGH > 0 ? min(token_tiles - group * HIGH, HIGH) : token_tiles;
     g.row_group = in_group / high;
     g.token_tile = group * HIGH + in_group - g.row_group * high;
     return true;
@@ -254,7 +255,7 @@ __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(MmParams p)
     // workgroups are dealt to the eight XCDs in turn: each gets a run of tiles, token groups of one row group next to each other
     int c0, m0;
     if constexpr (GROUPED) {
-        if (!enter_group<R * 16, HALF ? 8 : T * 16, 1 << 24, WAVES * 64>(p, c0, m0)) return;
+        if (!enter_group<R * 16, HALF ? 8 : T * 16, 0, WAVES * 64>(p, c0, m0)) return;
     } else {
         const int tiles = p.row_groups * p.token_groups, run = (tiles + 7) >> 3;
         const int tile = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);

@@ -68,6 +68,15 @@ def test_experts_that_have_more_or_fewer_rows_than_the_average(spread):
     check(*args, run(*args))
 
 
+@pytest.mark.parametrize("counts", [[1, 2, 0, 1], [9, 10, 3], [20, 30, 1], [60, 3], [150, 20], [300, 0]])
+@pytest.mark.parametrize("N", [2050, 4096, 9000])
+def test_many_columns(counts, N):
+    """more groups of columns than a few, in every kind of tile"""
+    print(f"case many columns {counts} N={N}", flush=True)
+    args = problem(counts, 1, N, 128, N)
+    check(*args, run(*args))
+
+
 def test_one_expert_is_the_ungrouped_product():
     for M, N, K in ((5, 300, 256), (70, 130, 384), (600, 512, 256)):
         x, xs, offsets, w, ws = problem([M], 0, N, K, M)

@@ -135,6 +135,7 @@ def test_adapter_refusals_and_shapes():
         return A.alpha_moe_add_adapters(base, x, xs, a, b, ids, scale, out, M, N, K, rank, L, ws, nws, None)
     assert call(M=0) == OK and call(M=-1) == SHAPE and call(N=0) == SHAPE and call(K=0) == SHAPE and call(K=64) == SHAPE
     assert call(K=65536 + 128) == SHAPE and call(L=0) == SHAPE and call(M=1048561) == SHAPE and call(N=2 ** 31 - 1) == SHAPE
+    assert call(N=2 ** 24 + 1) == SHAPE and call(M=1048560, N=2 ** 24) == SHAPE       # (more threads than a launch has)
     for rank in (0, -8, 4, 12, 136):
         assert call(rank=rank) == SHAPE, rank
     for name in ("base", "x", "a", "b", "ids", "out"):
