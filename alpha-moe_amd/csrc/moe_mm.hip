@@ -104,6 +104,7 @@ struct TokenScales {
 // value by value 8192 x 4095 x 1024 takes 124 us, so 62; 4094 columns 128 and 48, 4096 43.)
 typedef uint32_t any2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t v4w __attribute__((ext_vector_type(4)));
 
 // Columns n .. n + 3 of row m; what is behind the last row or column is not there.
 __device__ __forceinline__ void store4(const MmParams &p, int m, int n, v4f v)
@@ -139,43 +140,68 @@ __device__ __forceinline__ int wave_scan(int v)   // inclusive sums over the wav
 }
 
 // The tile of this workgroup, if there is one.  How many there are, only the device knows: each wavefront counts the experts' tiles,
-// a run of experts to a lane, and looks for its own.  An expert's tiles follow each other, its tiles of tokens in groups of HIGH (0: all of
-// them) next to each other; each XCD gets a run of tiles.  Offsets are taken into [0, M], and where they do not ascend then, nobody has a tile.
+// 256 experts' offsets in flight at a time, and looks for its own.  (A run of experts to a lane, one offset
+// behind the other, took some 0.3 us more of every workgroup.)  An expert's tiles follow each other, its tiles of tokens in groups
+// of HIGH (0: all of them) next to each other; each XCD gets a run of tiles.  Offsets are taken into [0, M], and where they do not ascend
+// then, nobody has a tile.
 template <int TOKENS, int HIGH>
 __device__ __forceinline__ bool find_tile(const MmParams &p, GroupTile &g)
 {
-    const int lane = threadIdx.x & 63, groups = p.E + 1;
-    const int per = (groups + 63) >> 6, first = lane * per;
-    auto bound = [&](int e) { return e == 0 ? 0 : e > p.E ? p.M : min(max(p.offsets[e], 0), p.M); };
+    constexpr int Q = 4;
+    const int lane = threadIdx.x & 63;
+    auto clamped = [&](int row) { return min(max(row, 0), p.M); };
     auto tiles_of_rows = [](int rows) { return rows > 0 ? (rows + TOKENS - 1) / TOKENS : 0; };
-    int sum = 0, from = first < groups ? bound(first) : 0;
+    int from[Q], to[Q];
+    auto load = [&](int base) {
+#pragma unroll
+        for (int j = 0; j < Q; j++) {
+            const int e = base + 64 * j + lane;
+            from[j] = e < p.E && e > 0 ? p.offsets[e] : 0;
+            to[j] = e < p.E ? p.offsets[e + 1] : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < Q; j++) from[j] = clamped(from[j]), to[j] = clamped(to[j]);
+    };
+    const int last = clamped(p.offsets[p.E]);
+    int sum = 0;
     bool ascend = true;
-    for (int e = first; e < min(first + per, groups); e++) {
-        const int to = bound(e + 1);
-        ascend &= to >= from;
-        sum += tiles_of_rows(to - from);
-        from = to;
+    for (int base = 0; base < p.E; base += 64 * Q) {
+        load(base);
+#pragma unroll
+        for (int j = 0; j < Q; j++) {
+            ascend &= to[j] >= from[j];
+            sum += tiles_of_rows(to[j] - from[j]);
+        }
     }
     if (!__all(ascend)) return false;
-    const int incl = wave_scan(sum);
-    const int total = __builtin_amdgcn_readlane(incl, 63) * p.row_groups, run = (total + 7) >> 3;
+    const int of_experts = __builtin_amdgcn_readlane(wave_scan(sum), 63), tail = tiles_of_rows(p.M - last);
+    const int total = (of_experts + tail) * p.row_groups, run = (total + 7) >> 3;
     const int in_run = (int)(blockIdx.x >> 3), tile = (int)(blockIdx.x & 7) * run + in_run;
     if (in_run >= run || tile >= total) return false;
     const int at = tile / p.row_groups;   // among the tiles of tokens
-    const int owner = (int)__builtin_ctzll(__ballot(incl > at));
-    int before = incl - sum, e = first, rows = 0;
-    from = first < groups ? bound(first) : 0;
-    for (; e < min(first + per, groups); e++) {
-        const int to = bound(e + 1);
-        rows = to - from;
-        if (before + tiles_of_rows(rows) > at) break;
-        before += tiles_of_rows(rows);
-        from = to;
+    int before = of_experts;
+    g.expert = p.E, g.lo = last, g.rows = p.M - last;
+    if (at < of_experts) {
+        before = 0;
+        bool found = false;
+        for (int base = 0; !found; base += 64 * Q) {
+            if (p.E > 64 * Q) load(base);   // (otherwise they are all there)
+#pragma unroll
+            for (int j = 0; j < Q; j++) {
+                const int tiles = tiles_of_rows(to[j] - from[j]), incl = wave_scan(tiles), all = __builtin_amdgcn_readlane(incl, 63);
+                if (!found && at < before + all) {
+                    const int owner = (int)__builtin_ctzll(__ballot(before + incl > at));
+                    g.expert = base + 64 * j + owner;
+                    g.lo = __builtin_amdgcn_readlane(from[j], owner);
+                    g.rows = __builtin_amdgcn_readlane(to[j] - from[j], owner);
+                    before += __builtin_amdgcn_readlane(incl - tiles, owner);
+                    found = true;
+                }
+                if (!found) before += all;
+            }
+        }
     }
-    g.expert = __builtin_amdgcn_readlane(e, owner);
-    g.lo = __builtin_amdgcn_readlane(from, owner);
-    g.rows = __builtin_amdgcn_readlane(rows, owner);
-    const int token_tiles = tiles_of_rows(g.rows), inside = tile - __builtin_amdgcn_readlane(before, owner) * p.row_groups;
+    const int token_tiles = tiles_of_rows(g.rows), inside = tile - before * p.row_groups;
     // (a launch has fewer than 2^24 tiles, so HIGH, which is 8, times the groups of columns is an int)
     const int per_group = HIGH * p.row_groups, group = HIGH > 0 ? inside / per_group : 0, in_group = inside - group * per_group;
     const int high = HIGH > 0 ? min(token_tiles - group * HIGH, HIGH) : token_tiles;
@@ -315,7 +341,7 @@ __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(MmParams p)
             if (!RUN && lane < T * 16) dma4(xsbuf, xs_off, 4u * (unsigned)kb, at + (R + T) * 2048);
             if (RUN && scales.loads(kb, i == 0)) scales.load(xsbuf, xs_off, kb, 0, lane < T * 16, xs);
         } else if constexpr (j < 2 * R) {
-            dma16<HALF ? 2 : 0>(wbuf, w_off[j / 2][j % 2], 128u * kb, at + j * 1024);
+            dma16<HALF || (GROUPED && T == 1) ? 2 : 0>(wbuf, w_off[j / 2][j % 2], 128u * kb, at + j * 1024);
         } else {
             constexpr int t = HALF ? tj : tj / 2, h = HALF ? 0 : tj % 2;
             dma16<0>(xbuf, x_off[t][h], 128u * kb, at + (R + t) * 2048 + h * 1024);
@@ -466,31 +492,16 @@ struct Tile {
     static_assert(kCols >= 128 ? (TN * 16) <= 128 : 128 % kCols == 0, "a wavefront's columns share their scales");
 };
 
+// The tile of columns from c0 and tokens from m0 on.
 template <int TN, int TM, int WN, int WM, int S, int LOADERS, bool GROUPED>
-__global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(MmParams p)
+__device__ __forceinline__ void mm_tile(const MmParams &p, int c0, int m0, uint8_t *lds)
 {
     typedef Tile<TN, TM, WN, WM, S, LOADERS> T;
-    __shared__ __attribute__((aligned(128))) uint8_t lds[T::kBytes];
     const int tid = threadIdx.x, lane = tid & 63, w = rfl(tid >> 6);
     const int wn = w % WN, wm = w / WN;
     const int lw = LOADERS > 0 ? w - T::kWaves : w;   // which of the loading wavefronts it is
     const bool loads = LOADERS == 0 || lw >= 0;
     const int n = lane & 15, q = lane >> 4;
-
-    // each XCD gets a run of tiles, in groups of eight tiles of tokens, so that those at work at a time share rows and columns
-    constexpr int kGroup = 8;
-    int c0, m0;
-    if constexpr (GROUPED) {
-        if (!enter_group<T::kCols, T::kTokens, kGroup, (T::kWaves + LOADERS) * 64>(p, c0, m0)) return;
-    } else {
-        const int tiles = p.row_groups * p.token_groups, run = (tiles + 7) >> 3;
-        const int tile = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
-        if (tile >= tiles) return;
-        const int per_group = kGroup * p.row_groups, group = tile / per_group, in_group = tile - group * per_group;
-        const int high = p.token_groups - group * kGroup < kGroup ? p.token_groups - group * kGroup : kGroup;
-        const int rg = in_group / high, tg = group * kGroup + in_group - rg * high;
-        c0 = rg * T::kCols, m0 = tg * T::kTokens;
-    }
     const int K = p.K, nkb = p.nkb;
 
     // Matrix row r of a wavefront's weight tile k is its column 4 TN (r / 4) + 4 k + r % 4, so a lane's results of all tiles are 4 TN
@@ -550,6 +561,7 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(Mm
                 stage = stage + 1 < S ? stage + 1 : 0;
             }
             wait_vmcnt<0>();   // (the workgroup's memory is given back)
+            if constexpr (GROUPED) lds_barrier();
             return;
         }
     } else {
@@ -634,6 +646,35 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(Mm
     static_assert(TN * TM % 2 == 0, "");
     acc[TN - 2][TM - 1] += prod[0] * fac[0];
     acc[TN - 1][TM - 1] += prod[1] * fac[1];
+    if constexpr (GROUPED) {
+        // Through LDS into whole lines: as the results lie, a store of all lanes is sixteen tokens' 64 bytes.
+        lds_barrier();   // (the last stage has been read, and nothing is on its way into LDS)
+        const int first = c0 + wn * 64;
+        if (first + 64 <= p.N) {
+            static_assert(TN == 4, "");
+            uint8_t *mine = lds + w * 16 * 144;
+            const int row = lane >> 3, chunk = lane & 7;
+#pragma unroll
+            for (int t = 0; t < TM; t++) {
+#pragma unroll
+                for (int k = 0; k < TN; k += 2)
+                    *reinterpret_cast<v4w *>(mine + n * 144 + q * 32 + k * 8) =
+                        (v4w){pack_bf16x2(acc[k][t][0], acc[k][t][1]), pack_bf16x2(acc[k][t][2], acc[k][t][3]),
+                              pack_bf16x2(acc[k + 1][t][0], acc[k + 1][t][1]), pack_bf16x2(acc[k + 1][t][2], acc[k + 1][t][3])};
+                __builtin_amdgcn_wave_barrier();
+                asm volatile("" ::: "memory");   // (of one wavefront: its LDS accesses complete in order)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int m = m0 + (wm * TM + t) * 16 + 8 * h + row;
+                    const any4 v = *reinterpret_cast<const v4w *>(mine + (8 * h + row) * 144 + chunk * 16);
+                    if (m < p.M) *reinterpret_cast<any4 *>(p.out + (size_t)m * p.N + first + 8 * chunk) = v;
+                }
+                __builtin_amdgcn_wave_barrier();
+                asm volatile("" ::: "memory");
+            }
+            return;
+        }
+    }
     const int col = c0 + wn * TN * 16 + 4 * TN * q;
 #pragma unroll
     for (int t = 0; t < TM; t++) {
@@ -652,6 +693,40 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(Mm
             for (int k = 0; k < TN; k++) store4(p, m, col + 4 * k, acc[k][t]);
         }
     }
+}
+
+template <int TN, int TM, int WN, int WM, int S, int LOADERS, bool GROUPED>
+__global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(MmParams p)
+{
+    typedef Tile<TN, TM, WN, WM, S, LOADERS> T;
+    __shared__ __attribute__((aligned(128))) uint8_t lds[T::kBytes];
+    // each XCD gets a run of tiles, in groups of eight tiles of tokens, so that those at work at a time share rows and columns
+    constexpr int kGroup = 8;
+    int c0, m0;
+    if constexpr (GROUPED) {
+        if (!enter_group<T::kCols, T::kTokens, kGroup, (T::kWaves + LOADERS) * 64>(p, c0, m0)) return;
+    } else {
+        const int tiles = p.row_groups * p.token_groups, run = (tiles + 7) >> 3;
+        const int tile = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
+        if (tile >= tiles) return;
+        const int per_group = kGroup * p.row_groups, group = tile / per_group, in_group = tile - group * per_group;
+        const int high = p.token_groups - group * kGroup < kGroup ? p.token_groups - group * kGroup : kGroup;
+        const int rg = in_group / high, tg = group * kGroup + in_group - rg * high;
+        c0 = rg * T::kCols, m0 = tg * T::kTokens;
+    }
+    mm_tile<TN, TM, WN, WM, S, LOADERS, GROUPED>(p, c0, m0, lds);
+}
+
+// Tiles of 256 x 256 of which an expert's last one, if it has at most 128 rows, is multiplied as one of 256 x 128.
+__global__ __launch_bounds__(512, 2) void mm_ragged_tile_kernel(MmParams p)
+{
+    typedef Tile<4, 8, 4, 2, 2, 0> Whole;
+    typedef Tile<4, 4, 4, 2, 3, 0> Half;
+    __shared__ __attribute__((aligned(128))) uint8_t lds[Whole::kBytes > Half::kBytes ? Whole::kBytes : Half::kBytes];
+    int c0, m0;
+    if (!enter_group<Whole::kCols, Whole::kTokens, 8, 512>(p, c0, m0)) return;
+    if (p.M - m0 > Half::kTokens) mm_tile<4, 8, 4, 2, 2, 0, true>(p, c0, m0, lds);
+    else mm_tile<4, 4, 4, 2, 3, 0, true>(p, c0, m0, lds);
 }
 
 template <int TN, int TM, int WN, int WM, int S, int LOADERS, bool GROUPED = false>
@@ -697,29 +772,47 @@ Plan plan(int M, int N)
     return best;
 }
 
-// Of a grouped call: by the rows that an expert has on average.
-Plan grouped_plan(int M, int N, int E)
+// Of a grouped call, by the rows that an expert has on average; how they are spread, only the device knows.  MI355X, us, experts drawn as
+// a router's are (the largest has four times the average), 32x16 / 128x64 / 256x128 / 256x256 tile: 256 experts, N = 512, K = 7168: 2 rows
+// on average 102 / 131 / 146 / 207, 8 rows 157 / 167 / 170 / 226, 32 rows 285 / 201 / 204 / 259, 64 rows 416 / 227 / 220 / 312, 256 rows
+// 1300 / 492 / 414 / 443; 128 experts, N = 1536, K = 2048: 16 rows 105 / 74 / 82 / 105, 128 rows 420 / 142 / 124 / 134, 512 rows 1457 / 402 /
+// 306 / 278.  With few K blocks (N = 7168, K = 256) most wavefronts of the streaming kernel have nothing to do, and what a tile takes beside
+// its K blocks counts: 2 rows 199 / 126 / - / -, 256 rows - / 787 / 610 / 459.  Fewer tiles than units: the smallest (8 rows of 8 experts,
+// N = 512, K = 7168, 16x16 9.2, 32x16 10.2).
+Plan grouped_plan(int M, int N, int K, int E)
 {
-    const int mean = M / E;
-    return mean <= 4 ? kStreamHalf2 : mean <= 12 ? kStream2x1 : mean <= 24 ? kStream2x2 : mean <= 48 ? kTile128x64 : mean <= 128 ? kTile128x128 : kTile256x256;
+    const int mean = M / E, nkb = K / 128;
+    if (tiles_of(M, N, 32, 1) <= kUnits / 2) return kStreamHalf1;
+    if (mean <= 8 && nkb >= 12) return kStream2x1;
+    return mean >= 12 * nkb ? kTile256x256 : mean <= 40 ? kTile128x64 : kTile256x128;
 }
 
 template <bool G>
 int launch_plan(Plan plan, const MmParams &p, hipStream_t hs)
 {
     hipError_t err = hipErrorInvalidValue;
-    switch (plan) {
-    case kStreamHalf1: err = launch_stream_mm<1, 1, 8, 2, true, G>(p, hs); break;
-    case kStreamHalf2: err = launch_stream_mm<2, 1, 8, 2, true, G>(p, hs); break;
-    case kStream1x1: err = launch_stream_mm<1, 1, 8, 2, false, G>(p, hs); break;
-    case kStream2x1: err = launch_stream_mm<2, 1, 4, 2, false, G>(p, hs); break;
-    case kStream2x2: err = launch_stream_mm<2, 2, 4, 2, false, G>(p, hs); break;
-    case kStream4x2: err = launch_stream_mm<4, 2, 4, 2, false, G>(p, hs); break;
-    case kStream4x4: err = launch_stream_mm<4, 4, 4, 1, false, G>(p, hs); break;
-    case kTile128x64: err = launch_tile_mm<4, 2, 2, 2, 3, 4, G>(p, hs); break;
-    case kTile128x128: err = launch_tile_mm<4, 4, 2, 2, 4, 4, G>(p, hs); break;
-    case kTile256x128: err = launch_tile_mm<4, 4, 4, 2, 3, 4, G>(p, hs); break;
-    case kTile256x256: err = launch_tile_mm<4, 8, 4, 2, 2, 0, G>(p, hs); break;
+    if constexpr (G) {   // (grouped_plan() names no others)
+        switch (plan) {
+        case kStreamHalf1: err = launch_stream_mm<1, 1, 8, 2, true, true>(p, hs); break;
+        case kStream2x1: err = launch_stream_mm<2, 1, 4, 2, false, true>(p, hs); break;
+        case kTile128x64: err = launch_tile_mm<4, 2, 2, 2, 3, 4, true>(p, hs); break;
+        case kTile256x128: err = launch_tile_mm<4, 4, 4, 2, 3, 4, true>(p, hs); break;
+        default: err = launch_tiles(mm_ragged_tile_kernel, p, 256, 256, 512, true, hs); break;
+        }
+    } else {
+        switch (plan) {
+        case kStreamHalf1: err = launch_stream_mm<1, 1, 8, 2, true>(p, hs); break;
+        case kStreamHalf2: err = launch_stream_mm<2, 1, 8, 2, true>(p, hs); break;
+        case kStream1x1: err = launch_stream_mm<1, 1, 8, 2, false>(p, hs); break;
+        case kStream2x1: err = launch_stream_mm<2, 1, 4, 2, false>(p, hs); break;
+        case kStream2x2: err = launch_stream_mm<2, 2, 4, 2, false>(p, hs); break;
+        case kStream4x2: err = launch_stream_mm<4, 2, 4, 2, false>(p, hs); break;
+        case kStream4x4: err = launch_stream_mm<4, 4, 4, 1, false>(p, hs); break;
+        case kTile128x64: err = launch_tile_mm<4, 2, 2, 2, 3, 4>(p, hs); break;
+        case kTile128x128: err = launch_tile_mm<4, 4, 2, 2, 4, 4>(p, hs); break;
+        case kTile256x128: err = launch_tile_mm<4, 4, 4, 2, 3, 4>(p, hs); break;
+        case kTile256x256: err = launch_tile_mm<4, 8, 4, 2, 2, 0>(p, hs); break;
+        }
     }
     return err == hipSuccess ? ALPHA_MOE_OK : err == hipErrorInvalidConfiguration ? ALPHA_MOE_ERR_SHAPE : ALPHA_MOE_ERR_LAUNCH;
 }
@@ -760,5 +853,5 @@ extern "C" int alpha_moe_grouped_block_scaled_mm(const uint8_t *x, const float *
     p.M = M, p.N = N, p.K = K, p.nkb = K / 128;
     p.quads = p.nkb >= 4;
     p.offsets = offsets, p.E = num_experts;
-    return launch_plan<true>(grouped_plan(M, N, num_experts), p, static_cast<hipStream_t>(stream));
+    return launch_plan<true>(grouped_plan(M, N, K, num_experts), p, static_cast<hipStream_t>(stream));
 }
