@@ -355,13 +355,14 @@ struct AdaptPlan {
     AdaptPlan(int M, int K, int rank, int adapters)
     {
         const int nkb = K / 128;
-        T = M <= 1024 ? 1 : rank > 64 ? 2 : 4;
+        T = M <= 2048 ? 1 : rank > 64 ? 2 : 4;
         const int64_t tiles = ceil_div(M, 16 * T);
         const int most = adapters < 16 * T ? adapters : 16 * T;
-        sharers = tiles < 32 ? (int)ceil_div(128, tiles) : 4;
+        sharers = tiles < 32 ? (int)ceil_div(128, tiles) : T == 1 && tiles >= 96 ? 2 : 4;
         sharers = sharers > most ? most : sharers;
         sharers = sharers > M ? M : sharers;
-        const int64_t want = ceil_div(1024, tiles * sharers), can = ceil_div(nkb, 4);
+        const int64_t groups = tiles * sharers, can = ceil_div(nkb, 4);
+        const int64_t want = T > 1 ? ceil_div(1024, groups) : groups < 128 ? ceil_div(1024, groups) : 8;
         splits = (int)(want > can ? can : want);
     }
 };
