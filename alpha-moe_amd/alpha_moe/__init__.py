@@ -84,7 +84,7 @@ c_abi.alpha_moe_route_topk.restype = ctypes.c_int
 c_abi.alpha_moe_route_topk.argtypes = (
     [ctypes.c_void_p, ctypes.c_int] + [ctypes.c_void_p] * 3 + [ctypes.c_int] * 8 + [ctypes.c_float, ctypes.c_void_p])
 c_abi.alpha_moe_sort_workspace_bytes.restype = ctypes.c_size_t
-c_abi.alpha_moe_sort_workspace_bytes.argtypes = [ctypes.c_int] * 2
+c_abi.alpha_moe_sort_workspace_bytes.argtypes = [ctypes.c_int] * 3
 c_abi.alpha_moe_sort_tokens.restype = ctypes.c_int
 c_abi.alpha_moe_sort_tokens.argtypes = (
     [ctypes.c_void_p, ctypes.c_int] + [ctypes.c_void_p] * 6 + [ctypes.c_int] * 4 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p])

@@ -40,12 +40,14 @@ __device__ __forceinline__ v4w load_piece(const uint8_t *row, int v, int64_t byt
         if (at + 2 * i < bytes) r[i / 2] |= (uint32_t) * reinterpret_cast<const uint16_t *>(row + at + 2 * i) << (16 * (i & 1));
     return r;
 }
+// Non-temporal: rows are written once, and most of them are many (8192 tokens of 7168 codes to 8 rows each 127 us without, 103 with it;
+// sums of 4096 x 8 rows of 2048 bf16 33 and 29).
 template <int A>
 __device__ __forceinline__ void store_piece(uint8_t *row, int v, int64_t bytes, v4w r)
 {
     const int64_t at = (int64_t)v * 16;
     if (A == 16 || at + 16 <= bytes) {
-        *reinterpret_cast<typename Piece<A>::type *>(row + at) = r;
+        __builtin_nontemporal_store((typename Piece<A>::type)r, reinterpret_cast<typename Piece<A>::type *>(row + at));
         return;
     }
 #pragma unroll
@@ -65,16 +67,19 @@ struct SortParams {
     int scale_cols, M, top_k, E, numel, pieces;
 };
 
-// The U pieces v0, v0 + step, ... of token t's row to its slots' rows, and (columns c0, c0 + c_step, ...) its scales.  at(s): the slot's
-// entry in the map.
-template <int A, int U, typename At>
-__device__ __forceinline__ void spread(const SortParams &p, int t, int v0, int step, int c0, int c_step, At at)
+// The U pieces v0, v0 + step, ... of token t's row.
+template <int A, int U>
+__device__ __forceinline__ void gather(const SortParams &p, int t, int v0, int step, v4w (&piece)[U])
 {
     const uint8_t *from = p.x + (int64_t)t * p.row_bytes;
-    v4w piece[U];
 #pragma unroll
     for (int u = 0; u < U; u++)
         if (v0 + u * step < p.pieces) piece[u] = load_piece<A>(from, v0 + u * step, p.row_bytes);
+}
+// They go to the rows of its slots, and so do (columns c0, c0 + c_step, ...) its scales.  at(s): the slot's entry in the map.
+template <int A, int U, typename At>
+__device__ __forceinline__ void spread(const SortParams &p, int t, int v0, int step, const v4w (&piece)[U], int c0, int c_step, At at)
+{
     for (int s = 0; s < p.top_k; s++) {
         const int m = at(s);
         const int64_t row = m < 0 ? ~m : m;
@@ -98,8 +103,7 @@ __device__ __forceinline__ int bucket(int id, int E) { return (unsigned)id < (un
 
 // Few slots, in one launch: a workgroup to a token (and 16 KiB of its row) finds its slots' rows by itself - a slot's row is the number of slots
 // in front of it, by (expert, slot) - and one more workgroup counts the experts.
-constexpr int kSortFew = 8192;
-constexpr int kSortMaxExperts = 4096;
+constexpr int kSortMaxExperts = 4096, kMaxTopK = 64;
 template <int A>
 __global__ __launch_bounds__(256) void sort_few_kernel(const SortParams p)
 {
@@ -126,7 +130,9 @@ __global__ __launch_bounds__(256) void sort_few_kernel(const SortParams p)
         }
         return;
     }
-    const int t = blockIdx.x;
+    const int t = blockIdx.x, part = blockIdx.y;
+    v4w piece[4];
+    gather<A, 4>(p, t, part * 1024 + tid, 256, piece);
     constexpr int G = 8;   // slots looked at together
     for (int s0 = 0; s0 < p.top_k; s0 += G) {
         int key[G], count[G];
@@ -136,6 +142,7 @@ __global__ __launch_bounds__(256) void sort_few_kernel(const SortParams p)
             key[g] = __builtin_amdgcn_readfirstlane(bucket(p.ids[i], p.E) * p.numel + i);
             count[g] = 0;
         }
+#pragma unroll 4
         for (int j0 = wave * 64; j0 < p.numel; j0 += 256) {
             const int j = j0 + lane;
             const int other = j < p.numel ? bucket(p.ids[j], p.E) * p.numel + j : INT32_MAX;
@@ -148,14 +155,15 @@ __global__ __launch_bounds__(256) void sort_few_kernel(const SortParams p)
                 if (s0 + g < p.top_k) lds[(s0 + g) * 4 + wave] = count[g];
     }
     __syncthreads();
-    auto at = [&](int s) {
-        const int row = lds[s * 4] + lds[s * 4 + 1] + lds[s * 4 + 2] + lds[s * 4 + 3];
-        return (unsigned)p.ids[t * p.top_k + s] < (unsigned)p.E ? row : ~row;
-    };
-    if (blockIdx.y == 0)
-        for (int s = tid; s < p.top_k; s += 256) p.row_of_slot[t * p.top_k + s] = at(s);
-    const int part = blockIdx.y;
-    spread<A, 4>(p, t, part * 1024 + tid, 256, part == 0 ? tid : p.scale_cols, 256, at);
+    int *entry = lds + 4 * kMaxTopK;
+    if (tid < p.top_k) {
+        const int row = lds[tid * 4] + lds[tid * 4 + 1] + lds[tid * 4 + 2] + lds[tid * 4 + 3], i = t * p.top_k + tid;
+        entry[tid] = (unsigned)p.ids[i] < (unsigned)p.E ? row : ~row;
+        if (part == 0) p.row_of_slot[i] = entry[tid];
+    }
+    __syncthreads();
+    auto at = [&](int s) { return entry[s]; };
+    spread<A, 4>(p, t, part * 1024 + tid, 256, piece, part == 0 ? tid : p.scale_cols, 256, at);
 }
 
 // Many slots: histograms of segments, places, copies.
@@ -225,15 +233,16 @@ __global__ __launch_bounds__(1024) void sort_place_kernel(const SortParams p, in
         for (int e = threadIdx.x; e < buckets; e += blockDim.x) p.offsets[e] = start[e];
 }
 
-template <int A, int U>
+template <int A, int U, bool ONE>
 __global__ __launch_bounds__(256) void spread_kernel(const SortParams p)
 {
-    const int t = blockIdx.x * blockDim.y + threadIdx.y;
+    const int t = ONE ? (int)blockIdx.x : (int)(blockIdx.x * blockDim.y + threadIdx.y);
     if (t >= p.M) return;
     const int32_t *map = p.row_of_slot + (int64_t)t * p.top_k;
-    const int part = blockIdx.y, step = blockDim.x;
-    spread<A, U>(p, t, part * U * step + (int)threadIdx.x, step, part == 0 ? (int)threadIdx.x : p.scale_cols, step,
-                 [&](int s) { return map[s]; });
+    const int part = blockIdx.y, step = blockDim.x, first = part * U * step + (int)threadIdx.x;
+    v4w piece[U];
+    gather<A, U>(p, t, first, step, piece);
+    spread<A, U>(p, t, first, step, piece, part == 0 ? (int)threadIdx.x : p.scale_cols, step, [&](int s) { return map[s]; });
 }
 
 // ---- combine -----------------------------------------------------------------------------------------------
@@ -278,11 +287,11 @@ struct Values<float> {
 
 // A thread to 16 bytes of a token's sum, up to eight rows in flight.
 constexpr int kCombineInFlight = 8;
-template <typename T, int A>
+template <typename T, int A, bool ONE>
 __global__ __launch_bounds__(256) void combine_kernel(const CombineParams p)
 {
     constexpr int N = Values<T>::N;
-    const int64_t t = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    const int64_t t = ONE ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     const int v = blockIdx.y * blockDim.x + threadIdx.x;
     if (t >= p.M || v >= p.pieces) return;
     const int32_t *map = p.map + t * p.top_k;
@@ -392,7 +401,6 @@ __global__ __launch_bounds__(256) void combine_grad_kernel(const CombineParams p
 // ---- launches ----------------------------------------------------------------------------------------------
 constexpr int kSortSeg = 1024, kSortMaxSeg = 512;
 constexpr size_t kDefaultLds = 64 << 10;   // dynamic LDS a kernel may have without a word
-constexpr int kMaxTopK = 64;
 
 struct Segments {
     int seg, n, words;
@@ -421,10 +429,19 @@ int threads_along(int pieces, int U)
     return n;
 }
 
+// Whether the workgroups find their slots' rows by themselves: every wavefront looks at a quarter of the slots for each eight of its token's.
+// MI355X, us, so / in three launches: 2048 rows of 2048 bf16 6.5 / 10.7, 5120 10.4 / 11.4, 6144 12.1 / 12.3, 7200 14.4 / 13.3; a token of
+// 61 with 9 rows of 7168 codes 7.0 / 11.5; 8000 rows of 4000 tokens 30 / 9.5, 8192 rows of 128 tokens 73 / 23.
+bool sort_few(int64_t M, int64_t top_k)
+{
+    const int64_t looks = (top_k + 7) / 8 * M * top_k;
+    return looks <= 6400 && looks * M <= 5000000;
+}
+
 template <int A>
 int sort_rows(SortParams p, int id_bits, hipStream_t hs)
 {
-    if (p.numel <= kSortFew)
+    if (sort_few(p.M, p.top_k))
         return status(launch(sort_few_kernel<A>, dim3(p.M + 1, (p.pieces + 1023) / 1024), dim3(256), 0, hs, p));
     const Segments g(p.numel, p.E);
     hipError_t err = launch(sort_hist_kernel, dim3(g.n), dim3(256), g.words * sizeof(int), hs, p, g.words, g.seg);
@@ -440,9 +457,9 @@ int sort_rows(SortParams p, int id_bits, hipStream_t hs)
     if (err != hipSuccess) return status(err);
     const int U = p.pieces <= 256 ? 1 : p.pieces <= 512 ? 2 : 4, along = threads_along(p.pieces, U), tokens = 256 / along;
     const dim3 grid((p.M + tokens - 1) / tokens, (p.pieces + along * U - 1) / (along * U)), block(along, tokens);
-    err = U == 1   ? launch(spread_kernel<A, 1>, grid, block, 0, hs, p)
-          : U == 2 ? launch(spread_kernel<A, 2>, grid, block, 0, hs, p)
-                   : launch(spread_kernel<A, 4>, grid, block, 0, hs, p);
+    const auto kernel = tokens > 1 ? spread_kernel<A, 1, false> : U == 1 ? spread_kernel<A, 1, true>
+                      : U == 2   ? spread_kernel<A, 2, true> : spread_kernel<A, 4, true>;
+    err = launch(kernel, grid, block, 0, hs, p);
     return status(err);
 }
 
@@ -450,7 +467,8 @@ template <typename T, int A>
 int combine_rows(const CombineParams &p, hipStream_t hs)
 {
     const int along = threads_along(p.pieces, 1), tokens = 256 / along;
-    return status(launch(combine_kernel<T, A>, dim3((p.M + tokens - 1) / tokens, (p.pieces + along - 1) / along), dim3(along, tokens), 0, hs, p));
+    return status(launch(tokens == 1 ? combine_kernel<T, A, true> : combine_kernel<T, A, false>,
+                         dim3((p.M + tokens - 1) / tokens, (p.pieces + along - 1) / along), dim3(along, tokens), 0, hs, p));
 }
 
 template <typename T, int A>
@@ -479,10 +497,10 @@ bool sizes_fit(int M, int top_k, int K, int value_bytes)
 
 using namespace alpha_moe;
 
-extern "C" size_t alpha_moe_sort_workspace_bytes(int numel, int num_experts)
+extern "C" size_t alpha_moe_sort_workspace_bytes(int M, int top_k, int num_experts)
 {
-    if (numel <= kSortFew || num_experts <= 0) return 0;
-    const Segments g(numel, num_experts);
+    if (!sizes_fit(M, top_k, 1, 1) || num_experts <= 0 || sort_few(M, top_k)) return 0;
+    const Segments g(M * top_k, num_experts);
     return (size_t)g.n * g.words * sizeof(int);
 }
 
@@ -504,7 +522,8 @@ extern "C" int alpha_moe_sort_tokens(const void *x, int value_bytes, const float
     p.pieces = (int)((p.row_bytes + 15) / 16);
     p.scale_cols = x_scale ? K / 128 : 0;
     p.M = M, p.top_k = top_k, p.E = num_experts, p.numel = M * top_k;
-    if (workspace_bytes < alpha_moe_sort_workspace_bytes(p.numel, num_experts) || (p.numel > kSortFew && !workspace))
+    const size_t need = alpha_moe_sort_workspace_bytes(M, top_k, num_experts);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3) != 0))
         return ALPHA_MOE_ERR_WORKSPACE;
     int id_bits = 0;
     while ((1 << id_bits) < num_experts + 1) id_bits++;

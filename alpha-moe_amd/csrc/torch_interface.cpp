@@ -689,7 +689,7 @@ Sorted run_sort(const at::Tensor &x, const at::Tensor *x_scale, const at::Tensor
     if (x_scale) r.scale = empty_on(dev, {M * top_k, K / 128}, at::kFloat);
     r.offsets = empty_on(dev, {num_experts + 1}, at::kInt);
     r.row_of_slot = empty_on(dev, {M, top_k}, at::kInt);
-    const size_t ws_bytes = alpha_moe_sort_workspace_bytes(static_cast<int>(M * top_k), static_cast<int>(num_experts));
+    const size_t ws_bytes = alpha_moe_sort_workspace_bytes(static_cast<int>(M), static_cast<int>(top_k), static_cast<int>(num_experts));
     at::Tensor ws;
     if (ws_bytes > 0) ws = empty_on(dev, {static_cast<int64_t>(ws_bytes)}, at::kByte);
     const int rc = alpha_moe_sort_tokens(

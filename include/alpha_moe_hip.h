@@ -291,7 +291,7 @@ int alpha_moe_route_topk(const void *logits, int is_f32, const float *bias, floa
  *   scale                x_scale's rows in the same order, zeros behind them (NULL exactly if x_scale is)
  *   offsets [num_experts + 1]  the first row of each expert; the last one is the number of slots that have one
  *   row_of_slot [M, top_k]     the slot's row r, or ~r (negative) where the row is one of the zeros
- * More than a few thousand slots need alpha_moe_sort_workspace_bytes(M * top_k, num_experts) bytes of workspace (any contents; 0: none).
+ * Larger calls need alpha_moe_sort_workspace_bytes(M, top_k, num_experts) bytes of workspace (any contents; 0: none).
  * M = 0 writes offsets.
  *
  * alpha_moe_combine_tokens: out[t] = scaling_factor * sum over s of topk_weights[t, s] * rows[row_of_slot[t, s]], summed in fp32 by ascending
@@ -304,7 +304,7 @@ int alpha_moe_route_topk(const void *logits, int is_f32, const float *bias, floa
  * [0, M * top_k) is neither read nor written.
  * M < 2^24 - 1, a row has at most 2^27 bytes.
  */
-size_t alpha_moe_sort_workspace_bytes(int numel, int num_experts);
+size_t alpha_moe_sort_workspace_bytes(int M, int top_k, int num_experts);
 int alpha_moe_sort_tokens(const void *x, int value_bytes, const float *x_scale, const int32_t *topk_ids, void *rows, float *scale,
                           int32_t *offsets, int32_t *row_of_slot, int M, int K, int top_k, int num_experts, void *workspace,
                           size_t workspace_bytes, void *stream /* hipStream_t */);

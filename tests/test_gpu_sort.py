@@ -243,7 +243,7 @@ def test_nothing_beside_the_results(M, top_k, E, K):
     R = M * top_k
     slots, offsets, at = L.sort_slots(ids, E)
     rows, off, row_of = guarded(R * K, torch.bfloat16), guarded(E + 1, torch.int32), guarded(R, torch.int32)
-    need = alpha_moe.c_abi.alpha_moe_sort_workspace_bytes(R, E)
+    need = alpha_moe.c_abi.alpha_moe_sort_workspace_bytes(M, top_k, E)
     ws = torch.full((need + 512,), 7, dtype=torch.uint8, device=DEV)
     xd, idd = x.to(DEV), ids.to(DEV)
     assert c_abi("alpha_moe_sort_tokens", xd.data_ptr(), 2, None, idd.data_ptr(), rows.data_ptr(), None, off.data_ptr(), row_of.data_ptr(),

@@ -26,10 +26,10 @@ def test_sort_refusals():
     assert sort(size=1, K=128, scale_in=4096) == NULL and sort(size=1, K=128, scale=4096) == NULL      # both or neither
     assert sort(x=4104) == ALIGN and sort(rows=4098) == ALIGN
     big = dict(M=40000, top_k=8, E=256)
-    need = A.alpha_moe_sort_workspace_bytes(320000, 256)
+    need = A.alpha_moe_sort_workspace_bytes(40000, 8, 256)
     assert need > 0 and sort(**big) == WORKSPACE and sort(**big, ws=4096, nws=need - 1) == WORKSPACE and sort(**big, nws=need) == WORKSPACE
-    assert A.alpha_moe_sort_workspace_bytes(64, 256) == 0 and A.alpha_moe_sort_workspace_bytes(-1, 8) == 0
-    assert A.alpha_moe_sort_workspace_bytes(320000, 0) == 0
+    assert A.alpha_moe_sort_workspace_bytes(8, 8, 256) == 0 and A.alpha_moe_sort_workspace_bytes(-1, 8, 8) == 0
+    assert A.alpha_moe_sort_workspace_bytes(40000, 8, 0) == 0 and A.alpha_moe_sort_workspace_bytes(40000, 65, 8) == 0
 
 
 def test_combine_refusals():
