@@ -10,10 +10,12 @@ for a ROCm build, and keeps the logic here so that it can be exercised without S
   helpers and the storing variant of the operator in place of zero-fill + add;
 * :func:`norm_moe`, :func:`norm_dense_mlp` - the feed-forward halves of a decoder layer from the residual addition on, an
   expert layer and a dense one, on this library's norm, router and block-scaled product (the reference has no part of
-  these; its callers take them from SGLang).
+  these; its callers take them from SGLang);
+* :func:`norm_sorted_moe` - an expert layer whose experts are spread over GPUs or whose weights the fused operator does not take,
+  on sorted tokens and one product for all experts.
 """
 import os
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -98,15 +100,63 @@ def norm_moe(hidden_states: torch.Tensor, residual: torch.Tensor, norm_weight: t
     return out, x.residual
 
 
+def norm_sorted_moe(hidden_states: torch.Tensor, residual: torch.Tensor, norm_weight: torch.Tensor, gate_weight: torch.Tensor,
+                    w13: torch.Tensor, w2: torch.Tensor, w13_scale: torch.Tensor, w2_scale: torch.Tensor, top_k: int,
+                    scoring: str = "softmax", correction_bias: Optional[torch.Tensor] = None, num_groups: int = 1,
+                    top_groups: int = 1, renormalize: bool = True, routed_scaling_factor: Optional[float] = None,
+                    eps: float = 1e-6, first_expert: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """An expert layer from the residual addition on, of which this GPU holds the experts ``first_expert, first_expert + 1, ...``:
+    ``(output, residual)``, both ``[M, K]`` bf16; the outputs of all GPUs add up to the layer's.
+
+    ``w13 [E, 2 I, K]`` and ``w2 [E, K, I]`` are in checkpoint order (the gate's rows, then the up projection's, NOT interleaved) with
+    scales per 128 x 128 block; ``gate_weight`` has the rows of all GPUs' experts.  Every token is routed; the slots of this GPU's experts
+    are sorted by expert as FP8 codes, go through both products, and come back as weighted sums.  Where the whole
+    layer's experts are here and interleaved, :func:`norm_moe` is the faster way."""
+    from .layer_hip import (combine_tokens, grouped_block_scaled_mm, rms_norm_quant_fp8, route_topk, sort_tokens,
+                            swiglu_quant_fp8)
+
+    experts = w13.shape[0]
+    if first_expert < 0 or first_expert + experts > gate_weight.shape[0]:
+        raise ValueError(f"experts {first_expert} to {first_expert + experts - 1} are not all of the gate's {gate_weight.shape[0]}")
+    bias = None if correction_bias is None else correction_bias.to(torch.float32)
+    x = rms_norm_quant_fp8(hidden_states, norm_weight, eps, residual=residual, keep_norm=True)
+    logits = torch.nn.functional.linear(x.norm.to(gate_weight.dtype), gate_weight)
+    weights, ids = route_topk(logits, top_k, scoring=scoring, bias=bias, num_groups=num_groups, top_groups=top_groups,
+                              renormalize=renormalize)
+    if first_expert:
+        ids = ids - first_expert
+    s = sort_tokens(x.q, ids, experts, x_scale=x.scale)
+    q, scale = swiglu_quant_fp8(grouped_block_scaled_mm(s.rows, s.scale, s.offsets, w13, w13_scale))
+    rows = grouped_block_scaled_mm(q, scale, s.offsets, w2, w2_scale)
+    return combine_tokens(rows, s.row_of_slot, weights, routed_scaling_factor or 1.0), x.residual
+
+
+class Adapters(NamedTuple):
+    """Low-rank adapters of a dense layer's two products, and which of them each token has (``layer_hip.add_adapters``)."""
+    a13: torch.Tensor
+    b13: torch.Tensor
+    a2: torch.Tensor
+    b2: torch.Tensor
+    ids: torch.Tensor
+    scale: Optional[torch.Tensor] = None
+
+
 def norm_dense_mlp(hidden_states: torch.Tensor, residual: torch.Tensor, norm_weight: torch.Tensor, w13: torch.Tensor,
-                   w2: torch.Tensor, w13_scale: torch.Tensor, w2_scale: torch.Tensor,
-                   eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+                   w2: torch.Tensor, w13_scale: torch.Tensor, w2_scale: torch.Tensor, eps: float = 1e-6,
+                   adapters: Optional[Adapters] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """A dense layer (or an unfused shared expert) from the residual addition on: ``(output, residual)``, both ``[M, K]`` bf16.
 
     ``w13 [2 I, K]`` holds the gate's rows, then the up projection's, as checkpoints do (NOT interleaved), ``w2 [K, I]``; scales
-    are per 128 x 128 block.  Four kernels: norm, product, SwiGLU, product."""
-    from .layer_hip import block_scaled_mm, rms_norm_quant_fp8, swiglu_quant_fp8
+    are per 128 x 128 block.  Four kernels: norm, product, SwiGLU, product.  With ``adapters`` (``a13 [L, rank, K]``, ``b13 [L, 2 I, rank]``,
+    ``a2 [L, rank, I]``, ``b2 [L, K, rank]``) two more behind each product, which read the codes that it reads."""
+    from .layer_hip import add_adapters, block_scaled_mm, rms_norm_quant_fp8, swiglu_quant_fp8
 
     x = rms_norm_quant_fp8(hidden_states, norm_weight, eps, residual=residual)
-    q, scale = swiglu_quant_fp8(block_scaled_mm(x.q, x.scale, w13, w13_scale))
-    return block_scaled_mm(q, scale, w2, w2_scale), x.residual
+    gate_up = block_scaled_mm(x.q, x.scale, w13, w13_scale)
+    if adapters is not None:
+        gate_up = add_adapters(gate_up, x.q, adapters.a13, adapters.b13, adapters.ids, adapters.scale, x.scale)
+    q, scale = swiglu_quant_fp8(gate_up)
+    out = block_scaled_mm(q, scale, w2, w2_scale)
+    if adapters is not None:
+        out = add_adapters(out, q, adapters.a2, adapters.b2, adapters.ids, adapters.scale, scale)
+    return out, x.residual

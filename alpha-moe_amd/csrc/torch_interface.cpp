@@ -865,22 +865,27 @@ at::Tensor combine_through_dispatcher(const at::Tensor &rows, const at::Tensor &
     return typed_op<decltype(combine_tokens)>("alpha_moe::combine_tokens").call(rows, row_of_slot, topk_weights, scaling_factor);
 }
 
+// (Only the rows are an output of the function: one that nobody can differentiate costs the backward pass as much as one that one can.)
 struct SortTokens : public torch::autograd::Function<SortTokens> {
-    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &topk_ids,
-                                                  int64_t num_experts)
+    struct Rest {
+        at::Tensor offsets, row_of_slot;
+    };
+    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &topk_ids, int64_t num_experts,
+                              Rest *rest)
     {
         const at::AutoDispatchBelowADInplaceOrView below;
-        const auto [rows, offsets, row_of_slot] =
+        auto [rows, offsets, row_of_slot] =
             typed_op<decltype(sort_tokens)>("alpha_moe::sort_tokens").call(x, topk_ids, num_experts);
         ctx->save_for_backward({row_of_slot});
-        ctx->mark_non_differentiable({offsets, row_of_slot});
-        return {rows, offsets, row_of_slot};
+        *rest = {std::move(offsets), std::move(row_of_slot)};
+        return std::move(rows);
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads)
     {
-        if (!grads[0].defined()) return {at::Tensor(), at::Tensor(), at::Tensor()};
-        return {combine_through_dispatcher(grads[0].contiguous(), ctx->get_saved_variables()[0], c10::nullopt, 1.0), at::Tensor(),
-                at::Tensor()};
+        at::Tensor grad;
+        if (grads[0].defined())
+            grad = combine_through_dispatcher(grads[0].contiguous(), ctx->get_saved_variables()[0], c10::nullopt, 1.0);
+        return {std::move(grad), at::Tensor(), at::Tensor(), at::Tensor()};
     }
 };
 std::tuple<at::Tensor, at::Tensor, at::Tensor> sort_tokens_autograd(c10::DispatchKeySet keys, const at::Tensor &x,
@@ -890,8 +895,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> sort_tokens_autograd(c10::Dispatc
     if (wanted && at::isFloat8Type(x.scalar_type())) refuse_gradient(x, "x");   // (of codes)
     if (!wanted)
         return typed_op<decltype(sort_tokens)>("alpha_moe::sort_tokens").redispatch(keys & c10::after_autograd_keyset, x, topk_ids, num_experts);
-    auto r = SortTokens::apply(x, topk_ids, num_experts);
-    return {r[0], r[1], r[2]};
+    SortTokens::Rest rest;
+    at::Tensor rows = SortTokens::apply(x, topk_ids, num_experts, &rest);
+    return {std::move(rows), std::move(rest.offsets), std::move(rest.row_of_slot)};
 }
 
 struct CombineTokens : public torch::autograd::Function<CombineTokens> {
