@@ -122,10 +122,11 @@ __device__ __forceinline__ void store4(const MmParams &p, int m, int n, v4f v)
 }
 
 // ---- groups of tokens with weights of their own ---------------------------------------------------------------
-// A tile of a grouped launch: rows [lo, lo + rows) of x, `token_tile` of the group's `token_tiles`, and a group of columns; expert E
-// stands for the rows behind the last expert's, which become 0.
+// A tile of a grouped launch: of rows [lo, lo + rows) of x those from m0 on, columns from c0 on; expert E stands for the rows behind the last
+// expert's, which become 0.  half: at most half as many tokens as a whole tile's.
 struct GroupTile {
-    int expert, lo, rows, token_tile, row_group;
+    int expert, lo, rows, m0, c0;
+    bool half;
 };
 
 __device__ __forceinline__ int wave_scan(int v)   // inclusive sums over the wavefront
@@ -140,17 +141,18 @@ __device__ __forceinline__ int wave_scan(int v)   // inclusive sums over the wav
 }
 
 // The tile of this workgroup, if there is one.  How many there are, only the device knows: each wavefront counts the experts' tiles,
-// 256 experts' offsets in flight at a time, and looks for its own.  (A run of experts to a lane, one offset
-// behind the other, took some 0.3 us more of every workgroup.)  An expert's tiles follow each other, its tiles of tokens in groups
-// of HIGH (0: all of them) next to each other; each XCD gets a run of tiles.  Offsets are taken into [0, M], and where they do not ascend
-// then, nobody has a tile.
-template <int TOKENS, int HIGH>
+// 256 experts' offsets in flight at a time, and looks for its own.  (A run of experts to a lane, one offset behind the other, took some
+// 0.3 us more of every workgroup.)  An expert's tiles follow each other, its tiles of tokens in groups of HIGH (0: all of them) next to each
+// other; each XCD gets a run of tiles.  HALVES: an expert's last tile may be a half one, and those come behind all whole ones, so that
+// what is left at the end is short.  Offsets are taken into [0, M], and where they do not ascend then, nobody has a tile.
+template <int COLS, int TOKENS, int HIGH, bool HALVES>
 __device__ __forceinline__ bool find_tile(const MmParams &p, GroupTile &g)
 {
     constexpr int Q = 4;
     const int lane = threadIdx.x & 63;
     auto clamped = [&](int row) { return min(max(row, 0), p.M); };
-    auto tiles_of_rows = [](int rows) { return rows > 0 ? (rows + TOKENS - 1) / TOKENS : 0; };
+    auto wholes_in = [](int rows) { return rows > 0 ? (rows + (HALVES ? TOKENS / 2 : TOKENS) - 1) / TOKENS : 0; };
+    auto halves_in = [](int rows) { return HALVES && rows > 0 && (unsigned)(rows - 1) % TOKENS < TOKENS / 2 ? 1 : 0; };
     int from[Q], to[Q];
     auto load = [&](int base) {
 #pragma unroll
@@ -163,37 +165,47 @@ __device__ __forceinline__ bool find_tile(const MmParams &p, GroupTile &g)
         for (int j = 0; j < Q; j++) from[j] = clamped(from[j]), to[j] = clamped(to[j]);
     };
     const int last = clamped(p.offsets[p.E]);
-    int sum = 0;
+    int sum = 0, half_sum = 0;
     bool ascend = true;
     for (int base = 0; base < p.E; base += 64 * Q) {
         load(base);
 #pragma unroll
         for (int j = 0; j < Q; j++) {
             ascend &= to[j] >= from[j];
-            sum += tiles_of_rows(to[j] - from[j]);
+            sum += wholes_in(to[j] - from[j]);
+            half_sum += halves_in(to[j] - from[j]);
         }
     }
     if (!__all(ascend)) return false;
-    const int of_experts = __builtin_amdgcn_readlane(wave_scan(sum), 63), tail = tiles_of_rows(p.M - last);
-    const int total = (of_experts + tail) * p.row_groups, run = (total + 7) >> 3;
-    const int in_run = (int)(blockIdx.x >> 3), tile = (int)(blockIdx.x & 7) * run + in_run;
-    if (in_run >= run || tile >= total) return false;
+    const int of_experts = __builtin_amdgcn_readlane(wave_scan(sum), 63), tail = (p.M - last + TOKENS - 1) / TOKENS;
+    const int wholes = (of_experts + tail) * p.row_groups, run = (wholes + 7) >> 3;
+    int in_run = (int)(blockIdx.x >> 3), tile = (int)(blockIdx.x & 7) * run + in_run;
+    g.half = HALVES && in_run >= run;
+    if (g.half) {
+        const int halves = __builtin_amdgcn_readlane(wave_scan(half_sum), 63) * p.row_groups, half_run = (halves + 7) >> 3;
+        in_run -= run;
+        tile = (int)(blockIdx.x & 7) * half_run + in_run;
+        if (in_run >= half_run || tile >= halves) return false;
+    } else if (in_run >= run || tile >= wholes) {
+        return false;
+    }
     const int at = tile / p.row_groups;   // among the tiles of tokens
     int before = of_experts;
     g.expert = p.E, g.lo = last, g.rows = p.M - last;
-    if (at < of_experts) {
+    if (g.half || at < of_experts) {
         before = 0;
         bool found = false;
         for (int base = 0; !found; base += 64 * Q) {
             if (p.E > 64 * Q) load(base);   // (otherwise they are all there)
 #pragma unroll
             for (int j = 0; j < Q; j++) {
-                const int tiles = tiles_of_rows(to[j] - from[j]), incl = wave_scan(tiles), all = __builtin_amdgcn_readlane(incl, 63);
+                const int rows = to[j] - from[j], tiles = g.half ? halves_in(rows) : wholes_in(rows), incl = wave_scan(tiles),
+                          all = __builtin_amdgcn_readlane(incl, 63);
                 if (!found && at < before + all) {
                     const int owner = (int)__builtin_ctzll(__ballot(before + incl > at));
                     g.expert = base + 64 * j + owner;
                     g.lo = __builtin_amdgcn_readlane(from[j], owner);
-                    g.rows = __builtin_amdgcn_readlane(to[j] - from[j], owner);
+                    g.rows = __builtin_amdgcn_readlane(rows, owner);
                     before += __builtin_amdgcn_readlane(incl - tiles, owner);
                     found = true;
                 }
@@ -201,28 +213,33 @@ __device__ __forceinline__ bool find_tile(const MmParams &p, GroupTile &g)
             }
         }
     }
-    const int token_tiles = tiles_of_rows(g.rows), inside = tile - before * p.row_groups;
+    const int inside = tile - before * p.row_groups;
+    if (g.half) {
+        g.c0 = inside * COLS;
+        g.m0 = g.rows / TOKENS * TOKENS;
+        return true;
+    }
     // (a launch has fewer than 2^24 tiles, so HIGH, which is 8, times the groups of columns is an int)
+    const int token_tiles = g.expert == p.E ? tail : wholes_in(g.rows);
     const int per_group = HIGH * p.row_groups, group = HIGH > 0 ? inside / per_group : 0, in_group = inside - group * per_group;
     const int high = HIGH > 0 ? min(token_tiles - group * HIGH, HIGH) : token_tiles;
-    g.row_group = in_group / high;
-    g.token_tile = group * HIGH + in_group - g.row_group * high;
+    const int row_group = in_group / high;
+    g.c0 = row_group * COLS;
+    g.m0 = (group * HIGH + in_group - row_group * high) * TOKENS;
     return true;
 }
 
 // What a workgroup multiplies, of a grouped launch: p becomes the expert's own product, rows [m0, p.M) and columns from c0 on.  Returns
 // false where there is nothing to multiply.
-template <int COLS, int TOKENS, int HIGH, int THREADS>
-__device__ __forceinline__ bool enter_group(MmParams &p, int &c0, int &m0)
+template <int COLS, int TOKENS, int HIGH, int THREADS, bool HALVES>
+__device__ __forceinline__ bool enter_group(MmParams &p, GroupTile &g)
 {
-    GroupTile g;
-    if (!find_tile<TOKENS, HIGH>(p, g)) return false;
-    c0 = g.row_group * COLS, m0 = g.token_tile * TOKENS;
-    p.M = min(g.rows, m0 + TOKENS);
+    if (!find_tile<COLS, TOKENS, HIGH, HALVES>(p, g)) return false;
+    p.M = min(g.rows, g.m0 + TOKENS);
     p.out += (size_t)g.lo * p.N;
     if (g.expert == p.E) {
         for (int i = threadIdx.x; i < TOKENS * (COLS / 8); i += THREADS) {
-            const int m = m0 + i / (COLS / 8), n = c0 + i % (COLS / 8) * 8;
+            const int m = g.m0 + i / (COLS / 8), n = g.c0 + i % (COLS / 8) * 8;
             if (m >= p.M) break;
             uint16_t *at = p.out + (size_t)m * p.N + n;
             if (n + 8 <= p.N) *reinterpret_cast<any4 *>(at) = (any4){0, 0, 0, 0};
@@ -281,7 +298,9 @@ __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(MmParams p)
     // workgroups are dealt to the eight XCDs in turn: each gets a run of tiles, token groups of one row group next to each other
     int c0, m0;
     if constexpr (GROUPED) {
-        if (!enter_group<R * 16, HALF ? 8 : T * 16, 0, WAVES * 64>(p, c0, m0)) return;
+        GroupTile g;
+        if (!enter_group<R * 16, HALF ? 8 : T * 16, 0, WAVES * 64, false>(p, g)) return;
+        c0 = g.c0, m0 = g.m0;
     } else {
         const int tiles = p.row_groups * p.token_groups, run = (tiles + 7) >> 3;
         const int tile = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
@@ -441,10 +460,10 @@ hipError_t launch_tiles(Kernel kernel, MmParams p, int cols, int tokens, int thr
 {
     const int64_t token_groups = grouped ? most_token_tiles(p.M, p.E, tokens) : (p.M + (int64_t)tokens - 1) / tokens;
     const int64_t tiles = ((int64_t)p.N + cols - 1) / cols * token_groups;
-    if (!grid_fits(tiles, threads)) return hipErrorInvalidConfiguration;
+    if (!grid_fits(tiles + (grouped ? 8 : 0), threads)) return hipErrorInvalidConfiguration;
     p.row_groups = (p.N + cols - 1) / cols;
     p.token_groups = (int)token_groups;
-    const unsigned run = (unsigned)((tiles + 7) / 8);
+    const unsigned run = (unsigned)((tiles + 7) / 8) + (grouped ? 1 : 0);   // (runs of whole and of half tiles: each may be one longer)
     void *args[] = {&p};
     return hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3(run * 8), dim3(threads), args, 0, stream);
 }
@@ -704,7 +723,9 @@ __global__ __launch_bounds__((WN * WM + LOADERS) * 64, 2) void mm_tile_kernel(Mm
     constexpr int kGroup = 8;
     int c0, m0;
     if constexpr (GROUPED) {
-        if (!enter_group<T::kCols, T::kTokens, kGroup, (T::kWaves + LOADERS) * 64>(p, c0, m0)) return;
+        GroupTile g;
+        if (!enter_group<T::kCols, T::kTokens, kGroup, (T::kWaves + LOADERS) * 64, false>(p, g)) return;
+        c0 = g.c0, m0 = g.m0;
     } else {
         const int tiles = p.row_groups * p.token_groups, run = (tiles + 7) >> 3;
         const int tile = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
@@ -723,10 +744,10 @@ __global__ __launch_bounds__(512, 2) void mm_ragged_tile_kernel(MmParams p)
     typedef Tile<4, 8, 4, 2, 2, 0> Whole;
     typedef Tile<4, 4, 4, 2, 3, 0> Half;
     __shared__ __attribute__((aligned(128))) uint8_t lds[Whole::kBytes > Half::kBytes ? Whole::kBytes : Half::kBytes];
-    int c0, m0;
-    if (!enter_group<Whole::kCols, Whole::kTokens, 8, 512>(p, c0, m0)) return;
-    if (p.M - m0 > Half::kTokens) mm_tile<4, 8, 4, 2, 2, 0, true>(p, c0, m0, lds);
-    else mm_tile<4, 4, 4, 2, 3, 0, true>(p, c0, m0, lds);
+    GroupTile g;
+    if (!enter_group<Whole::kCols, Whole::kTokens, 8, 512, true>(p, g)) return;
+    if (!g.half) mm_tile<4, 8, 4, 2, 2, 0, true>(p, g.c0, g.m0, lds);
+    else mm_tile<4, 4, 4, 2, 3, 0, true>(p, g.c0, g.m0, lds);
 }
 
 template <int TN, int TM, int WN, int WM, int S, int LOADERS, bool GROUPED = false>

@@ -154,3 +154,11 @@ def test_replays_with_other_groups():
         torch.cuda.synchronize()
         assert torch.equal(out, layer_hip.grouped_block_scaled_mm(*args))
         check(*(t.cpu() for t in args), out)
+
+
+@pytest.mark.parametrize("rest", [0, 1, 127, 128, 129, 255])
+def test_last_tiles_of_any_length(rest):
+    """many rows of few K blocks take the largest tile, whose last one of an expert may be a half one"""
+    counts = [256 * k + rest for k in (0, 1, 3)] + [0, 700, 40]
+    args = problem(counts, 5, 300, 256, rest)
+    check(*args, run(*args))
