@@ -97,7 +97,7 @@ c_abi.alpha_moe_combine_tokens_grad.argtypes = (
 c_abi.alpha_moe_grouped_block_scaled_mm.restype = ctypes.c_int
 c_abi.alpha_moe_grouped_block_scaled_mm.argtypes = [ctypes.c_void_p] * 6 + [ctypes.c_int] * 4 + [ctypes.c_void_p]
 c_abi.alpha_moe_adapters_workspace_bytes.restype = ctypes.c_size_t
-c_abi.alpha_moe_adapters_workspace_bytes.argtypes = [ctypes.c_int] * 4
+c_abi.alpha_moe_adapters_workspace_bytes.argtypes = [ctypes.c_int] * 5
 c_abi.alpha_moe_add_adapters.restype = ctypes.c_int
 c_abi.alpha_moe_add_adapters.argtypes = (
     [ctypes.c_void_p] * 8 + [ctypes.c_int] * 5 + [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p])

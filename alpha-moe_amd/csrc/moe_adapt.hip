@@ -349,20 +349,24 @@ __global__ __launch_bounds__(256, RT == 8 ? 3 : 4) void adapt_out_kernel(const A
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tokens of a tile, workgroups that share a tile's adapters, and parts of K.
+// Tokens of a tile, workgroups that share a tile's adapters, and parts of K.  A tile of 64 tokens reads its adapters a quarter as often, one of
+// 16 is seldom of two requests.  MI355X, us, 16 / 64 tokens: 2048 tokens of 64 requests, K = 7168, N = 2112, rank 32 29 / 35; 8000
+// of 20, K = 7168, N = 512, rank 64 98 / 54; 8192 of 37, K = 2048, N = 7168, rank 64 140 / 87; 7759 of one, K = 3200, N = 177, rank 16
+// 22 / 27; 4000 of 20, K = 4096, N = 1024, rank 16 20 / 23.  One workgroup to a tile's adapters instead of two to sixteen: 61 tokens of 48
+// adapters 28 for 13.5, 8192 of 37 requests 109 for 87 (what a tile does not need ends at once, but takes its turn).
 struct AdaptPlan {
     int T, sharers, splits;
-    AdaptPlan(int M, int K, int rank, int adapters)
+    AdaptPlan(int M, int N, int K, int rank, int adapters)
     {
         const int nkb = K / 128;
-        T = M <= 2048 ? 1 : rank > 64 ? 2 : 4;
+        T = M <= 2048 || (rank <= 32 && N <= 1024) ? 1 : rank > 64 ? 2 : 4;
         const int64_t tiles = ceil_div(M, 16 * T);
         const int most = adapters < 16 * T ? adapters : 16 * T;
         sharers = tiles < 32 ? (int)ceil_div(128, tiles) : T == 1 && tiles >= 96 ? 2 : 4;
         sharers = sharers > most ? most : sharers;
         sharers = sharers > M ? M : sharers;
         const int64_t groups = tiles * sharers, can = ceil_div(nkb, 4);
-        const int64_t want = T > 1 ? ceil_div(1024, groups) : groups < 128 ? ceil_div(1024, groups) : 8;
+        const int64_t want = T > 1 || groups < 128 ? ceil_div(1024, groups) : groups <= 512 ? 8 : 4;
         splits = (int)(want > can ? can : want);
     }
 };
@@ -399,10 +403,10 @@ bool sizes_fit(int M, int N, int K, int rank, int adapters)
 
 using namespace alpha_moe;
 
-extern "C" size_t alpha_moe_adapters_workspace_bytes(int M, int K, int rank, int num_adapters)
+extern "C" size_t alpha_moe_adapters_workspace_bytes(int M, int N, int K, int rank, int num_adapters)
 {
-    if (M <= 0 || !sizes_fit(M, 1, K, rank, num_adapters)) return 0;
-    return (size_t)AdaptPlan(M, K, rank, num_adapters).splits * M * rank * sizeof(float);
+    if (M <= 0 || !sizes_fit(M, N, K, rank, num_adapters)) return 0;
+    return (size_t)AdaptPlan(M, N, K, rank, num_adapters).splits * M * rank * sizeof(float);
 }
 
 extern "C" int alpha_moe_add_adapters(const uint16_t *base, const void *x, const float *x_scale, const uint16_t *a, const uint16_t *b,
@@ -418,9 +422,9 @@ extern "C" int alpha_moe_add_adapters(const uint16_t *base, const void *x, const
         all |= reinterpret_cast<uintptr_t>(ptr);
     if ((all & 15) != 0) return ALPHA_MOE_ERR_ALIGNMENT;
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
-        workspace_bytes < alpha_moe_adapters_workspace_bytes(M, K, rank, num_adapters))
+        workspace_bytes < alpha_moe_adapters_workspace_bytes(M, N, K, rank, num_adapters))
         return ALPHA_MOE_ERR_WORKSPACE;
-    const AdaptPlan plan(M, K, rank, num_adapters);
+    const AdaptPlan plan(M, N, K, rank, num_adapters);
     AdaptParams p = {};
     p.base = base, p.a = a, p.b = b, p.x = static_cast<const uint8_t *>(x), p.x_scale = x_scale, p.scale = scale;
     p.ids = adapter_ids, p.out = out, p.part = static_cast<float *>(workspace);

@@ -804,6 +804,9 @@ Plan grouped_plan(int M, int N, int K, int E)
 {
     const int mean = M / E, nkb = K / 128;
     if (tiles_of(M, N, 32, 1) <= kUnits / 2) return kStreamHalf1;
+    // Too few tiles of 128 x 64 for the units (if every other expert has one more than its rows fill), and a long K, which the streaming
+    // kernel's wavefronts share: 32x16 / 128x64 8 experts, 25 rows, N = 142, K = 6528 8.7 / 22; 60 rows, N = 903, K = 1408 10.4 / 9.1.
+    if (mean <= nkb && (M / 64 + (E < M ? E : M) / 2 + 1) * (int64_t)((N + 127) / 128) <= kUnits / 2) return kStream2x1;
     if (mean <= 8 && nkb >= 12) return kStream2x1;
     return mean >= 12 * nkb ? kTile256x256 : mean <= 40 ? kTile128x64 : kTile256x128;
 }

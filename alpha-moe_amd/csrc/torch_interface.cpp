@@ -608,8 +608,8 @@ at::Tensor add_adapters(const at::Tensor &base, const at::Tensor &x, const c10::
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(dev);
     hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream();
     at::Tensor out = empty_on(dev, {M, N}, at::kBFloat16);
-    const size_t ws_bytes = alpha_moe_adapters_workspace_bytes(static_cast<int>(M), static_cast<int>(K), static_cast<int>(rank),
-                                                               static_cast<int>(L));
+    const size_t ws_bytes = alpha_moe_adapters_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K),
+                                                               static_cast<int>(rank), static_cast<int>(L));
     at::Tensor ws = empty_on(dev, {static_cast<int64_t>(ws_bytes)}, at::kByte);
     const int rc = alpha_moe_add_adapters(
         static_cast<const uint16_t *>(base.const_data_ptr()), x.const_data_ptr(),

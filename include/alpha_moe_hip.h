@@ -335,7 +335,7 @@ int alpha_moe_grouped_block_scaled_mm(const uint8_t *x, const float *x_scale, co
  * may stand for one of a small value and it: what an infinity in b meets is infinite or NaN.  workspace:
  * alpha_moe_adapters_workspace_bytes() bytes, 16-byte aligned, any contents, for one call at a time.
  */
-size_t alpha_moe_adapters_workspace_bytes(int M, int K, int rank, int num_adapters);
+size_t alpha_moe_adapters_workspace_bytes(int M, int N, int K, int rank, int num_adapters);
 int alpha_moe_add_adapters(const uint16_t *base, const void *x, const float *x_scale, const uint16_t *a, const uint16_t *b,
                            const int32_t *adapter_ids, const float *scale, uint16_t *out, int M, int N, int K, int rank,
                            int num_adapters, void *workspace, size_t workspace_bytes, void *stream /* hipStream_t */);

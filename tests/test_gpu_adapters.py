@@ -57,7 +57,9 @@ def check(p, got):
     (17, 65, 128, 40, 2, False), (33, 257, 1152, 64, 33, True), (61, 2112, 1024, 8, 48, True), (64, 300, 512, 128, 7, False),
     (100, 129, 256, 72, 100, True), (257, 1000, 384, 48, 9, False), (600, 130, 128, 16, 600, False), (1025, 66, 256, 16, 20, False),
     (1100, 255, 128, 32, 6, True), (1030, 513, 384, 56, 11, True), (1040, 64, 256, 104, 5, False), (2000, 31, 128, 8, 70, True),
-    (5, 96, 65536, 16, 2, True), (3, 40, 16384, 128, 3, False)])
+    (5, 96, 65536, 16, 2, True), (3, 40, 16384, 128, 3, False),
+    (2100, 33, 128, 16, 9, False), (2300, 1040, 128, 24, 7, True), (2070, 1100, 256, 64, 3, False), (2080, 70, 128, 48, 12, True),
+    (2060, 40, 128, 128, 5, False)])
 def test_adapters(M, N, K, rank, adapters, fp8, ids):
     print(f"case adapters M={M} N={N} K={K} rank={rank} of {adapters} fp8={fp8} {ids}", flush=True)
     p = problem(M, N, K, rank, adapters, ids, fp8, scaled=M % 2 == 1)
@@ -141,7 +143,7 @@ def test_nothing_beside_the_rows_and_in_place(M, N, rank):
     p = problem(M, N, K, rank, adapters, "mixed")
     d = {k: None if v is None else v.to(DEV) for k, v in p.items()}
     want = run(p)
-    need = alpha_moe.c_abi.alpha_moe_adapters_workspace_bytes(M, K, rank, adapters)
+    need = alpha_moe.c_abi.alpha_moe_adapters_workspace_bytes(M, N, K, rank, adapters)
     ws = torch.full((need + 512,), 7, dtype=torch.uint8, device=DEV)
     out = torch.cat([p["base"].flatten(), torch.full((2048,), 7.0, dtype=BF)]).to(DEV)
     rc = alpha_moe.c_abi.alpha_moe_add_adapters(out.data_ptr(), d["x"].data_ptr(), None, d["a"].data_ptr(), d["b"].data_ptr(),

@@ -142,9 +142,9 @@ def test_adapter_refusals_and_shapes():
         assert call(**{name: None}) == NULL, name
     for name in ("base", "x", "a", "b", "out"):
         assert call(**{name: 4104}) == ALIGN, name
-    need = A.alpha_moe_adapters_workspace_bytes(4, 256, 16, 8)
+    need = A.alpha_moe_adapters_workspace_bytes(4, 100, 256, 16, 8)
     assert need >= 4 * 16 * 4 and call(ws=None) == WORKSPACE and call(ws=4104) == WORKSPACE and call(nws=need - 1) == WORKSPACE
-    assert A.alpha_moe_adapters_workspace_bytes(0, 256, 16, 8) == 0 and A.alpha_moe_adapters_workspace_bytes(4, 256, 15, 8) == 0
+    assert A.alpha_moe_adapters_workspace_bytes(0, 100, 256, 16, 8) == 0 and A.alpha_moe_adapters_workspace_bytes(4, 100, 256, 15, 8) == 0
     base, x, ids = meta((6, 100), torch.bfloat16), meta((6, 256), torch.bfloat16), meta((6,), torch.int32)
     a, b = meta((3, 16, 256), torch.bfloat16), meta((3, 100, 16), torch.bfloat16)
     out = layer_hip.add_adapters(base, x, a, b, ids, scale=meta((3,)))
