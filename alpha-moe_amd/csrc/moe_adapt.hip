@@ -30,7 +30,7 @@ struct AdaptParams {
     const int32_t *ids;
     uint16_t *out;
     float *part;               // [splits][M][rank]
-    int M, N, K, rank, adapters, nkb, splits, sharers, run, tiles, pieces;
+    int M, N, K, rank, adapters, nkb, splits, sharers, run, tiles, pieces, rank_groups;
 };
 
 // LDS accesses of one wavefront complete in order; this keeps the compiler to the written order
@@ -97,16 +97,17 @@ __device__ __forceinline__ void widen(v4i codes, v8bf (&to)[2])
     to[1] = __builtin_bit_cast(v8bf, half[1]);
 }
 
-// part[split][token][rank]: RT tiles of 16 ranks, T tiles of 16 tokens; the four wavefronts take the split's K blocks in turn.
+// part[split][token][rank]: RT tiles of 16 ranks of p.rank_groups times as many, T tiles of 16 tokens; the four wavefronts take the split's K
+// blocks in turn.
 template <int RT, int T, bool FP8>
-__global__ __launch_bounds__(256) void adapt_in_kernel(const AdaptParams p)
+__global__ __launch_bounds__(256, 2) void adapt_in_kernel(const AdaptParams p)
 {
     __shared__ v4f sums[4][RT * T][64];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, q = lane >> 4;
     Place place;
-    if (!find_place(p.tiles, p.splits, place)) return;
-    const int m0 = place.tile * (16 * T), split = place.piece;
+    if (!find_place(p.tiles, p.splits * p.rank_groups, place)) return;
+    const int m0 = place.tile * (16 * T), split = place.piece / p.rank_groups, r0 = (place.piece - split * p.rank_groups) * (16 * RT);
     const int first = (int)((int64_t)split * p.nkb / p.splits), last = (int)((int64_t)(split + 1) * p.nkb / p.splits);
     const int id = lane < 16 * T && m0 + lane < p.M ? p.ids[m0 + lane] : -1;
     const int K = p.K;
@@ -122,7 +123,7 @@ __global__ __launch_bounds__(256) void adapt_in_kernel(const AdaptParams p)
             v8bf av[RT][4], xv[T][4];
 #pragma unroll
             for (int r = 0; r < RT; r++) {
-                const v8bf *at = reinterpret_cast<const v8bf *>(a + (size_t)min(16 * r + n, p.rank - 1) * K + kb * 128 + q * 16);
+                const v8bf *at = reinterpret_cast<const v8bf *>(a + (size_t)min(r0 + 16 * r + n, p.rank - 1) * K + kb * 128 + q * 16);
 #pragma unroll
                 for (int i = 0; i < 4; i++) av[r][i] = at[8 * (i / 2) + i % 2];
             }
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(256) void adapt_in_kernel(const AdaptParams p)
             for (int t = 0; t < T; t++) sums[w][r * T + t][lane] = acc[r][t];
         __syncthreads();
         for (int e = tid; e < RT * T * 64; e += 256) {
-            const int l = e & 63, t = (e >> 6) % T, r = (e >> 6) / T, rank = 16 * r + 4 * (l >> 4), at = 16 * t + (l & 15);
+            const int l = e & 63, t = (e >> 6) % T, r = (e >> 6) / T, rank = r0 + 16 * r + 4 * (l >> 4), at = 16 * t + (l & 15);
             const v4f s = sums[0][e >> 6][l] + sums[1][e >> 6][l] + sums[2][e >> 6][l] + sums[3][e >> 6][l];
             if (rank < p.rank && ((same >> at) & 1))
                 *reinterpret_cast<v4f *>(p.part + ((size_t)split * p.M + m0 + at) * p.rank + rank) = s;
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(256, RT == 8 ? 3 : 4) void adapt_out_kernel(const A
             const float *from = p.part + (size_t)(m0 + t) * rank + r;
             const size_t step = (size_t)p.M * rank;
             v4f v = {0.f, 0.f, 0.f, 0.f};
-            constexpr int F = T == 1 ? 8 : 2;   // loads in flight
+            constexpr int F = T == 1 ? 8 : 4;   // loads in flight
             for (int s0 = 0; s0 < p.splits; s0 += F) {
                 v4f in[F];
 #pragma unroll
@@ -349,24 +350,30 @@ __global__ __launch_bounds__(256, RT == 8 ? 3 : 4) void adapt_out_kernel(const A
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tokens of a tile, workgroups that share a tile's adapters, and parts of K.  A tile of 64 tokens reads its adapters a quarter as often, one of
-// 16 is seldom of two requests.  MI355X, us, 16 / 64 tokens: 2048 tokens of 64 requests, K = 7168, N = 2112, rank 32 29 / 35; 8000
-// of 20, K = 7168, N = 512, rank 64 98 / 54; 8192 of 37, K = 2048, N = 7168, rank 64 140 / 87; 7759 of one, K = 3200, N = 177, rank 16
-// 22 / 27; 4000 of 20, K = 4096, N = 1024, rank 16 20 / 23.  One workgroup to a tile's adapters instead of two to sixteen: 61 tokens of 48
-// adapters 28 for 13.5, 8192 of 37 requests 109 for 87 (what a tile does not need ends at once, but takes its turn).
+// Each kernel's tokens of a tile and workgroups that share a tile's adapters, and the parts of K.  A tile of 64 tokens reads its adapters a
+// quarter as often; one of 16 is seldom of two requests, and has less to do one behind the other.  MI355X, us, 16 / 64 tokens in the first
+// kernel: 2048 tokens of 64 requests, K = 7168, N = 2112, rank 32 28.8 / 33.5, 3890 of 40, K = 5120, N = 173, rank 64 48 / 40, 7759 of one, K =
+// 3200, N = 177, rank 16 22 / 19; in the second: 8192 of 37, K = 2048, N = 7168, rank 64 113 / 85, 3890 of 40 as before 40 / 50.  One workgroup
+// to a tile's adapters instead of two to sixteen: 61 tokens of 48 adapters 28 for 13, 8192 of 37 requests 109 for 87 (those a tile has no
+// adapters for end at once, but take their turn).
 struct AdaptPlan {
-    int T, sharers, splits;
+    struct Tiles {
+        int tokens, sharers;
+    } in, out;
+    int splits;
     AdaptPlan(int M, int N, int K, int rank, int adapters)
     {
-        const int nkb = K / 128;
-        T = M <= 2048 || (rank <= 32 && N <= 1024) ? 1 : rank > 64 ? 2 : 4;
-        const int64_t tiles = ceil_div(M, 16 * T);
-        const int most = adapters < 16 * T ? adapters : 16 * T;
-        sharers = tiles < 32 ? (int)ceil_div(128, tiles) : T == 1 && tiles >= 96 ? 2 : 4;
-        sharers = sharers > most ? most : sharers;
-        sharers = sharers > M ? M : sharers;
-        const int64_t groups = tiles * sharers, can = ceil_div(nkb, 4);
-        const int64_t want = T > 1 || groups < 128 ? ceil_div(1024, groups) : groups <= 512 ? 8 : 4;
+        auto shared = [&](int tokens) {
+            const int64_t tiles = ceil_div(M, tokens);
+            int64_t n = tiles < 32 ? ceil_div(128, tiles) : tokens == 16 && tiles >= 96 ? 2 : 4;
+            for (const int most : {adapters, tokens, M}) n = n < most ? n : most;
+            return Tiles{tokens, (int)n};
+        };
+        in = shared((int64_t)M * rank > 65536 ? 64 : 16);
+        out = shared(M <= 2048 || N <= 1024 ? 16 : rank > 64 ? 32 : 64);
+        const int64_t groups = ceil_div(M, in.tokens) * in.sharers, can = ceil_div(K / 128, 4);
+        int64_t want = in.tokens == 16 ? (groups <= 512 ? 8 : 4) : ceil_div(1024, groups);
+        if (in.tokens == 64 && M > 2048 && want > 4) want = 4;
         splits = (int)(want > can ? can : want);
     }
 };
@@ -378,18 +385,29 @@ hipError_t launch(void (*kernel)(Args...), dim3 grid, dim3 block, hipStream_t st
     return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, list, 0, stream);
 }
 
-template <int RT, int T>
-hipError_t adapt(AdaptParams p, hipStream_t hs)
+// A kernel with `each` times `sharers` workgroups to a tile.  A launch has less than 2^32 threads.
+hipError_t launch_tiles(void (*kernel)(AdaptParams), AdaptParams p, const AdaptPlan::Tiles &tiles, int64_t each, hipStream_t hs)
 {
-    p.tiles = (int)ceil_div(p.M, 16 * T);
+    p.tiles = (int)ceil_div(p.M, tiles.tokens), p.sharers = tiles.sharers;
+    const int64_t groups = 8 * ceil_div(p.tiles * each, 8) * p.sharers;
+    if (groups * 256 >= (int64_t(1) << 32)) return hipErrorInvalidConfiguration;
+    return launch(kernel, dim3((unsigned)groups), dim3(256), hs, p);
+}
+
+// Of many ranks, each workgroup of the first kernel takes a group: 32 of few tokens, whose parts are little work for many units (44 tokens,
+// K = 4736, N = 1357, rank 128 15 us in one, 11.5 in four), 64 of many, so that 64 tokens' sums fit the registers.
+template <int RT>
+hipError_t adapt(AdaptParams p, const AdaptPlan &plan, hipStream_t hs)
+{
+    constexpr int kFew = RT < 2 ? RT : 2, kMany = RT < 4 ? RT : 4, kOut = RT == 8 ? 2 : 4;
+    const bool many = plan.in.tokens == 64, fp8 = p.x_scale != nullptr;
+    p.rank_groups = (int)ceil_div(p.rank, 16 * (many ? kMany : kFew));
     p.pieces = (int)ceil_div(p.N, 256 * (int64_t)p.run);
-    if (8 * (ceil_div((int64_t)p.tiles * (p.pieces > p.splits ? p.pieces : p.splits), 8)) * p.sharers * 256 >= (int64_t(1) << 32))
-        return hipErrorInvalidConfiguration;   // (a launch has less than 2^32 threads)
-    auto grid = [&](int pieces) { return dim3((unsigned)(8 * ceil_div((int64_t)p.tiles * pieces, 8) * p.sharers)); };
-    const auto in = p.x_scale ? adapt_in_kernel<RT, T, true> : adapt_in_kernel<RT, T, false>;
-    const hipError_t err = launch(in, grid(p.splits), dim3(256), hs, p);
-    if (err != hipSuccess) return err;
-    return launch(adapt_out_kernel<RT, T>, grid(p.pieces), dim3(256), hs, p);
+    const auto in = many ? (fp8 ? adapt_in_kernel<kMany, 4, true> : adapt_in_kernel<kMany, 4, false>)
+                         : (fp8 ? adapt_in_kernel<kFew, 1, true> : adapt_in_kernel<kFew, 1, false>);
+    const auto out = plan.out.tokens == 16 ? adapt_out_kernel<RT, 1> : adapt_out_kernel<RT, kOut>;
+    const hipError_t err = launch_tiles(in, p, plan.in, (int64_t)p.splits * p.rank_groups, hs);
+    return err != hipSuccess ? err : launch_tiles(out, p, plan.out, p.pieces, hs);
 }
 
 bool sizes_fit(int M, int N, int K, int rank, int adapters)
@@ -429,14 +447,10 @@ extern "C" int alpha_moe_add_adapters(const uint16_t *base, const void *x, const
     p.base = base, p.a = a, p.b = b, p.x = static_cast<const uint8_t *>(x), p.x_scale = x_scale, p.scale = scale;
     p.ids = adapter_ids, p.out = out, p.part = static_cast<float *>(workspace);
     p.M = M, p.N = N, p.K = K, p.rank = rank, p.adapters = num_adapters, p.nkb = K / 128;
-    p.splits = plan.splits, p.sharers = plan.sharers;
-    const int64_t pieces = ceil_div(N, 256) * ceil_div(M, 16 * plan.T) / 1536;   // 256 columns of a tile
+    p.splits = plan.splits;
+    const int64_t pieces = ceil_div(N, 256) * ceil_div(M, plan.out.tokens) / 1536;   // 256 columns of a tile
     p.run = pieces < 1 ? 1 : pieces > 4 ? 4 : (int)pieces;
     hipStream_t hs = static_cast<hipStream_t>(stream);
-    const int T = plan.T;
-    const hipError_t err = rank <= 16   ? (T == 1 ? adapt<1, 1>(p, hs) : adapt<1, 4>(p, hs))
-                           : rank <= 32 ? (T == 1 ? adapt<2, 1>(p, hs) : adapt<2, 4>(p, hs))
-                           : rank <= 64 ? (T == 1 ? adapt<4, 1>(p, hs) : adapt<4, 4>(p, hs))
-                                        : (T == 1 ? adapt<8, 1>(p, hs) : adapt<8, 2>(p, hs));
+    const hipError_t err = rank <= 16 ? adapt<1>(p, plan, hs) : rank <= 32 ? adapt<2>(p, plan, hs) : rank <= 64 ? adapt<4>(p, plan, hs) : adapt<8>(p, plan, hs);
     return err == hipSuccess ? ALPHA_MOE_OK : err == hipErrorInvalidConfiguration ? ALPHA_MOE_ERR_SHAPE : ALPHA_MOE_ERR_LAUNCH;
 }

@@ -808,7 +808,25 @@ Plan grouped_plan(int M, int N, int K, int E)
     // kernel's wavefronts share: 32x16 / 128x64 8 experts, 25 rows, N = 142, K = 6528 8.7 / 22; 60 rows, N = 903, K = 1408 10.4 / 9.1.
     if (mean <= nkb && (M / 64 + (E < M ? E : M) / 2 + 1) * (int64_t)((N + 127) / 128) <= kUnits / 2) return kStream2x1;
     if (mean <= 8 && nkb >= 12) return kStream2x1;
-    return mean >= 12 * nkb ? kTile256x256 : mean <= 40 ? kTile128x64 : kTile256x128;
+    // The tile whose rounds over the compute units take the least time: what a tile takes beside its K blocks, and for each of them with
+    // tiles for half the units and with as many as run at a time (as plan() has them).
+    static const struct {
+        Plan plan;
+        int cols, tokens, resident;
+        float beside, half, full;
+    } kinds[] = {{kTile128x64, 128, 64, 2, 5.f, 0.38f, 0.67f}, {kTile256x128, 256, 128, 1, 7.f, 0.70f, 0.97f}, {kTile256x256, 256, 256, 1, 8.f, 1.36f, 1.80f}};
+    const int64_t used = E < M ? E : M;
+    Plan best = kTile128x64;
+    float least = 0.f;
+    for (const auto &k : kinds) {
+        int64_t token_tiles = M / k.tokens + used / 2;   // (every other expert has one more than its rows fill)
+        if (token_tiles < used) token_tiles = used;
+        const int64_t tiles = token_tiles * ((N + k.cols - 1) / k.cols), slots = kUnits * k.resident;
+        const float full = k.beside + nkb * k.full, half = k.beside + nkb * k.half;
+        const float time = tiles <= slots / 2 ? half : tiles <= slots ? full : (float)tiles / (float)slots * full;
+        if (k.plan == kTile128x64 || time < least) best = k.plan, least = time;
+    }
+    return best;
 }
 
 template <bool G>
