@@ -385,13 +385,16 @@ hipError_t launch(void (*kernel)(Args...), dim3 grid, dim3 block, hipStream_t st
     return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, list, 0, stream);
 }
 
-// A kernel with `each` times `sharers` workgroups to a tile.  A launch has less than 2^32 threads.
+// The workgroups of a kernel with `each` times `sharers` to a tile.
+int64_t workgroups(const AdaptParams &p, const AdaptPlan::Tiles &tiles, int64_t each)
+{
+    return 8 * ceil_div(ceil_div(p.M, tiles.tokens) * each, 8) * tiles.sharers;
+}
+
 hipError_t launch_tiles(void (*kernel)(AdaptParams), AdaptParams p, const AdaptPlan::Tiles &tiles, int64_t each, hipStream_t hs)
 {
     p.tiles = (int)ceil_div(p.M, tiles.tokens), p.sharers = tiles.sharers;
-    const int64_t groups = 8 * ceil_div(p.tiles * each, 8) * p.sharers;
-    if (groups * 256 >= (int64_t(1) << 32)) return hipErrorInvalidConfiguration;
-    return launch(kernel, dim3((unsigned)groups), dim3(256), hs, p);
+    return launch(kernel, dim3((unsigned)workgroups(p, tiles, each)), dim3(256), hs, p);
 }
 
 // Of many ranks, each workgroup of the first kernel takes a group: 32 of few tokens, whose parts are little work for many units (44 tokens,
@@ -406,7 +409,9 @@ hipError_t adapt(AdaptParams p, const AdaptPlan &plan, hipStream_t hs)
     const auto in = many ? (fp8 ? adapt_in_kernel<kMany, 4, true> : adapt_in_kernel<kMany, 4, false>)
                          : (fp8 ? adapt_in_kernel<kFew, 1, true> : adapt_in_kernel<kFew, 1, false>);
     const auto out = plan.out.tokens == 16 ? adapt_out_kernel<RT, 1> : adapt_out_kernel<RT, kOut>;
-    const hipError_t err = launch_tiles(in, p, plan.in, (int64_t)p.splits * p.rank_groups, hs);
+    const int64_t of_in = (int64_t)p.splits * p.rank_groups, most = (int64_t(1) << 32) / 256;
+    if (workgroups(p, plan.in, of_in) >= most || workgroups(p, plan.out, p.pieces) >= most) return hipErrorInvalidConfiguration;   // (a launch has less than 2^32 threads)
+    const hipError_t err = launch_tiles(in, p, plan.in, of_in, hs);
     return err != hipSuccess ? err : launch_tiles(out, p, plan.out, p.pieces, hs);
 }
 

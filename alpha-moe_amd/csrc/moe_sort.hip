@@ -14,8 +14,8 @@
 namespace alpha_moe {
 namespace {
 
-// 16 bytes of a row that starts at any multiple of A bytes (16, or 2: rows whose length is no multiple of 16; memory takes such
-// loads and stores as a whole).
+// 16 bytes of a row that starts at any multiple of A bytes (16, or 2: rows whose length is no multiple of 16, or a tensor that does not
+// start at one; memory takes such loads and stores as a whole).
 template <int A>
 struct Piece;
 template <>
@@ -482,7 +482,13 @@ int combine_rows_grad(const CombineParams &p, hipStream_t hs)
     return status(launch(kernel, dim3(p.M), dim3(threads), lds, hs, p));
 }
 
-bool aligned16(const void *a, const void *b) { return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0; }
+// The largest power of two up to 16 that rows of `row_bytes` bytes of all these tensors start at multiples of.
+template <typename... Ptr>
+int alignment(int64_t row_bytes, Ptr... tensors)
+{
+    const uintptr_t all = (uintptr_t)row_bytes | (reinterpret_cast<uintptr_t>(tensors) | ...) | 16;
+    return (int)(all & (~all + 1));
+}
 
 // Sizes that all calls share: M tokens of top_k slots, rows of K values of 1, 2 or 4 bytes.  A launch has less than 2^32 threads and
 // a row at most 65535 pieces of 4 KiB.
@@ -513,7 +519,8 @@ extern "C" int alpha_moe_sort_tokens(const void *x, int value_bytes, const float
         return ALPHA_MOE_ERR_SHAPE;
     if (!offsets || (M > 0 && (!x || !topk_ids || !rows || !row_of_slot)) || (!x_scale) != (!scale)) return ALPHA_MOE_ERR_NULL_POINTER;
     if (x_scale && value_bytes != 1) return ALPHA_MOE_ERR_SHAPE;
-    if (!aligned16(x, rows)) return ALPHA_MOE_ERR_ALIGNMENT;
+    const int starts = alignment((int64_t)K * value_bytes, x, rows);
+    if (starts < (value_bytes == 1 ? 16 : value_bytes)) return ALPHA_MOE_ERR_ALIGNMENT;
     SortParams p = {};
     p.x = static_cast<const uint8_t *>(x), p.x_scale = x_scale, p.ids = topk_ids;
     p.rows = static_cast<uint8_t *>(rows), p.scale = scale, p.offsets = offsets, p.row_of_slot = row_of_slot;
@@ -528,7 +535,7 @@ extern "C" int alpha_moe_sort_tokens(const void *x, int value_bytes, const float
     int id_bits = 0;
     while ((1 << id_bits) < num_experts + 1) id_bits++;
     hipStream_t hs = static_cast<hipStream_t>(stream);
-    return p.row_bytes % 16 == 0 ? sort_rows<16>(p, id_bits, hs) : sort_rows<2>(p, id_bits, hs);
+    return starts == 16 ? sort_rows<16>(p, id_bits, hs) : sort_rows<2>(p, id_bits, hs);
 }
 
 extern "C" int alpha_moe_combine_tokens(const void *rows, int is_f32, const int32_t *row_of_slot, const float *topk_weights, void *out,
@@ -538,13 +545,14 @@ extern "C" int alpha_moe_combine_tokens(const void *rows, int is_f32, const int3
     if (!sizes_fit(M, top_k, K, size)) return ALPHA_MOE_ERR_SHAPE;
     if (M == 0) return ALPHA_MOE_OK;
     if (!rows || !row_of_slot || !out) return ALPHA_MOE_ERR_NULL_POINTER;
-    if (!aligned16(rows, out)) return ALPHA_MOE_ERR_ALIGNMENT;
+    const int starts = alignment((int64_t)K * size, rows, out);
+    if (starts < size) return ALPHA_MOE_ERR_ALIGNMENT;
     CombineParams p = {};
     p.rows = static_cast<const uint8_t *>(rows), p.map = row_of_slot, p.weights = topk_weights, p.out = static_cast<uint8_t *>(out);
     p.row_bytes = (int64_t)K * size, p.numel = (int64_t)M * top_k, p.pieces = (int)((p.row_bytes + 15) / 16);
     p.scaling = scaling_factor, p.M = M, p.top_k = top_k;
     hipStream_t hs = static_cast<hipStream_t>(stream);
-    const bool whole = p.row_bytes % 16 == 0;
+    const bool whole = starts == 16;
     if (is_f32) return whole ? combine_rows<float, 16>(p, hs) : combine_rows<float, 2>(p, hs);
     return whole ? combine_rows<uint16_t, 16>(p, hs) : combine_rows<uint16_t, 2>(p, hs);
 }
@@ -557,14 +565,15 @@ extern "C" int alpha_moe_combine_tokens_grad(const void *grad, const void *rows,
     if (!sizes_fit(M, top_k, K, size)) return ALPHA_MOE_ERR_SHAPE;
     if (M == 0 || (!grad_rows && !grad_weights)) return ALPHA_MOE_OK;
     if (!grad || !row_of_slot || (grad_weights && !rows)) return ALPHA_MOE_ERR_NULL_POINTER;
-    if (!aligned16(rows, grad) || !aligned16(grad_rows, nullptr)) return ALPHA_MOE_ERR_ALIGNMENT;
+    const int starts = alignment((int64_t)K * size, rows, grad, grad_rows);
+    if (starts < size) return ALPHA_MOE_ERR_ALIGNMENT;
     CombineParams p = {};
     p.rows = static_cast<const uint8_t *>(rows), p.grad = static_cast<const uint8_t *>(grad), p.map = row_of_slot;
     p.weights = topk_weights, p.out = static_cast<uint8_t *>(grad_rows), p.grad_weights = grad_weights;
     p.row_bytes = (int64_t)K * size, p.numel = (int64_t)M * top_k, p.pieces = (int)((p.row_bytes + 15) / 16);
     p.scaling = scaling_factor, p.M = M, p.top_k = top_k;
     hipStream_t hs = static_cast<hipStream_t>(stream);
-    const bool whole = p.row_bytes % 16 == 0;
+    const bool whole = starts == 16;
     if (is_f32) return whole ? combine_rows_grad<float, 16>(p, hs) : combine_rows_grad<float, 2>(p, hs);
     return whole ? combine_rows_grad<uint16_t, 16>(p, hs) : combine_rows_grad<uint16_t, 2>(p, hs);
 }

@@ -283,7 +283,8 @@ int alpha_moe_route_topk(const void *logits, int is_f32, const float *bias, floa
                          float shared_weight, void *stream /* hipStream_t */);
 
 /*
- * Tokens sorted by expert and back.  Slot t * top_k + s is expert topk_ids[t, s] of token t, top_k <= 64, num_experts <= 4096.
+ * Tokens sorted by expert and back.  Slot t * top_k + s is expert topk_ids[t, s] of token t, top_k <= 64, num_experts <= 4096.  Tensors of
+ * values of 2 or 4 bytes may start at any multiple of those.
  *
  * alpha_moe_sort_tokens: x [M, K] of values of value_bytes bytes (1: FP8 codes, K % 128 == 0, with x_scale [M, K/128] or NULL; 2; 4) ->
  *   rows [M * top_k, K]  the tokens of the slots, by ascending expert, equal experts by ascending slot; behind them a row of zeros for each

@@ -177,3 +177,23 @@ def test_replays_and_streams():
     torch.cuda.synchronize()
     want = [layer_hip.add_adapters(**q) for q in others]
     assert all(torch.equal(t, want[i % 2]) for i, t in enumerate(got))
+
+
+def test_offsets_past_32_bits():
+    """adapters of more than 4 GiB each way"""
+    L_, rank, K, N, M = 300, 128, 65536, 70000, 9
+    a = torch.zeros((L_, rank, K), dtype=BF, device=DEV)
+    b = torch.zeros((L_, N, rank), dtype=BF, device=DEV)
+    assert a.numel() * 2 > 2 ** 32 and b.numel() * 2 > 2 ** 32
+    ids = torch.tensor([299, 0, 298, 299, 150, -1, 299, 298, 0], dtype=torch.int32)
+    for l in set(ids.tolist()) - {-1}:
+        a[l, l % rank, K - 1], b[l, N - 1, l % rank], b[l, 5, l % rank] = 2.0, 3.0, float(l % 7)
+    x = torch.zeros((M, K), dtype=BF, device=DEV)
+    x[:, K - 1] = torch.arange(1, M + 1).to(BF).to(DEV)
+    base = torch.ones((M, N), dtype=BF, device=DEV)
+    got = layer_hip.add_adapters(base, x, a, b, ids.to(DEV)).cpu()
+    for m, l in enumerate(ids.tolist()):
+        want = torch.ones(N)
+        if l >= 0:
+            want[N - 1], want[5] = 1 + 6.0 * (m + 1), 1 + 2.0 * (m + 1) * (l % 7)
+        assert torch.equal(got[m].float(), want), m

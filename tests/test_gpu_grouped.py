@@ -162,3 +162,31 @@ def test_last_tiles_of_any_length(rest):
     counts = [256 * k + rest for k in (0, 1, 3)] + [0, 700, 40]
     args = problem(counts, 5, 300, 256, rest)
     check(*args, run(*args))
+
+
+def test_offsets_past_32_bits():
+    """weights of more than 4 GiB and results of more than 4 GiB: small integers, exact"""
+    E, N, K = 130, 4096, 8192 + 128
+    w = torch.zeros((E, N, K), device=DEV, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    assert w.numel() > 2 ** 32
+    for e in (0, 100, 129):
+        w.view(torch.uint8)[e, N - 3, K - 2] = torch.tensor([2.0]).to(torch.float8_e4m3fn).view(torch.uint8).item()
+    counts = torch.zeros(E, dtype=torch.int64)
+    counts[0], counts[100], counts[129] = 3, 20, 2
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), counts.cumsum(0)]).to(torch.int32).to(DEV)
+    x = torch.ones((25, K), device=DEV).to(torch.float8_e4m3fn)
+    out = layer_hip.grouped_block_scaled_mm(x, torch.ones((25, K // 128), device=DEV), offsets, w, torch.ones((E, N // 128, K // 128), device=DEV))
+    want = torch.zeros((25, N))
+    want[:, N - 3] = 2.0
+    assert torch.equal(out.cpu().float(), want)
+    del w, out
+    R, N, K = 40000, 65536, 128                      # (5 GiB of results)
+    x = torch.ones((R, K), device=DEV).to(torch.float8_e4m3fn)
+    w = torch.zeros((2, N, K), device=DEV).to(torch.float8_e4m3fn)
+    w[1, N - 1, 7] = 3.0
+    out = layer_hip.grouped_block_scaled_mm(x, torch.ones((R, 1), device=DEV), torch.tensor([0, 17, R - 2], dtype=torch.int32, device=DEV), w,
+                                            torch.ones((2, N // 128, 1), device=DEV))
+    assert out.numel() * 2 > 2 ** 32
+    last = out[:, N - 1]
+    assert bool((last[17:R - 2] == 3).all()) and not bool(last[:17].any()) and not bool(last[R - 2:].any())
+    assert int(out[-5000:].count_nonzero()) == 4998

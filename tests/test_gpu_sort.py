@@ -304,6 +304,65 @@ def test_views_and_expanded_gradients():
         layer_hip.combine_tokens(s.rows.detach(), s.row_of_slot.t().contiguous().t())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("K", [7, 64, 333])
+def test_tensors_that_start_anywhere(dtype, K):
+    """parts of larger tensors, as gradients of concatenated results are: any multiple of a value's size"""
+    M, top_k, E = 9, 3, 5
+    ids = make_ids(M, top_k, E, "some", 3)
+    _, _, at = L.sort_slots(ids, E)
+    part = lambda t: torch.cat([t.flatten()[:1], t.flatten()]).to(DEV)[1:].view(t.shape)
+    x, rows, g, w = make_rows(M, K, dtype, 1), make_rows(M * top_k, K, dtype, 2), make_rows(M, K, dtype, 3), torch.rand((M, top_k))
+    assert part(x).data_ptr() % 16 != 0
+    a, b = (layer_hip.sort_tokens(t, ids.to(DEV), E) for t in (part(x), x.to(DEV)))
+    assert torch.equal(a.rows, b.rows)
+    xd = x.to(DEV).requires_grad_()
+    s = layer_hip.sort_tokens(xd, ids.to(DEV), E)
+    both = torch.cat([s.rows[:0], torch.ones((1, K), dtype=dtype, device=DEV), s.rows])          # (its gradient is a part that starts behind a row)
+    want = L.combine_tokens(rows, at)[0]
+    got = torch.autograd.grad(both, xd, torch.cat([rows[:1], rows]).to(DEV))[0]
+    assert_within(got, want, half_step(dtype) * want.abs() + 8 * U * L.combine_tokens(rows, at)[1], "gradient of the tokens")
+    for r, gg in ((part(rows), g.to(DEV)), (rows.to(DEV), part(g)), (part(rows), part(g))):
+        rd, wd = r.requires_grad_(), w.to(DEV).requires_grad_()
+        got = torch.autograd.grad(layer_hip.combine_tokens(rd, at.to(DEV), wd), (rd, wd), gg)
+        rp, wp = rows.to(DEV).requires_grad_(), w.to(DEV).requires_grad_()
+        want = torch.autograd.grad(layer_hip.combine_tokens(rp, at.to(DEV), wp), (rp, wp), g.to(DEV))
+        assert torch.equal(got[0], want[0])
+        assert_within(got[1], want[1].cpu().double(), (K / 32 + 48) * U * L.combine_tokens_grad(g, rows, at, w)[2], "gradient of the weights")
+
+
+def test_offsets_past_32_bits():
+    """rows of more than 4 GiB, there and back"""
+    M, top_k, E, K = 6000, 8, 40, 57344
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn((M, K), generator=g, device=DEV, dtype=torch.bfloat16)
+    ids = torch.randint(0, E, (M, top_k), generator=g, device=DEV, dtype=torch.int32)
+    s = layer_hip.sort_tokens(x, ids, E)
+    order = torch.sort(ids.flatten(), stable=True)[1]
+    for lo in (0, 20000, M * top_k - 300):           # (also behind 4 GiB: row 37450 and on)
+        assert torch.equal(s.rows[lo:lo + 300], x[order[lo:lo + 300] // top_k])
+    assert s.rows.numel() * 2 > 2 ** 32
+    out = layer_hip.combine_tokens(s.rows, s.row_of_slot, None, 1 / top_k)
+    assert torch.equal(out, x)                       # (the mean of eight equal values: sums of three bits more are exact in fp32)
+    rows = s.rows.requires_grad_()
+    got = torch.autograd.grad(layer_hip.combine_tokens(rows, s.row_of_slot), rows, x)[0]
+    assert torch.equal(got[-200:], x[order[-200:] // top_k]) and torch.equal(got[:200], x[order[:200] // top_k])
+
+
+def test_operators_trace_with_their_gradients():
+    """schemas, fake implementations and the registration of the gradients, as torch's own checks see them"""
+    M, top_k, E, K = 5, 3, 4, 12
+    ids = make_ids(M, top_k, E, "some", 3).to(DEV)
+    x = torch.randn((M, K), device=DEV, requires_grad=True)
+    at = layer_hip.sort_tokens(x.detach(), ids, E).row_of_slot
+    rows, w = torch.randn((M * top_k, K), device=DEV, requires_grad=True), torch.rand((M, top_k), device=DEV, requires_grad=True)
+    import alpha_moe_ops  # noqa: F401  (fake implementations)
+    O = torch.ops.alpha_moe
+    torch.library.opcheck(O.sort_tokens.default, (x, ids, E))
+    torch.library.opcheck(O.combine_tokens.default, (rows, at, w, 0.5))
+    torch.library.opcheck(O.combine_tokens.default, (rows, at, None, 1.0))
+
+
 def test_refusals():
     x, ids = torch.zeros((4, 128), device=DEV), torch.zeros((4, 2), dtype=torch.int32, device=DEV)
     rows, at, w = torch.zeros((8, 128), device=DEV), torch.zeros((4, 2), dtype=torch.int32, device=DEV), torch.ones((4, 2), device=DEV)
@@ -318,7 +377,7 @@ def test_refusals():
             (lambda: H.sort_tokens(x, torch.zeros((4, 0), dtype=torch.int32, device=DEV), 4), "top_k"),
             (lambda: H.sort_tokens(x, ids, 4, x_scale=sc), "goes with codes"), (lambda: H.sort_tokens(q, ids, 4, x_scale=sc[:3]), "x_scale"),
             (lambda: H.sort_tokens(q[:, :64].contiguous(), ids, 4), "128"), (lambda: H.sort_tokens(q, ids, 4, x_scale=sc.half()), "dtype"),
-            (lambda: H.sort_tokens(torch.zeros((4 * 128 + 1,), device=DEV)[1:].view(4, 128), ids, 4), "multiple of 16"),
+            (lambda: H.sort_tokens(torch.zeros((4 * 128 + 8,), device=DEV).to(FP8)[8:].view(4, 128), ids, 4), "multiple of 16"),
             (lambda: H.combine_tokens(rows.half(), at), "bfloat16 or float32"), (lambda: H.combine_tokens(rows[:7], at), "one row for each"),
             (lambda: H.combine_tokens(rows, at, w[:, :1]), "contiguous"), (lambda: H.combine_tokens(rows, at, w[:3]), "shape"), (lambda: H.combine_tokens(rows, at, w.bfloat16()), "dtype"),
             (lambda: H.combine_tokens(rows, at.long()), "dtype"), (lambda: H.combine_tokens(rows, at, w.cpu()), "must be on"),

@@ -24,7 +24,7 @@ def test_sort_refusals():
     for name in ("x", "ids", "rows", "offsets", "row_of_slot"):
         assert sort(**{name: None}) == NULL, name
     assert sort(size=1, K=128, scale_in=4096) == NULL and sort(size=1, K=128, scale=4096) == NULL      # both or neither
-    assert sort(x=4104) == ALIGN and sort(rows=4098) == ALIGN
+    assert sort(x=4097) == ALIGN and sort(rows=4099) == ALIGN and sort(size=4, x=4098) == ALIGN and sort(size=1, K=128, x=4104) == ALIGN
     big = dict(M=40000, top_k=8, E=256)
     need = A.alpha_moe_sort_workspace_bytes(40000, 8, 256)
     assert need > 0 and sort(**big) == WORKSPACE and sort(**big, ws=4096, nws=need - 1) == WORKSPACE and sort(**big, nws=need) == WORKSPACE
@@ -38,7 +38,7 @@ def test_combine_refusals():
     assert call(M=0) == OK and call(M=-1) == SHAPE and call(K=0) == SHAPE and call(top_k=0) == SHAPE and call(top_k=65) == SHAPE
     assert call(M=2 ** 24) == SHAPE and call(K=2 ** 26 + 1) == SHAPE
     assert call(rows=None) == NULL and call(at=None) == NULL and call(out=None) == NULL
-    assert call(rows=4104) == ALIGN and call(out=4104) == ALIGN
+    assert call(rows=4097) == ALIGN and call(out=4103) == ALIGN
 
     def grad(g=4096, rows=4096, at=4096, weights=4096, grad_rows=4096, grad_weights=4096, M=4, K=8, top_k=2):
         return A.alpha_moe_combine_tokens_grad(g, rows, 0, at, weights, grad_rows, grad_weights, M, K, top_k, 1.0, None)
@@ -46,7 +46,7 @@ def test_combine_refusals():
     assert grad(M=-1) == SHAPE and grad(K=0) == SHAPE and grad(top_k=65) == SHAPE
     assert grad(g=None) == NULL and grad(at=None) == NULL and grad(rows=None) == NULL
     for name in ("g", "rows", "grad_rows"):
-        assert grad(**{name: 4104}) == ALIGN, name
+        assert grad(**{name: 4097}) == ALIGN, name
 
 
 def meta(shape, dtype=torch.float32):
