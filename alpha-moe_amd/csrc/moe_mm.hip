@@ -141,10 +141,10 @@ __device__ __forceinline__ int wave_scan(int v)   // inclusive sums over the wav
 }
 
 // The tile of this workgroup, if there is one.  How many there are, only the device knows: each wavefront counts the experts' tiles,
-// 256 experts' offsets in flight at a time, and looks for its own.  (A run of experts to a lane, one offset behind the other, took some
-// 0.3 us more of every workgroup.)  An expert's tiles follow each other, its tiles of tokens in groups of HIGH (0: all of them) next to each
-// other; each XCD gets a run of tiles.  HALVES: an expert's last tile may be a half one, and those come behind all whole ones, so that
-// what is left at the end is short.  Offsets are taken into [0, M], and where they do not ascend then, nobody has a tile.
+// 256 experts' offsets in flight at a time, and looks for its own.  (A run of experts to a lane, one offset behind the other, took
+// some 0.3 us more of every workgroup.)  An expert's tiles follow each other, its tiles of tokens in groups of HIGH (0: all of them)
+// next to each other; each XCD gets a run of tiles.  HALVES: an expert's last tile may be a half one, and those come behind all whole
+// ones, so that what is left at the end is short.  Offsets are taken into [0, M], and where they do not ascend then, nobody has a tile.
 template <int COLS, int TOKENS, int HIGH, bool HALVES>
 __device__ __forceinline__ bool find_tile(const MmParams &p, GroupTile &g)
 {
@@ -195,7 +195,7 @@ __device__ __forceinline__ bool find_tile(const MmParams &p, GroupTile &g)
     if (g.half || at < of_experts) {
         before = 0;
         bool found = false;
-        for (int base = 0; !found; base += 64 * Q) {
+        for (int base = 0; base < p.E && !found; base += 64 * Q) {
             if (p.E > 64 * Q) load(base);   // (otherwise they are all there)
 #pragma unroll
             for (int j = 0; j < Q; j++) {
@@ -212,6 +212,7 @@ __device__ __forceinline__ bool find_tile(const MmParams &p, GroupTile &g)
                 if (!found) before += all;
             }
         }
+        if (!found) return false;   // (offsets that somebody has written meanwhile)
     }
     const int inside = tile - before * p.row_groups;
     if (g.half) {

@@ -143,3 +143,37 @@ def test_a_training_step_on_sorted_tokens():
     assert_within(out, want_out, torch.full_like(want_out, 1e-4 * want_out.abs().max().item()), "output")
     for a, b, name in zip(got, want, ("tokens", "experts' weights", "router's weights")):
         assert_within(a, b, torch.full_like(b, 1e-4 * b.abs().max().item()), name)
+
+
+def test_layers_without_tokens():
+    """a batch of nothing: results of no rows, gradients of zeros"""
+    K, I, E, top_k, L_ = 512, 128, 4, 2, 3
+    norm, gate, w13, w2, s13, s2 = (t.to(DEV) for t in layer(E, K, I, E, 3))
+    nothing = torch.empty((0, K), dtype=torch.bfloat16, device=DEV)
+    for t in norm_sorted_moe(nothing, nothing, norm, gate, w13, w2, s13, s2, top_k):
+        assert t.shape == (0, K) and t.dtype == torch.bfloat16
+    low = lambda *shape: torch.zeros(shape, dtype=torch.bfloat16, device=DEV)
+    ad = Adapters(low(L_, 8, K), low(L_, 2 * I, 8), low(L_, 8, I), low(L_, K, 8), torch.empty(0, dtype=torch.int32, device=DEV))
+    for t in norm_dense_mlp(nothing, nothing, norm, w13[0].contiguous(), w2[0].contiguous(), s13[0].contiguous(), s2[0].contiguous(), adapters=ad):
+        assert t.shape == (0, K) and t.dtype == torch.bfloat16
+    x = nothing.clone().requires_grad_()
+    w = torch.empty((0, top_k), device=DEV, requires_grad=True)
+    s = layer_hip.sort_tokens(x, torch.empty((0, top_k), dtype=torch.int32, device=DEV), E)
+    assert s.offsets.tolist() == [0] * (E + 1)
+    gx, gw = torch.autograd.grad(layer_hip.combine_tokens(s.rows, s.row_of_slot, w).sum(), (x, w))
+    assert gx.shape == (0, K) and gw.shape == (0, top_k)
+
+
+def test_more_experts_than_offsets_in_flight():
+    """above 256 experts their offsets are looked through twice: every expert's rows, the last one's and those behind it"""
+    E, K, N = 700, 128, 128
+    g = torch.Generator().manual_seed(11)
+    w, ws = block_quant_fp8(torch.randn((E, N, K), generator=g))
+    for mean in (1, 40):
+        ids = torch.randint(-1, E, (mean * E // 2, 2), generator=g, dtype=torch.int32)
+        ids[0, 0] = E - 1
+        x = torch.randn((ids.shape[0], K), generator=g).to(DEV)
+        q = layer_hip.rms_norm_quant_fp8(x, torch.ones(K, device=DEV))
+        s = layer_hip.sort_tokens(q.q, ids.to(DEV), E, x_scale=q.scale)
+        out = layer_hip.grouped_block_scaled_mm(s.rows, s.scale, s.offsets, w.to(DEV), ws.to(DEV))
+        check_grouped(s.rows.cpu(), s.scale.cpu(), s.offsets.cpu(), w, ws, out)
