@@ -1,8 +1,9 @@
 """``import alpha_moe`` registers ``torch.ops.alpha_moe.fused_moe_w8a8_up_down`` (as the reference's extension
 module of the same name does, csrc/torch_interface.cpp:105-131) by loading the in-tree HIP libraries, together with
 the two input-preparation operators ``per_token_group_quant_fp8`` and ``moe_align_block_size`` and the operators that run
-around a layer call: ``rms_norm_quant_fp8``, ``add_rms_norm_quant_fp8``, ``swiglu_quant_fp8``, ``block_scaled_mm`` and
-``route_topk`` (``alpha_moe_python.layer_hip`` is their front).
+around a layer call: ``rms_norm_quant_fp8``, ``add_rms_norm_quant_fp8``, ``swiglu_quant_fp8``, ``block_scaled_mm``,
+``route_topk``, ``sort_tokens``, ``combine_tokens``, ``grouped_block_scaled_mm`` and ``add_adapters``
+(``alpha_moe_python.layer_hip`` is their front).
 
 There is no fallback: if the libraries are not built the import fails.
 """

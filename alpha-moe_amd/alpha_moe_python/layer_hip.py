@@ -1,14 +1,19 @@
-"""The operators around the fused experts: what a decoder layer runs in front of ``fused_moe_w8a8_up_down``, and the FP8
-products of its dense layers.  Callers of the reference take these from their serving engine.
+"""The operators around the fused experts: what a decoder layer runs in front of ``fused_moe_w8a8_up_down``, the FP8 products of
+its dense layers, and what brings tokens to weights of their own outside the fused call.  Callers of the reference take these from their serving engine.
 
 * :func:`rms_norm_quant_fp8` - residual addition, RMS norm and per-token-group FP8 quantisation in one kernel;
 * :func:`route_topk`         - the router's selection, in the form ``moe_align_block_size`` and the fused operator take;
 * :func:`block_scaled_mm`    - FP8 matrix product with the layer's scales (1 x 128 for tokens, 128 x 128 for weights);
-* :func:`swiglu_quant_fp8`   - SwiGLU and quantisation between the two products of a dense layer.
+* :func:`swiglu_quant_fp8`   - SwiGLU and quantisation between the two products of a dense layer;
+* :func:`sort_tokens`, :func:`combine_tokens` - the tokens of all routing slots sorted by expert, and their weighted sums back;
+* :func:`grouped_block_scaled_mm` - the block-scaled product of sorted tokens with each expert's weights;
+* :func:`add_adapters`       - low-rank adapters of many requests beside a shared projection.
 
 HIP kernels on the current stream of the inputs' device; nothing is kept between calls, so they may be captured into HIP graphs
-and run on several streams at once.  Inputs are contiguous.  Inference only: inputs that require gradients are refused while
-gradients are recorded, and inputs that carry a forward-mode tangent wherever tangents are, in a trace too.
+and run on several streams at once.  Inputs are contiguous.  :func:`sort_tokens` and :func:`combine_tokens` are differentiable (once:
+what has no second derivative says so), capture forward and backward pass together, and hold no eager graph of the same
+leaves while a backward pass is captured.  The others are for inference only: inputs that require gradients are refused while gradients
+are recorded, and inputs that carry a forward-mode tangent wherever tangents are, by all of them, in a trace too.
 """
 from typing import NamedTuple, Optional, Tuple
 

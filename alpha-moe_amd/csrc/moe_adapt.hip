@@ -12,6 +12,11 @@
 // their own column alone, so a tile is multiplied as a whole and what belongs to other adapters is not stored: nothing of
 // them, NaN or infinity, reaches a token.
 //
+// What bounds it: of many tokens memory, x once, base and result once each (8192 tokens, K = 2048, N = 7168, rank 64: 271 MB, 53 us at a
+// copy's rate; MI355X 20 us the first kernel and 65 the second, whose b is read again by every tile out of the L2); of few tokens two launches,
+// each one chain of loads and a sum over wavefronts (1 token 4.1 and 3.6 us, 61 tokens of 48 adapters 8.1 and 4.8).  One kernel for
+// both would have every column's workgroup contract all of K again, or wait for the others.
+//
 // Operands as in moe_common.hpp: adapters' rows are A, tokens B, results (row 4q + j, token n) in register j of lane (n, q).
 #include "moe_common.hpp"
 
@@ -40,8 +45,8 @@ __device__ __forceinline__ void lds_order()
     asm volatile("" ::: "memory");
 }
 
-// Workgroups are dealt to the eight XCDs in turn: each gets a run of tiles, so that an adapter's a and b are read into few of their L2s
-//.  A tile's workgroups: `pieces` times `sharers`.
+// Workgroups are dealt to the eight XCDs in turn: each gets a run of tiles, so that an adapter's a and b are read into few of their
+// L2s.  A tile's workgroups: `pieces` times `sharers`.
 struct Place {
     int tile, piece, turn;
 };
@@ -97,8 +102,9 @@ __device__ __forceinline__ void widen(v4i codes, v8bf (&to)[2])
     to[1] = __builtin_bit_cast(v8bf, half[1]);
 }
 
-// part[split][token][rank]: RT tiles of 16 ranks of p.rank_groups times as many, T tiles of 16 tokens; the four wavefronts take the split's K
-// blocks in turn.
+// part[split][token][rank]: RT tiles of 16 ranks of p.rank_groups times as many, T tiles of 16 tokens; the four wavefronts take the
+// split's K blocks in turn, operands straight from memory: each value of x is used by one wavefront only, and an adapter's a comes out of
+// the L2 (staged through LDS for all four it was no faster).
 template <int RT, int T, bool FP8>
 __global__ __launch_bounds__(256, 2) void adapt_in_kernel(const AdaptParams p)
 {
@@ -170,7 +176,7 @@ __global__ __launch_bounds__(256, 2) void adapt_in_kernel(const AdaptParams p)
     });
 }
 
-// out: each wavefront 64 columns of T tiles of 16 tokens.  Up to 16 ranks (RT = 1) their high and low parts lie behind each other in one
+// out: each wavefront 64 columns of T tiles of 16 tokens, whose b values stay in registers over the tiles.  Up to 16 ranks (RT = 1) their high and low parts lie behind each other in one
 // matrix instruction, and b's values twice; beyond, b's values of 32 ranks are multiplied with both.
 template <int RT, int T>
 __global__ __launch_bounds__(256, RT == 8 ? 3 : 4) void adapt_out_kernel(const AdaptParams p)
@@ -226,7 +232,8 @@ __global__ __launch_bounds__(256, RT == 8 ? 3 : 4) void adapt_out_kernel(const A
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 if (c0 + col + i < p.N)
-                    p.out[from + i] = (uint16_t)pack_bf16x2(__builtin_bit_cast(float, (uint32_t)p.base[from + i] << 16) + (i < 4 ? lo[h][i % 4] : hi[h][i % 4]), 0.f);
+                    p.out[from + i] = (uint16_t)pack_bf16x2(
+                        __builtin_bit_cast(float, (uint32_t)p.base[from + i] << 16) + (i < 4 ? lo[h][i % 4] : hi[h][i % 4]), 0.f);
         }
     };
     const unsigned long long with = __ballot((unsigned)id < (unsigned)p.adapters);
@@ -265,7 +272,8 @@ __global__ __launch_bounds__(256, RT == 8 ? 3 : 4) void adapt_out_kernel(const A
             for (int s = 0; s < S; s++)
 #pragma unroll
                 for (int k = 0; k < 4; k++)
-                    bv.v[s][k] = __builtin_bit_cast(v8bf, __builtin_amdgcn_raw_buffer_load_b128(from, (int)(b_at[s] + 32u * (uint32_t)(k * rank)), 0, 0));
+                    bv.v[s][k] = __builtin_bit_cast(
+                        v8bf, __builtin_amdgcn_raw_buffer_load_b128(from, (int)(b_at[s] + 32u * (uint32_t)(k * rank)), 0, 0));
         };
         Weights bv;
         load_weights(c_begin, bv);   // (in front of the parts' loads)
@@ -410,7 +418,8 @@ hipError_t adapt(AdaptParams p, const AdaptPlan &plan, hipStream_t hs)
                          : (fp8 ? adapt_in_kernel<kFew, 1, true> : adapt_in_kernel<kFew, 1, false>);
     const auto out = plan.out.tokens == 16 ? adapt_out_kernel<RT, 1> : adapt_out_kernel<RT, kOut>;
     const int64_t of_in = (int64_t)p.splits * p.rank_groups, most = (int64_t(1) << 32) / 256;
-    if (workgroups(p, plan.in, of_in) >= most || workgroups(p, plan.out, p.pieces) >= most) return hipErrorInvalidConfiguration;   // (a launch has less than 2^32 threads)
+    if (workgroups(p, plan.in, of_in) >= most || workgroups(p, plan.out, p.pieces) >= most)
+        return hipErrorInvalidConfiguration;   // (a launch has less than 2^32 threads)
     const hipError_t err = launch_tiles(in, p, plan.in, of_in, hs);
     return err != hipSuccess ? err : launch_tiles(out, p, plan.out, p.pieces, hs);
 }

@@ -9,6 +9,12 @@
 //
 // Sums are taken in fp32, slots in ascending order, and rounded once; there are no atomics on results.  What is negative in the map
 // takes no part: neither its row nor its weight is looked at.  An index of a row is checked against the rows before it is used.
+//
+// All of it is memory traffic: a row is read once and written once for each slot, in pieces of 16 bytes a thread, a token's row in registers
+// while it goes to all its slots.  MI355X: 8192 tokens of 7168 codes to 8 rows each 103 us, 93 of them the copies (545 MB, 5.9 TB/s; a copy
+// of 1 GiB runs at 5.1); sums of 4096 x 8 rows of 2048 bf16 24 us (151 MB, 6.2 TB/s, part of it out of the last-level cache), their backward
+// pass 55 (285 MB, 5.2).  What is left of small calls is the launch and one chain of dependent loads: 7.3 us for a token's 9 slots, 5.3 for
+// the sums of 61 tokens, of 2.2 for an empty kernel.
 #include "moe_count.hpp"
 
 namespace alpha_moe {
@@ -101,8 +107,9 @@ __device__ __forceinline__ void spread(const SortParams &p, int t, int v0, int s
 
 __device__ __forceinline__ int bucket(int id, int E) { return (unsigned)id < (unsigned)E ? id : E; }
 
-// Few slots, in one launch: a workgroup to a token (and 16 KiB of its row) finds its slots' rows by itself - a slot's row is the number of slots
-// in front of it, by (expert, slot) - and one more workgroup counts the experts.
+// Few slots, in one launch: a workgroup to a token (and 16 KiB of its row) finds its slots' rows by itself - a slot's row is the number
+// of slots in front of it, by (expert, slot) - and one more workgroup counts the experts.  Its row is on the way meanwhile.
+// MI355X: 9 slots 5.0 us, three launches 11.5.
 constexpr int kSortMaxExperts = 4096, kMaxTopK = 64;
 template <int A>
 __global__ __launch_bounds__(256) void sort_few_kernel(const SortParams p)
@@ -166,7 +173,7 @@ __global__ __launch_bounds__(256) void sort_few_kernel(const SortParams p)
     spread<A, 4>(p, t, part * 1024 + tid, 256, piece, part == 0 ? tid : p.scale_cols, 256, at);
 }
 
-// Many slots: histograms of segments, places, copies.
+// Many slots: histograms of segments, places, copies.  65536 slots: 5.0, 5.5 and, of 7168 codes, 93 us.
 __global__ __launch_bounds__(256) void sort_hist_kernel(const SortParams p, int words, int seg)
 {
     extern __shared__ int counts[];   // [words], 16 bits each
@@ -181,7 +188,9 @@ __global__ __launch_bounds__(256) void sort_hist_kernel(const SortParams p, int 
     for (int i = threadIdx.x; i < words; i += 256) p.hist[(size_t)blockIdx.x * words + i] = counts[i];
 }
 
-// One workgroup to a segment: it adds up the segments' histograms, all of them and those in front of its own, and places its slots.
+// One workgroup to a segment: it adds up the segments' histograms, all of them and those in front of its own, and places its slots (as the
+// aligner does, so that equal experts stay in order without a sort of keys).  Adding them up in every workgroup instead of in a launch
+// of its own saves a launch for n_seg * words * 4 bytes more from the L2.
 template <bool FEW>
 __global__ __launch_bounds__(1024) void sort_place_kernel(const SortParams p, int words, int seg, int id_bits, int n_waves)
 {
@@ -233,6 +242,9 @@ __global__ __launch_bounds__(1024) void sort_place_kernel(const SortParams p, in
         for (int e = threadIdx.x; e < buckets; e += blockDim.x) p.offsets[e] = start[e];
 }
 
+// A token's row to its slots' rows: U pieces a thread, which are read before the map's entries are there.  Rows shorter than a workgroup
+// share one; with ONE token to a workgroup its entries come by scalar loads (8192 tokens of 7168 codes 125 us before, 104 with it and
+// the stores above).
 template <int A, int U, bool ONE>
 __global__ __launch_bounds__(256) void spread_kernel(const SortParams p)
 {
@@ -285,7 +297,7 @@ struct Values<float> {
     }
 };
 
-// A thread to 16 bytes of a token's sum, up to eight rows in flight.
+// A thread to 16 bytes of a token's sum, up to eight rows in flight: rows are anywhere, so it is the loads in flight that carry it.
 constexpr int kCombineInFlight = 8;
 template <typename T, int A, bool ONE>
 __global__ __launch_bounds__(256) void combine_kernel(const CombineParams p)
@@ -336,7 +348,8 @@ __device__ __forceinline__ float sum_of_wave(float v)   // in lane 63
     return v;
 }
 
-// A workgroup to a token.  Its gradient stays in registers where U pieces a thread hold it (U > 0), otherwise it is read once for each slot.
+// A workgroup to a token.  Its gradient stays in registers where U pieces a thread hold it (U > 0), otherwise it is read once for each
+// slot.  Both gradients in one pass: g times a weight goes out while g times the row is added up.
 template <typename T, int A, int U>
 __global__ __launch_bounds__(256) void combine_grad_kernel(const CombineParams p)
 {

@@ -1,5 +1,6 @@
-"""The operators around the fused experts (norm, SwiGLU, block-scaled product, router, tokens sorted by expert and back, adapters) from their definitions in float64, on the
-CPU: what the tests of the HIP kernels compare with.  Written with loops where that is plainer."""
+"""The operators around the fused experts (norm, SwiGLU, block-scaled product, router, tokens sorted by expert and back, adapters)
+from their definitions in float64, on the CPU: what the tests of the HIP kernels compare with.  Written with loops where that is
+plainer."""
 import math
 
 import torch
