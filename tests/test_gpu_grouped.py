@@ -190,3 +190,42 @@ def test_offsets_past_32_bits():
     last = out[:, N - 1]
     assert bool((last[17:R - 2] == 3).all()) and not bool(last[:17].any()) and not bool(last[R - 2:].any())
     assert int(out[-5000:].count_nonzero()) == 4998
+
+
+@pytest.mark.parametrize("N,K", [(7168, 128), (5000, 256), (7169, 384), (4096, 512), (3000, 640), (2048, 768), (2040, 1152)])
+def test_lists_of_tiles(N, K):
+    """more tiles of 256 x 256 than units, whole and half ones, K blocks and places of scales of every remainder: a sample of each expert's
+    rows against the oracle, all of them against the ungrouped product"""
+    g = torch.Generator().manual_seed(N)
+    counts = [700, 0, 129, 128, 256, 257, 1, 2000, 385, 1024, 640, 0, 511, 1300, 896, 2500]
+    tail = 70
+    print(f"case lists N={N} K={K}", flush=True)
+    args = problem(counts, tail, N, K, K)
+    out = run(*args)
+    x, xs, offsets, w, ws = args
+    for e, (lo, hi) in enumerate(zip(offsets.tolist(), offsets.tolist()[1:])):
+        if lo == hi:
+            continue
+        pick = torch.unique(torch.cat([torch.randint(lo, hi, (6,), generator=g), torch.tensor([lo, hi - 1])]))
+        assert_mm(out.cpu()[pick], x[pick], xs[pick], w[e], ws[e])
+        alone = layer_hip.block_scaled_mm(*(t.to(DEV) for t in (x[lo:hi], xs[lo:hi], w[e], ws[e])))
+        size = alone.float().abs().max().item()
+        assert (out[lo:hi].float() - alone.float()).abs().max().item() <= 2.0 ** -7 * size
+    assert not bool(out[int(offsets[-1]):].any())
+    assert torch.equal(out, run(*args))
+
+
+def test_more_tiles_than_lists_of_the_units_hold():
+    """above 15360 tiles there are more workgroups than units"""
+    counts, tail, N, K = [90000, 0, 47000, 100, 300], 3, 8192, 128
+    g = torch.Generator(device=DEV).manual_seed(3)
+    R, E = sum(counts) + tail, len(counts)
+    x = torch.randn((R, K), generator=g, device=DEV).to(torch.float8_e4m3fn)
+    xs, ws = (0.5 + torch.rand(shape, generator=g, device=DEV) for shape in ((R, 1), (E, N // 128, 1)))
+    w = torch.randn((E, N, K), generator=g, device=DEV).to(torch.float8_e4m3fn)
+    offsets = torch.tensor([0] + counts).cumsum(0).to(torch.int32)
+    out = layer_hip.grouped_block_scaled_mm(x, xs, offsets.to(DEV), w, ws)
+    for e, (lo, hi) in enumerate(zip(offsets.tolist(), offsets.tolist()[1:])):
+        if lo < hi:      # one K block: a sum of its own, the same in every tile
+            assert torch.equal(out[lo:hi], layer_hip.block_scaled_mm(x[lo:hi], xs[lo:hi], w[e], ws[e])), e
+    assert not bool(out[R - tail:].any())
