@@ -167,8 +167,8 @@ def add_adapters(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     scale ``[L]`` float32 or None (all 1), adapter_ids ``[M]`` int32 in any order (neighbours of one adapter share its reading).  K a multiple of
     128 up to 65536, N at most 2^24, rank a multiple of 8 up to 128, M at most 1048560.
 
-    Sums are fp32, in an order that depends on the sizes alone; the ``rank`` values between the two products are good to 2^-16; one
-    rounding at the end.  Another request's adapter or activations, whatever they hold, change nothing of a token's result.
+    Sums and the ``rank`` values between the two products are fp32, sums in an order that depends on the sizes alone; one rounding at
+    the end.  Another request's adapter or activations, whatever they hold, change nothing of a token's result.
     What an infinity in b meets is infinite or NaN.
     """
     return _add_adapters(base, x, x_scale, a, b, adapter_ids, scale)

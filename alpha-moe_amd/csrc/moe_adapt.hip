@@ -3,9 +3,9 @@
 //
 // Two kernels.  The first contracts tokens with the adapters' a, K split over wavefronts and workgroups, into partial sums in fp32
 // (workspace, [split][token][rank]); the second adds them up, in their order, times scale, and contracts with b.  Between the two, a token's
-// `rank` values are taken as sums of two bf16 numbers, high and low part, so that the second product on the bf16 matrix cores is as
-// good as one of fp32 values: the high part is the value's upper 16 bits, the low part the rest rounded to 8 bits, together 2^-16 off.
-// Both parts lie next to each other along the contraction, in front of b's values twice.
+// `rank` values are taken as sums of three bf16 numbers, eight of their 24 bits each, so that the second product on the bf16 matrix
+// cores is one of the fp32 values themselves: what base and adapter leave of each other where they cancel is as good as theirs.
+// The parts lie behind each other along the contraction, in front of b's values again.
 //
 // A token's adapter is its own, whatever its neighbours have: a workgroup takes a tile of neighbouring tokens, and the distinct adapters
 // among them one after the other (or P workgroups share them).  Tokens are columns of the matrix instructions, whose results depend on
@@ -176,13 +176,12 @@ __global__ __launch_bounds__(256, 2) void adapt_in_kernel(const AdaptParams p)
     });
 }
 
-// out: each wavefront 64 columns of T tiles of 16 tokens, whose b values stay in registers over the tiles.  Up to 16 ranks (RT = 1) their high and low parts lie behind each other in one
-// matrix instruction, and b's values twice; beyond, b's values of 32 ranks are multiplied with both.
+// out: each wavefront 64 columns of T tiles of 16 tokens, whose b values stay in registers over the tiles.  Up to 16 ranks (RT = 1) two parts
+// lie behind each other in one matrix instruction, and b's values twice; beyond, b's values of 32 ranks are multiplied with each.
 template <int RT, int T>
 __global__ __launch_bounds__(256, RT == 8 ? 3 : 4) void adapt_out_kernel(const AdaptParams p)
 {
-    constexpr int S = RT == 1 ? 1 : RT / 2, PARTS = RT == 1 ? 1 : 2;   // matrix instructions along the ranks, and for each of them
-    constexpr int kLow = RT == 1 ? 0 : 64 * S;                         // RT > 1: where the low parts of a token begin
+    constexpr int S = RT == 1 ? 1 : RT / 2, PARTS = RT == 1 ? 2 : 3;   // matrix instructions along the ranks, and for each of them
     constexpr int kRow = 64 * S * PARTS + 16;   // bytes of a token's parts in LDS, and 16 so that tokens' rows begin at other banks
     __shared__ __attribute__((aligned(16))) uint8_t parts[16 * T * kRow];
     __shared__ __attribute__((aligned(16))) float turned[4][16][68];   // of each wavefront: 64 columns of 16 tokens, from columns to rows
@@ -294,17 +293,22 @@ __global__ __launch_bounds__(256, RT == 8 ? 3 : 4) void adapt_out_kernel(const A
                 for (int s = 0; s < F; s++)
                     if (s0 + s < p.splits) v += in[s];
             }
-            uint32_t high[4];
-            float low[4];
+            float rest[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float f = v[j] * scale;
-                high[j] = __builtin_bit_cast(uint32_t, f) & 0xffff0000u;
-                low[j] = fabsf(f) == __builtin_inff() ? 0.f : f - __builtin_bit_cast(float, high[j]);
-            }
+            for (int j = 0; j < 4; j++) rest[j] = v[j] * scale;
+            // the upper 16 bits of what is left, three times: 24 bits, exact down to 2^-103 (the last part of less may be subnormal)
             uint8_t *to = parts + t * kRow + 2 * r;
-            *reinterpret_cast<uint2 *>(to) = make_uint2(high[0] >> 16 | high[1], high[2] >> 16 | high[3]);
-            *reinterpret_cast<uint2 *>(to + (RT == 1 ? 2 * rank : kLow)) = make_uint2(pack_bf16x2(low[0], low[1]), pack_bf16x2(low[2], low[3]));
+#pragma unroll
+            for (int h = 0; h < 3; h++) {
+                uint32_t part[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    part[j] = __builtin_bit_cast(uint32_t, rest[j]) & 0xffff0000u;
+                    rest[j] = fabsf(rest[j]) == __builtin_inff() ? 0.f : rest[j] - __builtin_bit_cast(float, part[j]);
+                }
+                *reinterpret_cast<uint2 *>(to + (RT > 1 ? 64 * S * h : h == 1 ? 2 * rank : 32 * h)) =
+                    make_uint2(part[0] >> 16 | part[1], part[2] >> 16 | part[3]);
+            }
         }
         __syncthreads();
         // Tile t: matrix row r of column tile k is column 16 k + r; the results go through LDS into rows.
@@ -314,7 +318,7 @@ __global__ __launch_bounds__(256, RT == 8 ? 3 : 4) void adapt_out_kernel(const A
             for (int s = 0; s < S; s++) {
 #pragma unroll
                 for (int h = 0; h < PARTS; h++) {
-                    const v8bf v = *reinterpret_cast<const v8bf *>(parts + (16 * t + n) * kRow + h * kLow + 64 * s + 16 * q);
+                    const v8bf v = *reinterpret_cast<const v8bf *>(parts + (16 * t + n) * kRow + 64 * S * h + 64 * s + 16 * q);
 #pragma unroll
                     for (int k = 0; k < 4; k++) acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv.v[s][k], v, acc[k], 0, 0, 0);
                 }

@@ -331,9 +331,10 @@ int alpha_moe_grouped_block_scaled_mm(const uint8_t *x, const float *x_scale, co
  * out[m] = base[m] where l is outside [0, num_adapters).
  *   base, out [M, N] bf16 (out may be base), x [M, K] bf16 or, with x_scale [M, K/128] f32 (else NULL), FP8 codes, a [num_adapters, rank, K]
  *   and b [num_adapters, N, rank] bf16, scale [num_adapters] f32 or NULL (all 1), adapter_ids [M].
- * K % 128 == 0, K <= 65536, N <= 2^24, rank a multiple of 8 up to 128, M <= 1048560 (both near their limits: ALPHA_MOE_ERR_SHAPE).  Sums in fp32, in an order that depends on the sizes only;
- * the rank's values between the two products are good to 2^-16; rounded once.  A product of 0 and an infinity in b
- * may stand for one of a small value and it: what an infinity in b meets is infinite or NaN.  workspace:
+ * K % 128 == 0, K <= 65536, N <= 2^24, rank a multiple of 8 up to 128, M <= 1048560 (both near their limits:
+ * ALPHA_MOE_ERR_SHAPE).  Sums and the rank's values between the two products are fp32, sums in an order that depends on the sizes only;
+ * rounded once.  A rank's value goes through the second product in parts, of which some may be 0: what an infinity in b meets is
+ * infinite or NaN.  workspace:
  * alpha_moe_adapters_workspace_bytes() bytes, 16-byte aligned, any contents, for one call at a time.
  */
 size_t alpha_moe_adapters_workspace_bytes(int M, int N, int K, int rank, int num_adapters);

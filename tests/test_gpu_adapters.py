@@ -197,3 +197,31 @@ def test_offsets_past_32_bits():
         if l >= 0:
             want[N - 1], want[5] = 1 + 6.0 * (m + 1), 1 + 2.0 * (m + 1) * (l % 7)
         assert torch.equal(got[m].float(), want), m
+
+
+@pytest.mark.parametrize("M,N,rank,fp8", [(1, 70, 8, False), (20, 64, 16, True), (40, 257, 24, False), (40, 33, 40, False), (9, 130, 128, True),
+                                          (2100, 1100, 32, False), (2100, 1090, 64, True), (2100, 1100, 128, False), (8200, 1100, 8, False)])
+def test_rank_values_of_24_bits_and_what_cancels(M, N, rank, fp8):
+    """One rank's value needs 24 bits, and base and a second rank's value cancel the upper ones: every sum is exact in fp32 (multiples of
+    2^-23 below 4, times the token's power of two), and so is the result, which is the lower bits."""
+    K, adapters = 128, 3
+    low = [1, 2.0 ** -3, 2.0 ** -6]                                    # 2^-17 (1 + 2^-3 + 2^-6): seven bits
+    x = torch.zeros((M, K))
+    x[:, 0], x[:, 1] = 1.0, 2.0 ** -8
+    x[:, 2:5] = torch.tensor(low)
+    size = 2.0 ** (torch.arange(M) % 5 - 2).float()[:, None]
+    a, b = torch.zeros((adapters, rank, K), dtype=BF), torch.zeros((adapters, N, rank), dtype=BF)
+    if fp8:                                                            # (the powers of two in the scales and in a: codes hold 2^-6 and up)
+        x[:, 1] = 1.0
+        scale, x = size.clone(), x.to(torch.float8_e4m3fn)
+    else:
+        scale, x = None, (x * size).to(BF)
+    first, second = 1, rank - 1
+    a[:, first, 0], a[:, first, 1], a[:, first, 2:5] = 1.0, 2.0 ** -8 if fp8 else 1.0, 2.0 ** -17
+    a[:, second, 1] = -(2.0 ** -8) if fp8 else -1.0
+    sign = (1.0 - 2.0 * (torch.arange(N) % 2)) * 2.0 ** (torch.arange(N) % 3).float()
+    b[:, :, first], b[:, :, second] = sign.to(BF), sign.to(BF)
+    base = (-size * sign).to(BF)
+    got = layer_hip.add_adapters(base.to(DEV), x.to(DEV), a.to(DEV), b.to(DEV), (torch.arange(M) % adapters).to(torch.int32).to(DEV),
+                                 x_scale=None if scale is None else scale.to(DEV))
+    assert torch.equal(got.cpu().float(), sum(low) * 2.0 ** -17 * size * sign)
