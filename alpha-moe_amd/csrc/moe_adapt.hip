@@ -236,17 +236,24 @@ __global__ __launch_bounds__(256, RT == 8 ? 3 : 4) void adapt_out_kernel(const A
         }
     };
     const unsigned long long with = __ballot((unsigned)id < (unsigned)p.adapters);
-    if (place.turn == 0 && with != there) {   // tokens without an adapter
-        const v4f zero[2] = {};
+    if (place.turn == 0 && with != there) {   // tokens without an adapter: base's bits
+        const unsigned long long tokens = there & ~with;
 #pragma unroll 1
         for (int c0 = c_begin; c0 < c_end; c0 += 256)
 #pragma unroll 1
             for (int t = 0; t < T; t++)
                 if (c0 + 64 <= p.N) {
                     const v4w base[2] = {load_base(c0, t, 0), load_base(c0, t, 1)};
-                    finish(c0, t, there & ~with, base, zero, zero);
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        if ((tokens >> (16 * t + 8 * h + row)) & 1) store(c0, t, h, base[h]);
                 } else {
-                    finish_ragged(c0, t, there & ~with, zero, zero);
+                    for (int h = 0; h < 2; h++) {
+                        const int token = 16 * t + 8 * h + row;
+                        const size_t from = (size_t)(m0 + token) * p.N + c0 + col;
+                        for (int i = 0; i < 8; i++)
+                            if (((tokens >> token) & 1) && c0 + col + i < p.N) p.out[from + i] = p.base[from + i];
+                    }
                 }
     }
     // eight values of a chunk of b: the ranks' chunks one behind the other (RT == 1: twice), 0 behind the last one

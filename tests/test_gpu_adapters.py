@@ -225,3 +225,14 @@ def test_rank_values_of_24_bits_and_what_cancels(M, N, rank, fp8):
     got = layer_hip.add_adapters(base.to(DEV), x.to(DEV), a.to(DEV), b.to(DEV), (torch.arange(M) % adapters).to(torch.int32).to(DEV),
                                  x_scale=None if scale is None else scale.to(DEV))
     assert torch.equal(got.cpu().float(), sum(low) * 2.0 ** -17 * size * sign)
+
+
+@pytest.mark.parametrize("M,N,rank", [(3, 7, 8), (40, 64, 16), (70, 129, 40), (2100, 1091, 24), (2100, 1091, 72)])
+def test_tokens_without_an_adapter_keep_their_bits(M, N, rank):
+    """a zero's sign, NaN of any payload, subnormals: what base holds is what they get"""
+    p = problem(M, N, 128, rank, 3, "mixed")
+    odd = torch.tensor([-0x8000, 0x7f81, 0x7fff, -1, -0x7f, 0x7f80, -0x80, 1, -0x7fff, 0], dtype=torch.int16)
+    p["base"] = odd.repeat(M * N // 10 + 1)[:M * N].reshape(M, N).view(BF)
+    p["adapter_ids"][0] = -1
+    none = (p["adapter_ids"] < 0) | (p["adapter_ids"] >= 3)
+    assert torch.equal(run(p).cpu().view(torch.int16)[none], p["base"].view(torch.int16)[none])
