@@ -845,10 +845,21 @@ struct InferenceOnly<Op, R (*)(Args...)> {
 // Each is the other's adjoint: a row's gradient goes to its token as a combination without weights, a token's to its rows with the
 // weights.  Saved are the map and, for the combination, rows and weights.  The functions below stand at the dispatcher's Autograd key;
 // where nobody waits for a gradient they are a redispatch.
-template <typename Fn>
-auto &typed_op(const char *name, const char *overload = "")
+// The dispatcher's handle of the operator that Op implements, looked up once for each (operators of one signature are told apart).
+template <auto Op>
+constexpr const char *op_name = nullptr;
+template <>
+constexpr const char *op_name<&sort_tokens> = "alpha_moe::sort_tokens";
+template <>
+constexpr const char *op_name<&combine_tokens> = "alpha_moe::combine_tokens";
+template <>
+constexpr const char *op_name<&combine_tokens_grad> = "alpha_moe::combine_tokens_grad";
+template <auto Op>
+auto &typed_op()
 {
-    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow(name, overload).template typed<Fn>();
+    static_assert(op_name<Op> != nullptr, "give the operator its name above");
+    static const auto op =
+        c10::Dispatcher::singleton().findSchemaOrThrow(op_name<Op>, "").template typed<std::remove_pointer_t<decltype(Op)>>();
     return op;
 }
 
@@ -862,7 +873,7 @@ bool wants_gradient(const at::Tensor &t, const char *name)
 at::Tensor combine_through_dispatcher(const at::Tensor &rows, const at::Tensor &row_of_slot, const c10::optional<at::Tensor> &topk_weights,
                                       double scaling_factor)
 {
-    return typed_op<decltype(combine_tokens)>("alpha_moe::combine_tokens").call(rows, row_of_slot, topk_weights, scaling_factor);
+    return typed_op<&combine_tokens>().call(rows, row_of_slot, topk_weights, scaling_factor);
 }
 
 // (Only the rows are an output of the function: one that nobody can differentiate costs the backward pass as much as one that one can.)
@@ -874,8 +885,7 @@ struct SortTokens : public torch::autograd::Function<SortTokens> {
                               Rest *rest)
     {
         const at::AutoDispatchBelowADInplaceOrView below;
-        auto [rows, offsets, row_of_slot] =
-            typed_op<decltype(sort_tokens)>("alpha_moe::sort_tokens").call(x, topk_ids, num_experts);
+        auto [rows, offsets, row_of_slot] = typed_op<&sort_tokens>().call(x, topk_ids, num_experts);
         ctx->save_for_backward({row_of_slot});
         *rest = {std::move(offsets), std::move(row_of_slot)};
         return std::move(rows);
@@ -894,7 +904,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> sort_tokens_autograd(c10::Dispatc
     const bool wanted = wants_gradient(x, "x");
     if (wanted && at::isFloat8Type(x.scalar_type())) refuse_gradient(x, "x");   // (of codes)
     if (!wanted)
-        return typed_op<decltype(sort_tokens)>("alpha_moe::sort_tokens").redispatch(keys & c10::after_autograd_keyset, x, topk_ids, num_experts);
+        return typed_op<&sort_tokens>().redispatch(keys & c10::after_autograd_keyset, x, topk_ids, num_experts);
     SortTokens::Rest rest;
     at::Tensor rows = SortTokens::apply(x, topk_ids, num_experts, &rest);
     return {std::move(rows), std::move(rest.offsets), std::move(rest.row_of_slot)};
@@ -916,7 +926,7 @@ struct CombineTokens : public torch::autograd::Function<CombineTokens> {
         const auto saved = ctx->get_saved_variables();
         auto optional = [](const at::Tensor &t, bool there) { return there && t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
         const bool for_rows = ctx->needs_input_grad(0), for_weights = saved[0].defined() && ctx->needs_input_grad(2);
-        const auto [rows, weights] = typed_op<decltype(combine_tokens_grad)>("alpha_moe::combine_tokens_grad")
+        const auto [rows, weights] = typed_op<&combine_tokens_grad>()
             .call(grads[0].contiguous(), optional(saved[0], for_weights), saved[1], optional(saved[2], true),
                   ctx->saved_data["scaling"].toDouble(), for_rows);
         return {for_rows ? rows : at::Tensor(), at::Tensor(), for_weights ? weights : at::Tensor(), at::Tensor()};
@@ -928,7 +938,7 @@ at::Tensor combine_tokens_autograd(c10::DispatchKeySet keys, const at::Tensor &r
     const bool for_rows = wants_gradient(rows, "rows");
     const bool for_weights = topk_weights.has_value() && wants_gradient(*topk_weights, "topk_weights");
     if (!for_rows && !for_weights)
-        return typed_op<decltype(combine_tokens)>("alpha_moe::combine_tokens")
+        return typed_op<&combine_tokens>()
             .redispatch(keys & c10::after_autograd_keyset, rows, row_of_slot, topk_weights, scaling_factor);
     return CombineTokens::apply(rows, row_of_slot, topk_weights, scaling_factor);
 }
