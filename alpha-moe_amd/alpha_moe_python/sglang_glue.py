@@ -128,7 +128,7 @@ def norm_sorted_moe(hidden_states: torch.Tensor, residual: torch.Tensor, norm_we
     s = sort_tokens(x.q, ids, experts, x_scale=x.scale)
     q, scale = swiglu_quant_fp8(grouped_block_scaled_mm(s.rows, s.scale, s.offsets, w13, w13_scale))
     rows = grouped_block_scaled_mm(q, scale, s.offsets, w2, w2_scale)
-    return combine_tokens(rows, s.row_of_slot, weights, routed_scaling_factor or 1.0), x.residual
+    return combine_tokens(rows, s.row_of_slot, weights, 1.0 if routed_scaling_factor is None else routed_scaling_factor), x.residual
 
 
 class Adapters(NamedTuple):

@@ -165,3 +165,15 @@ def test_oracle_of_adapters_by_hand():
     out, inner, outer = L.add_adapters(base, x, a, b, torch.tensor([0, 5, 1]), torch.tensor([10.0, -1.0]))
     assert out.tolist() == [[21.0, -19.0], [1.0, 1.0], [2.5, 13.0]]
     assert inner.tolist() == [[20.0, 20.0], [0.0, 0.0], [1.5, 12.0]] == outer.tolist()
+
+
+@pytest.mark.parametrize("factor,applied", [(None, 1.0), (1.0, 1.0), (2.5, 2.5), (0.0, 0.0), (-1.0, -1.0)])
+def test_expert_layer_applies_the_factor_it_is_given(factor, applied, monkeypatch):
+    """a factor of 0 is one, too"""
+    from alpha_moe_python.sglang_glue import norm_sorted_moe
+    seen, combine = [], layer_hip.combine_tokens
+    monkeypatch.setattr(layer_hip, "combine_tokens", lambda rows, at, w, c: seen.append(c) or combine(rows, at, w, c))
+    M, K, I, E, f8, bf = 3, 256, 128, 4, torch.float8_e4m3fn, torch.bfloat16
+    out, residual = norm_sorted_moe(meta((M, K), bf), meta((M, K), bf), meta((K,), bf), meta((E, K), bf), meta((E, 2 * I, K), f8),
+                                    meta((E, K, I), f8), meta((E, 2, 2)), meta((E, 2, 1)), 2, routed_scaling_factor=factor)
+    assert out.shape == residual.shape == (M, K) and seen == [applied]
