@@ -13,6 +13,9 @@
  * alpha_moe_group_plan tells how the group kernel would serve a call: plan = {tiles of 16 rows its variant takes in a row block,
  * 64-column groups of a down-projection item, items' column slabs, w2 block scales an item's table holds}.  Returns
  * ALPHA_MOE_ERR_SHAPE for a call that another kernel serves.  Host only.
+ *
+ * alpha_moe_grouped_mm_plan tells how alpha_moe_grouped_block_scaled_mm would serve a call of the same sizes: plan = {columns, tokens} of a
+ * tile (256 x 256: lists of them).  Host only.
  */
 #ifndef ALPHA_MOE_TUNING_H
 #define ALPHA_MOE_TUNING_H
@@ -21,6 +24,7 @@ extern "C" {
 #endif
 int alpha_moe_set_tunable(const char *name, int value, int set);
 int alpha_moe_group_plan(int top_k, int M, int K, int N, int num_experts, int sorted_num, int block_m, int stages, int plan[4]);
+int alpha_moe_grouped_mm_plan(int M, int N, int K, int num_experts, int plan[2]);
 #ifdef __cplusplus
 }
 #endif

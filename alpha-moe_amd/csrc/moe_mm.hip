@@ -1196,6 +1196,12 @@ Plan grouped_plan(int M, int N, int K, int E)
     return best;
 }
 
+bool grouped_sizes_fit(int M, int N, int K, int E)
+{
+    return M >= 0 && N > 0 && K > 0 && K % 128 == 0 && K <= 128 * kMaxKBlocks && M <= INT32_MAX - 255 && N <= INT32_MAX - 255 && E > 0 &&
+           E <= 4096;
+}
+
 template <bool G>
 int launch_plan(Plan plan, const MmParams &p, hipStream_t hs)
 {
@@ -1250,9 +1256,7 @@ extern "C" int alpha_moe_grouped_block_scaled_mm(const uint8_t *x, const float *
                                                  const float *w_scale, uint16_t *out, int M, int N, int K, int num_experts, void *stream)
 {
     using namespace alpha_moe;
-    if (M < 0 || N <= 0 || K <= 0 || K % 128 != 0 || K > 128 * kMaxKBlocks || M > INT32_MAX - 255 || N > INT32_MAX - 255 ||
-        num_experts <= 0 || num_experts > 4096)
-        return ALPHA_MOE_ERR_SHAPE;
+    if (!grouped_sizes_fit(M, N, K, num_experts)) return ALPHA_MOE_ERR_SHAPE;
     if (M == 0) return ALPHA_MOE_OK;
     if (!x || !x_scale || !offsets || !w || !w_scale || !out) return ALPHA_MOE_ERR_NULL_POINTER;
     if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) & 15) != 0)
@@ -1263,4 +1267,18 @@ extern "C" int alpha_moe_grouped_block_scaled_mm(const uint8_t *x, const float *
     p.quads = p.nkb >= 4;
     p.offsets = offsets, p.E = num_experts;
     return launch_plan<true>(grouped_plan(M, N, K, num_experts), p, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int alpha_moe_grouped_mm_plan(int M, int N, int K, int num_experts, int plan[2])
+{
+    using namespace alpha_moe;
+    if (!grouped_sizes_fit(M, N, K, num_experts) || M == 0) return ALPHA_MOE_ERR_SHAPE;
+    switch (grouped_plan(M, N, K, num_experts)) {
+    case kStreamHalf1: plan[0] = 16, plan[1] = 8; break;
+    case kStream2x1: plan[0] = 32, plan[1] = 16; break;
+    case kTile128x64: plan[0] = 128, plan[1] = 64; break;
+    case kTile256x128: plan[0] = 256, plan[1] = 128; break;
+    default: plan[0] = plan[1] = 256; break;
+    }
+    return ALPHA_MOE_OK;
 }

@@ -1,5 +1,7 @@
 """The block-scaled product of sorted tokens with their experts' weights, on the GPU, expert by expert against the float64 oracle with
 the tolerance of the ungrouped product (test_gpu_layer.py)."""
+import ctypes
+
 import pytest
 import torch
 
@@ -229,3 +231,24 @@ def test_more_tiles_than_lists_of_the_units_hold():
         if lo < hi:      # one K block: a sum of its own, the same in every tile
             assert torch.equal(out[lo:hi], layer_hip.block_scaled_mm(x[lo:hi], xs[lo:hi], w[e], ws[e])), e
     assert not bool(out[R - tail:].any())
+
+
+# tile (columns, tokens), counts, rows behind them, N, K: an expert of more than eight tiles of tokens, experts of none and of one row, more than
+# one group of columns to each XCD's run, and a number of columns that no tile divides
+TILES = [
+    ((16, 8), [1, 0, 1, 1], 1, 1000, 640), ((32, 16), [150, 0, 1, 0, 0, 0, 3] + [1, 0] * 30, 5, 2049, 1664),
+    ((128, 64), [560, 0, 1, 64], 30, 2049, 640), ((128, 64), [3, 700, 0, 65], 0, 4099, 1152), ((128, 64), [1030] + [40, 0, 1] * 6, 70, 2562, 1152),
+    ((256, 128), [1100, 0, 1] + [30, 128, 0, 129, 20, 5, 8] * 2 + [70] + [0] * 6, 190, 2049, 896),
+    ((256, 128), [10, 1200] + [0, 1, 30] * 4 + [129, 200], 130, 2561, 1024), ((256, 128), [0, 2, 1050, 0, 64, 33, 1, 20, 3, 7, 9, 1], 10, 4099, 1024),
+    ((256, 256), [2500, 0, 1, 128, 129, 300], 50, 2309, 384)]
+
+
+@pytest.mark.parametrize("tile,counts,tail,N,K", TILES)
+def test_every_tile(tile, counts, tail, N, K):
+    print(f"case tile {tile} {counts[:8]} of {len(counts)} tail={tail} N={N} K={K}", flush=True)
+    plan = (ctypes.c_int * 2)()
+    assert alpha_moe.c_abi.alpha_moe_grouped_mm_plan(sum(counts) + tail, N, K, len(counts), plan) == 0 and tuple(plan) == tile
+    args = problem(counts, tail, N, K, N + K)
+    out = run(*args)
+    check(*args, out)
+    assert torch.equal(out, run(*args))

@@ -177,3 +177,22 @@ def test_expert_layer_applies_the_factor_it_is_given(factor, applied, monkeypatc
     out, residual = norm_sorted_moe(meta((M, K), bf), meta((M, K), bf), meta((K,), bf), meta((E, K), bf), meta((E, 2 * I, K), f8),
                                     meta((E, K, I), f8), meta((E, 2, 2)), meta((E, 2, 1)), 2, routed_scaling_factor=factor)
     assert out.shape == residual.shape == (M, K) and seen == [applied]
+
+
+def test_every_tile_of_the_grouped_product_has_a_case():
+    """the cases of the test on the GPU are of the tiles that they name, and leave none out"""
+    import ctypes
+    from test_gpu_grouped import TILES
+    plan = (ctypes.c_int * 2)()
+    for tile, counts, tail, N, K in TILES:
+        assert A.alpha_moe_grouped_mm_plan(sum(counts) + tail, N, K, len(counts), plan) == OK and tuple(plan) == tile, (tile, N, K, tuple(plan))
+    reached = set()
+    for M in (1, 8, 61, 300, 1000, 3000, 10000, 70000):
+        for E in (1, 8, 60, 256, 700):
+            for N in (17, 512, 2049, 7168):
+                for K in (128, 640, 1024, 2048, 7168):
+                    assert A.alpha_moe_grouped_mm_plan(M, N, K, E, plan) == OK
+                    reached.add(tuple(plan))
+    assert reached == {t[0] for t in TILES}
+    for M, N, K, E in ((0, 8, 128, 1), (8, 8, 64, 1), (8, 8, 128, 4097), (8, 0, 128, 1)):
+        assert A.alpha_moe_grouped_mm_plan(M, N, K, E, plan) == SHAPE
