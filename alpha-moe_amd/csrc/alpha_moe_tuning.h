@@ -14,8 +14,9 @@
  * 64-column groups of a down-projection item, items' column slabs, w2 block scales an item's table holds}.  Returns
  * ALPHA_MOE_ERR_SHAPE for a call that another kernel serves.  Host only.
  *
- * alpha_moe_grouped_mm_plan tells how alpha_moe_grouped_block_scaled_mm would serve a call of the same sizes: plan = {columns, tokens} of a
- * tile (256 x 256: lists of them).  Host only.
+ * alpha_moe_grouped_mm_plan and alpha_moe_adapters_plan tell how alpha_moe_grouped_block_scaled_mm and alpha_moe_add_adapters would serve
+ * a call of the same sizes: plan = {columns, tokens} of a tile (256 x 256: lists of them), and plan = {tokens of a tile, workgroups that
+ * share one's adapters} of the first and of the second kernel, {parts of K, 256 columns that a workgroup of the second takes}.  Host only.
  */
 #ifndef ALPHA_MOE_TUNING_H
 #define ALPHA_MOE_TUNING_H
@@ -25,6 +26,7 @@ extern "C" {
 int alpha_moe_set_tunable(const char *name, int value, int set);
 int alpha_moe_group_plan(int top_k, int M, int K, int N, int num_experts, int sorted_num, int block_m, int stages, int plan[4]);
 int alpha_moe_grouped_mm_plan(int M, int N, int K, int num_experts, int plan[2]);
+int alpha_moe_adapters_plan(int M, int N, int K, int rank, int num_adapters, int plan[6]);
 #ifdef __cplusplus
 }
 #endif

@@ -379,7 +379,7 @@ struct AdaptPlan {
     struct Tiles {
         int tokens, sharers;
     } in, out;
-    int splits;
+    int splits, run;   // parts of K, and 256 columns that a workgroup of the second kernel takes one behind the other
     AdaptPlan(int M, int N, int K, int rank, int adapters)
     {
         auto shared = [&](int tokens) {
@@ -394,6 +394,8 @@ struct AdaptPlan {
         int64_t want = in.tokens == 16 ? (groups <= 512 ? 8 : 4) : ceil_div(1024, groups);
         if (in.tokens == 64 && M > 2048 && want > 4) want = 4;
         splits = (int)(want > can ? can : want);
+        const int64_t pieces = ceil_div(N, 256) * ceil_div(M, out.tokens) / 1536;   // 256 columns of a tile
+        run = pieces < 1 ? 1 : pieces > 4 ? 4 : (int)pieces;
     }
 };
 
@@ -472,10 +474,17 @@ extern "C" int alpha_moe_add_adapters(const uint16_t *base, const void *x, const
     p.base = base, p.a = a, p.b = b, p.x = static_cast<const uint8_t *>(x), p.x_scale = x_scale, p.scale = scale;
     p.ids = adapter_ids, p.out = out, p.part = static_cast<float *>(workspace);
     p.M = M, p.N = N, p.K = K, p.rank = rank, p.adapters = num_adapters, p.nkb = K / 128;
-    p.splits = plan.splits;
-    const int64_t pieces = ceil_div(N, 256) * ceil_div(M, plan.out.tokens) / 1536;   // 256 columns of a tile
-    p.run = pieces < 1 ? 1 : pieces > 4 ? 4 : (int)pieces;
+    p.splits = plan.splits, p.run = plan.run;
     hipStream_t hs = static_cast<hipStream_t>(stream);
     const hipError_t err = rank <= 16 ? adapt<1>(p, plan, hs) : rank <= 32 ? adapt<2>(p, plan, hs) : rank <= 64 ? adapt<4>(p, plan, hs) : adapt<8>(p, plan, hs);
     return err == hipSuccess ? ALPHA_MOE_OK : err == hipErrorInvalidConfiguration ? ALPHA_MOE_ERR_SHAPE : ALPHA_MOE_ERR_LAUNCH;
+}
+
+extern "C" int alpha_moe_adapters_plan(int M, int N, int K, int rank, int num_adapters, int plan[6])
+{
+    if (M <= 0 || !sizes_fit(M, N, K, rank, num_adapters)) return ALPHA_MOE_ERR_SHAPE;
+    const AdaptPlan a(M, N, K, rank, num_adapters);
+    const int values[6] = {a.in.tokens, a.in.sharers, a.out.tokens, a.out.sharers, a.splits, a.run};
+    for (int i = 0; i < 6; i++) plan[i] = values[i];
+    return ALPHA_MOE_OK;
 }

@@ -5,6 +5,8 @@ behind each other, 2 u each if it cuts instead of rounding, some 64 more for the
 magnitudes.  The rank's values are then good to 2^-16, their second product is 2 rank additions of 2 u and a few roundings: 2^-16 + (4 rank +
 12) u.  The result is rounded to bf16, 2^-8.
 """
+import ctypes
+
 import pytest
 import torch
 
@@ -236,3 +238,69 @@ def test_tokens_without_an_adapter_keep_their_bits(M, N, rank):
     p["adapter_ids"][0] = -1
     none = (p["adapter_ids"] < 0) | (p["adapter_ids"] >= 3)
     assert torch.equal(run(p).cpu().view(torch.int16)[none], p["base"].view(torch.int16)[none])
+
+
+# (tokens of a tile in the first and the second kernel, 256 columns that a workgroup of the second takes), M, N, K, rank, adapters, fp8.  K of up to four
+# blocks is in one part, whatever the tile
+TILES = [
+    ((16, 16, 1), 40, 70, 128, 16, 5, False), ((16, 16, 1), 61, 200, 384, 8, 9, True), ((16, 16, 1), 700, 1300, 512, 32, 9, True), ((16, 16, 1), 500, 333, 256, 64, 6, False),
+    ((16, 16, 1), 300, 257, 384, 128, 9, True), ((64, 16, 1), 2000, 1100, 256, 40, 9, False), ((64, 16, 1), 8200, 130, 128, 8, 7, True),
+    ((16, 64, 1), 4000, 1091, 256, 16, 9, False), ((16, 64, 1), 2100, 1100, 384, 24, 5, True),
+    ((64, 64, 1), 8200, 1100, 128, 8, 11, False), ((64, 64, 1), 8200, 1025, 256, 8, 11, True), ((64, 64, 1), 4200, 1091, 384, 16, 9, False),
+    ((64, 64, 1), 4200, 1100, 128, 16, 9, True), ((64, 64, 1), 2800, 1090, 256, 24, 9, False), ((64, 64, 1), 2100, 1090, 512, 32, 4, True),
+    ((64, 64, 1), 2800, 1100, 128, 40, 30, False), ((64, 64, 1), 2100, 1091, 256, 64, 9, True), ((64, 32, 1), 2100, 1100, 128, 72, 9, False),
+    ((64, 32, 1), 2100, 1091, 256, 128, 9, True),
+    ((64, 64, 2), 8200, 6001, 128, 8, 37, False), ((64, 64, 2), 8200, 6081, 128, 24, 9, True), ((64, 64, 3), 8200, 9100, 128, 64, 9, False),
+    ((64, 32, 2), 4200, 6001, 128, 72, 9, False), ((64, 64, 4), 8200, 12101, 128, 16, 9, True), ((64, 32, 4), 8200, 7000, 128, 128, 9, False)]
+
+
+def plan_of(M, N, K, rank, adapters):
+    plan = (ctypes.c_int * 6)()
+    assert alpha_moe.c_abi.alpha_moe_adapters_plan(M, N, K, rank, adapters, plan) == 0
+    return plan[0], plan[2], plan[5]
+
+
+@pytest.mark.parametrize("tiles,M,N,K,rank,adapters,fp8", TILES)
+def test_every_tile_and_run(tiles, M, N, K, rank, adapters, fp8):
+    """Every token has the bits that it has in a call of few tokens (smaller tiles, one group of columns to a workgroup: sums are the same for K
+    of one part); a sample of tokens against the oracle."""
+    print(f"case tiles {tiles} M={M} N={N} K={K} rank={rank} of {adapters} fp8={fp8}", flush=True)
+    assert plan_of(M, N, K, rank, adapters) == tiles
+    g = torch.Generator().manual_seed(N)
+    # requests of some 40 tokens, so that tiles have one, two and more of them, and a part where every token has its own
+    ids = torch.randint(-1, adapters, (M // 40 + 2,), generator=g).repeat_interleave(40)[:M]
+    ids[M // 3:M // 3 + 150] = torch.randint(-1, adapters + 1, (M,), generator=g)[:len(ids[M // 3:M // 3 + 150])]
+    p = problem(M, N, K, rank, adapters, ids, fp8)
+    d = {k: None if v is None else v.to(DEV) for k, v in p.items()}
+    got = layer_hip.add_adapters(**d)
+    rows = ("base", "x", "adapter_ids", "x_scale")
+    for lo in range(0, M, 509):
+        part = {k: v[lo:lo + 509].clone() if k in rows and v is not None else v for k, v in d.items()}
+        assert plan_of(len(part["x"]), N, K, rank, adapters) == (16, 16, 1)
+        assert torch.equal(got[lo:lo + 509], layer_hip.add_adapters(**part)), lo
+    pick = torch.unique(torch.cat([torch.randint(0, M, (150,), generator=g), torch.tensor([0, M - 1])]))
+    check({k: v[pick] if k in rows and v is not None else v for k, v in p.items()}, got[pick.to(DEV)])
+
+
+@pytest.mark.parametrize("M,N,rank,fp8", [(8200, 1100, 8, False), (4200, 1091, 16, True), (2800, 1090, 24, False), (2100, 1100, 64, True),
+                                          (2100, 1091, 128, False), (8200, 6001, 8, False)])
+def test_large_tiles_look_at_no_other_request(M, N, rank, fp8):
+    """NaN and infinities in another adapter and in another token, in tiles that hold both"""
+    K, adapters = 128, 5
+    assert plan_of(M, N, K, rank, adapters)[:2] == (64, 32 if rank > 64 else 64)
+    p = problem(M, N, K, rank, adapters, "mixed", fp8)
+    clean = run(p)
+    bad = {k: None if v is None else v.clone() for k, v in p.items()}
+    bad["a"][2], bad["b"][2], bad["scale"][2] = float("nan"), float("inf"), float("nan")
+    for m in (77, M - 3):
+        bad["x"][m:m + 1] = torch.full((1, K), float("nan")).to(p["x"].dtype)
+    if fp8:
+        bad["x_scale"][M - 9] = float("inf")
+    got = run(bad)
+    keep = p["adapter_ids"] != 2
+    keep[77] = keep[M - 3] = keep[M - 9] = False
+    assert torch.equal(got.cpu()[keep], clean.cpu()[keep])
+    assert bool(got[(p["adapter_ids"] == 2).to(DEV)].isnan().all())
+    for m in (77, M - 3):
+        if 0 <= int(p["adapter_ids"][m]) < adapters:
+            assert bool(got[m].isnan().all())

@@ -179,6 +179,21 @@ def test_expert_layer_applies_the_factor_it_is_given(factor, applied, monkeypatc
     assert out.shape == residual.shape == (M, K) and seen == [applied]
 
 
+def test_every_kernel_of_the_adapters_has_a_case():
+    """the cases of the test on the GPU are of the tiles that they name; each kind of rank, tile and codes is among them"""
+    from test_gpu_adapters import TILES, plan_of
+    first, second, runs = set(), set(), set()
+    for tiles, M, N, K, rank, adapters, fp8 in TILES:
+        assert plan_of(M, N, K, rank, adapters) == tiles
+        kind = 16 if rank <= 16 else 32 if rank <= 32 else 64 if rank <= 64 else 128
+        first.add((tiles[0], min(kind, 64 if tiles[0] == 64 else 32), fp8))          # (of more ranks, workgroups take a part)
+        second.add((tiles[1], kind))
+        runs.add((tiles[1], tiles[2]))
+    assert first == {(t, k, f) for t, ks in ((16, (16, 32)), (64, (16, 32, 64))) for k in ks for f in (False, True)}
+    assert second == {(16, 16), (16, 32), (16, 64), (16, 128), (64, 16), (64, 32), (64, 64), (32, 128)}
+    assert runs == {(16, 1), (64, 1), (64, 2), (64, 3), (64, 4), (32, 1), (32, 2), (32, 4)}
+
+
 def test_every_tile_of_the_grouped_product_has_a_case():
     """the cases of the test on the GPU are of the tiles that they name, and leave none out"""
     import ctypes
