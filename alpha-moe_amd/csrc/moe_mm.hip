@@ -258,9 +258,10 @@ __device__ __forceinline__ bool enter_group(MmParams &p, GroupTile &g)
 // split within one launch, the last workgroup adding up, has not been tried.
 // Why through LDS, though no wavefront reads what another has loaded: a load into a matrix operand's registers takes 64 bytes of sixteen
 // lines, and lines are what the path counts (61 x 2112 x 7168 so 15.4 us, 1 x 4096 x 7168 7.8).
-// Weights are loaded non-temporally only with at most eight tokens, where they are read once and there is little else to read
+// Weights are loaded non-temporally (NT) only where one tile of tokens reads them and there is little else to read: with at most eight tokens
 // (1 x 4096 x 7168 from HBM 7.1 us against 7.6, 3 x 1280 x 5120 4.7 and 5.0; but 61 x 2112 x 7168 11.9 and 8.3.  A loop over one small
-// matrix would rather keep it in L2, 3 x 1280 x 5120 4.7 and 3.4 us; a model's layers come back after all the others).
+// matrix would rather keep it in L2, 3 x 1280 x 5120 4.7 and 3.4 us; a model's layers come back after all the others), and in a
+// grouped product whose experts have at most 16 rows on average (launch_plan()).
 // Deeper rings change nothing (16 x 4096 x 7168 with two, four K blocks 7.0, 7.05 us).  Eight wavefronts where a tile is 16 x 16 or
 // the tokens are few, four for larger ones, of which two fit a compute unit (17 x 4096 x 7168, 32 x 16 tile, eight 7.7, four 6.9 us; 32 x
 // 4096 x 7168 7.4, 7.1; 32 x 32 tile 61 x 2112 x 7168 8.7, 8.4; 16 x 16 tile, 16 x 4096 x 7168, 6.8 with eight).
@@ -277,7 +278,7 @@ struct StreamRing {
     static_assert(kBytes <= 160 * 1024, "");
 };
 
-template <int R, int T, int WAVES, int D, bool HALF, bool GROUPED>
+template <int R, int T, int WAVES, int D, bool HALF, bool GROUPED, bool NT>
 __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(MmParams p)
 {
     typedef StreamRing<R, T, WAVES, D, HALF> Ring;
@@ -351,7 +352,7 @@ __global__ __launch_bounds__(WAVES * 64) void mm_stream_kernel(MmParams p)
             if (!RUN && lane < T * 16) dma4(xsbuf, xs_off, 4u * (unsigned)kb, at + (R + T) * 2048);
             if (RUN && scales.loads(kb, i == 0)) scales.load(xsbuf, xs_off, kb, 0, lane < T * 16, xs);
         } else if constexpr (j < 2 * R) {
-            dma16<HALF || (GROUPED && T == 1) ? 2 : 0>(wbuf, w_off[j / 2][j % 2], 128u * kb, at + j * 1024);
+            dma16<NT ? 2 : 0>(wbuf, w_off[j / 2][j % 2], 128u * kb, at + j * 1024);
         } else {
             constexpr int t = HALF ? tj : tj / 2, h = HALF ? 0 : tj % 2;
             dma16<0>(xbuf, x_off[t][h], 128u * kb, at + (R + t) * 2048 + h * 1024);
@@ -461,10 +462,11 @@ hipError_t launch_tiles(Kernel kernel, MmParams p, int cols, int tokens, int thr
     return hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3(run * 8), dim3(threads), args, 0, stream);
 }
 
-template <int R, int T, int WAVES, int D, bool HALF, bool GROUPED = false>
+template <int R, int T, int WAVES, int D, bool HALF, bool GROUPED = false, bool NT = HALF>
 hipError_t launch_stream_mm(const MmParams &p, hipStream_t stream)
 {
-    return launch_tiles(mm_stream_kernel<R, T, WAVES, D, HALF, GROUPED>, p, R * 16, GROUPED && HALF ? 8 : T * 16, WAVES * 64, GROUPED, stream);
+    return launch_tiles(mm_stream_kernel<R, T, WAVES, D, HALF, GROUPED, NT>, p, R * 16, GROUPED && HALF ? 8 : T * 16, WAVES * 64, GROUPED,
+                        stream);
 }
 
 // Many tokens: WN x WM wavefronts, each with TN * 16 columns x TM * 16 tokens of a workgroup's tile, through S stages of one K
@@ -1166,7 +1168,7 @@ Plan grouped_plan(int M, int N, int K, int E)
     const int mean = M / E, nkb = K / 128;
     if (tiles_of(M, N, 32, 1) <= kUnits / 2) return kStreamHalf1;
     // Too few tiles of 128 x 64 for the units (if every other expert has one more than its rows fill), and a long K, which the streaming
-    // kernel's wavefronts share: 32x16 / 128x64 8 experts, 25 rows, N = 142, K = 6528 8.7 / 22; 60 rows, N = 903, K = 1408 10.4 / 9.1.
+    // kernel's wavefronts share: 32x16 / 128x64 8 experts, 25 rows, N = 142, K = 6528 7.1 / 20; 60 rows, N = 903, K = 1408 10.4 / 9.1.
     if (mean <= nkb && (M / 64 + (E < M ? E : M) / 2 + 1) * (int64_t)((N + 127) / 128) <= kUnits / 2) return kStream2x1;
     if (mean <= 8 && nkb >= 12) return kStream2x1;
     // The tile whose rounds over the compute units take the least time: what a tile takes beside its K blocks, and for each of them with
@@ -1209,7 +1211,12 @@ int launch_plan(Plan plan, const MmParams &p, hipStream_t hs)
     if constexpr (G) {   // (grouped_plan() names no others)
         switch (plan) {
         case kStreamHalf1: err = launch_stream_mm<1, 1, 8, 2, true, true>(p, hs); break;
-        case kStream2x1: err = launch_stream_mm<2, 1, 4, 2, false, true>(p, hs); break;
+        case kStream2x1:
+            // MI355X, weights from HBM, us, non-temporally / not: 256 experts, N = 512, K = 7168, routed, 2 rows on average 93 / 104, 6 rows 133 /
+            // 137, 2 or 7 rows and a 257th expert that all 61 or 200 tokens visit 94 / 105, 139 / 146; 8 experts, N = 1024, 12 rows 12.0 / 13.1,
+            // 17 rows 19.5 / 16.0, 40 rows 24.1 / 22.6, 56 rows 30.9 / 26.8; N = 142, K = 6528, 25 rows 8.7 / 7.1.
+            err = p.M / p.E <= 16 ? launch_stream_mm<2, 1, 4, 2, false, true, true>(p, hs) : launch_stream_mm<2, 1, 4, 2, false, true>(p, hs);
+            break;
         case kTile128x64: err = launch_tile_mm<4, 2, 2, 2, 3, 4, true>(p, hs); break;
         case kTile256x128: err = launch_tile_mm<4, 4, 4, 2, 3, 4, true>(p, hs); break;
         default: err = launch_ragged_mm(p, hs); break;

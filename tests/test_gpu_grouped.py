@@ -237,6 +237,7 @@ def test_more_tiles_than_lists_of_the_units_hold():
 # one group of columns to each XCD's run, and a number of columns that no tile divides
 TILES = [
     ((16, 8), [1, 0, 1, 1], 1, 1000, 640), ((32, 16), [150, 0, 1, 0, 0, 0, 3] + [1, 0] * 30, 5, 2049, 1664),
+    ((32, 16), [40, 0, 90, 1, 33, 16, 17, 23], 10, 142, 6528),
     ((128, 64), [560, 0, 1, 64], 30, 2049, 640), ((128, 64), [3, 700, 0, 65], 0, 4099, 1152), ((128, 64), [1030] + [40, 0, 1] * 6, 70, 2562, 1152),
     ((256, 128), [1100, 0, 1] + [30, 128, 0, 129, 20, 5, 8] * 2 + [70] + [0] * 6, 190, 2049, 896),
     ((256, 128), [10, 1200] + [0, 1, 30] * 4 + [129, 200], 130, 2561, 1024), ((256, 128), [0, 2, 1050, 0, 64, 33, 1, 20, 3, 7, 9, 1], 10, 4099, 1024),
