@@ -1,5 +1,6 @@
 """The operators around the fused experts: what a decoder layer runs in front of ``fused_moe_w8a8_up_down``, the FP8 products of
-its dense layers, and what brings tokens to weights of their own outside the fused call.  Callers of the reference take these from their serving engine.
+its dense layers, and what brings tokens to weights of their own outside the fused call.  Callers of the reference take these from
+their serving engine.
 
 * :func:`rms_norm_quant_fp8` - residual addition, RMS norm and per-token-group FP8 quantisation in one kernel;
 * :func:`route_topk`         - the router's selection, in the form ``moe_align_block_size`` and the fused operator take;

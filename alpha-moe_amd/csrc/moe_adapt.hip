@@ -13,9 +13,10 @@
 // them, NaN or infinity, reaches a token.
 //
 // What bounds it: of many tokens memory, x once, base and result once each (8192 tokens, K = 2048, N = 7168, rank 64: 271 MB, 53 us at a
-// copy's rate; MI355X 20 us the first kernel and 65 the second, whose b is read again by every tile out of the L2); of few tokens two launches,
-// each one chain of loads and a sum over wavefronts (1 token 4.1 and 3.6 us, 61 tokens of 48 adapters 8.1 and 4.8).  One kernel for
-// both would have every column's workgroup contract all of K again, or wait for the others.
+// copy's rate; MI355X 20 us the first kernel and 70 the second, whose b is read again by every tile out of the L2; it was 65 with two parts,
+// 2^-16 off, whose tiles fit a compute unit once more); of few tokens two launches, each one chain of loads and a sum over wavefronts (1 token 4.2
+// and 3.8 us, 61 tokens of 48 adapters 8.4 and 5.0).  One kernel for both would have every column's workgroup contract all of K again, or
+// wait for the others.
 //
 // Operands as in moe_common.hpp: adapters' rows are A, tokens B, results (row 4q + j, token n) in register j of lane (n, q).
 #include "moe_common.hpp"
@@ -476,7 +477,10 @@ extern "C" int alpha_moe_add_adapters(const uint16_t *base, const void *x, const
     p.M = M, p.N = N, p.K = K, p.rank = rank, p.adapters = num_adapters, p.nkb = K / 128;
     p.splits = plan.splits, p.run = plan.run;
     hipStream_t hs = static_cast<hipStream_t>(stream);
-    const hipError_t err = rank <= 16 ? adapt<1>(p, plan, hs) : rank <= 32 ? adapt<2>(p, plan, hs) : rank <= 64 ? adapt<4>(p, plan, hs) : adapt<8>(p, plan, hs);
+    const hipError_t err = rank <= 16   ? adapt<1>(p, plan, hs)
+                           : rank <= 32 ? adapt<2>(p, plan, hs)
+                           : rank <= 64 ? adapt<4>(p, plan, hs)
+                                        : adapt<8>(p, plan, hs);
     return err == hipSuccess ? ALPHA_MOE_OK : err == hipErrorInvalidConfiguration ? ALPHA_MOE_ERR_SHAPE : ALPHA_MOE_ERR_LAUNCH;
 }
 

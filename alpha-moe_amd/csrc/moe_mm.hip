@@ -20,10 +20,10 @@
 //
 // The grouped product (rows sorted by expert, an expert's weights for its rows) is the same kernels, whose workgroups find their tile from the
 // experts' offsets; grouped_plan() chooses.  No host knows how many rows an expert has, so the grid is the most there can be.  What bounds
-// it: with a row or two to an expert the weights (61 tokens, 8 of 256 experts each, N = 512, K = 7168 91 us for about 600 MB; MI355X, a copy
-// runs at 5.1 TB/s), with a single token the round trip to the offsets and the weights (7.8 us, 5.8 at a copy's rate), of many the matrix
-// cores and, of few K blocks, memory (65536 rows of 128 experts, N = 1536, K = 2048: 251 us, 1640 TFLOP/s; 156 at the rate of one 8192^3
-// product without block scales; 737 MB are 144 us of a copy; matrix cores are busy 48 % of the time, 62 in a dense product).
+// it: with a row or two to an expert the weights (61 tokens, 8 of 256 experts each, N = 512, K = 7168 88 - 102 us by card for 602 MB; MI355X, a
+// copy runs at 5.1 TB/s), with a single token the round trip to the offsets and the weights (7.8 us, 5.8 at a copy's rate), of many the matrix
+// cores and, of few K blocks, memory (65536 rows of 128 experts, N = 1536, K = 2048: 251 - 261 us by card, 1580 - 1640 TFLOP/s; 156 at the
+// rate of one 8192^3 product without block scales; 737 MB are 144 us of a copy; matrix cores are busy 48 % of the time, 62 in a dense product).
 #include <type_traits>
 #include <utility>
 
@@ -1158,26 +1158,26 @@ Plan plan(int M, int N)
 
 // Of a grouped call, by the rows that an expert has on average; how they are spread, only the device knows.  MI355X, us, experts drawn as
 // a router's are (the largest has four times the average), 32x16 / 128x64 / 256x128 / 256x256 tile: 256 experts, N = 512, K = 7168: 2 rows
-// on average 102 / 131 / 146 / 207, 8 rows 157 / 167 / 170 / 226, 32 rows 285 / 201 / 204 / 259, 64 rows 416 / 227 / 220 / 312, 256 rows
-// 1300 / 492 / 414 / 443; 128 experts, N = 1536, K = 2048: 16 rows 105 / 74 / 82 / 105, 128 rows 420 / 142 / 124 / 134, 512 rows 1457 / 402 /
-// 306 / 278.  With few K blocks (N = 7168, K = 256) most wavefronts of the streaming kernel have nothing to do, and what a tile takes beside
-// its K blocks counts: 2 rows 199 / 126 / - / -, 256 rows - / 787 / 610 / 459.  Fewer tiles than units: the smallest (8 rows of 8 experts,
-// N = 512, K = 7168, 16x16 9.2, 32x16 10.2).
+// on average 91 / 113 / 133 / 135, 8 rows 138 / 148 / 148 / 151, 32 rows 262 / 187 / 208 / 226, 64 rows 405 / 225 / 223 / 224, 256 rows
+// 1261 / 479 / 389 / 424; 128 experts, N = 1536, K = 2048: 16 rows 94 / 72 / 78 / 76, 128 rows 371 / 138 / 121 / 112, 512 rows 1319 / 380 /
+// 288 / 255.  With few K blocks (256 experts, N = 7168, K = 256) most wavefronts of the streaming kernel have nothing to do, and what a tile
+// takes beside its K blocks counts: 2 rows 202 / 121 / 147 / 103, 256 rows 3997 / 791 / 613 / 346.  Fewer tiles than units: the smallest (8 rows
+// of 8 experts, N = 512, K = 7168, 16x16 9.2, 32x16 10.2).
 Plan grouped_plan(int M, int N, int K, int E)
 {
     const int mean = M / E, nkb = K / 128;
     if (tiles_of(M, N, 32, 1) <= kUnits / 2) return kStreamHalf1;
     // Too few tiles of 128 x 64 for the units (if every other expert has one more than its rows fill), and a long K, which the streaming
-    // kernel's wavefronts share: 32x16 / 128x64 8 experts, 25 rows, N = 142, K = 6528 7.1 / 20; 60 rows, N = 903, K = 1408 10.4 / 9.1.
+    // kernel's wavefronts share: 32x16 / 128x64 8 experts, 25 rows, N = 142, K = 6528 7.1 / 20; 60 rows, N = 903, K = 1408 8.1 / 7.9.
     if (mean <= nkb && (M / 64 + (E < M ? E : M) / 2 + 1) * (int64_t)((N + 127) / 128) <= kUnits / 2) return kStream2x1;
     if (mean <= 8 && nkb >= 12) return kStream2x1;
     // The tile whose rounds over the compute units take the least time: what a tile takes beside its K blocks, and for each of them with
     // tiles for half the units and with as many as run at a time (as plan() has them; the largest, whose K blocks go on from tile to tile,
     // as its own calls have it).  An expert's last tile is half empty; of the largest, half a tile then.  Its lists are of whole numbers
     // of tiles, 0.75 rounds more than even ones.  MI355X, us, 256x256 and the better one of the others, the taken one first: 128 experts
-    // of 256 rows, N = 7168, K = 256 171 / 228, of 128 rows, N = K = 2048 152 / 162, 64 of 500, N = 2048, K = 128 31 / 57, 160 of 40, N = 5120,
-    // K = 384 95 / 114; 128 of 800, N = 512, K = 7168 428 / 501, 64 of 300, N = 2048, K = 7168 363 / 391.  The rule was at most 6 % behind in
-    // 29 such calls.
+    // of 256 rows, N = 7168, K = 256 176 / 297, of 128 rows, N = K = 2048 152 / 160, 64 of 500, N = 2048, K = 128 31 / 57, 160 of 40, N = 5120,
+    // K = 384 95 / 114; 128 of 800, N = 512, K = 7168 425 / 501, 64 of 300, N = 2048, K = 7168 362 / 393.  Of 34 such calls the rule took the best
+    // within half a percent in 27, one at most 4 % behind in six and one 9 % behind (64 experts of 128 rows, N = 1408, K = 2048 53 / 48, in 128x64).
     static const struct {
         Plan plan;
         int cols, tokens, resident;
