@@ -118,10 +118,11 @@ def sort_tokens(x: torch.Tensor, topk_ids: torch.Tensor, num_experts: int, x_sca
 
     x ``[M, K]`` bf16, fp32 or float8_e4m3fn codes (K a multiple of 128) with or without ``x_scale [M, K/128]`` float32; topk_ids
     ``[M, top_k]`` int32, top_k at most 64, at most 4096 experts, M below 2^24 - 1, rows of at most 2^27 bytes.
-    Returns ``rows [M * top_k, K]``: x's row of every slot by ascending expert, equal experts by ascending slot, and behind them a row of zeros for each slot whose id is outside ``[0, num_experts)`` (a padded
-    batch, experts of another GPU); ``scale`` in the same order; ``offsets [num_experts + 1]`` int32, the first row of each expert, the
-    last one the number of slots that have one; ``row_of_slot [M, top_k]`` int32, the slot's row r, or ``~r`` (negative) where that is one of
-    the zeros.  Nothing of it depends on anything but the inputs.
+    Returns ``rows [M * top_k, K]``: x's row of every slot by ascending expert, equal experts by ascending slot, and behind them
+    a row of zeros for each slot whose id is outside ``[0, num_experts)`` (a padded batch, experts of another GPU); ``scale`` in
+    the same order; ``offsets [num_experts + 1]`` int32, the first row of each expert, the last one the number of slots that
+    have one; ``row_of_slot [M, top_k]`` int32, the slot's row r, or ``~r`` (negative) where that is one of the zeros. Nothing
+    of it depends on anything but the inputs.
 
     Differentiable in x where there is no x_scale: a token's gradient is its slots' sum, in fp32, rounded once; what the rows of
     zeros are given counts for nothing.
@@ -153,7 +154,8 @@ def grouped_block_scaled_mm(x: torch.Tensor, x_scale: torch.Tensor, offsets: tor
 
     x ``[R, K]`` float8_e4m3fn, x_scale ``[R, K/128]`` and offsets ``[E + 1]`` int32 as :func:`sort_tokens` returns them (ascending, from 0
     on; rows behind the last become 0; with other offsets rows may be wrong or not written, and nothing beside them is touched);
-    w ``[E, N, K]`` float8_e4m3fn in checkpoint order, w_scale ``[E, ceil(N/128), K/128]``.  N is of any size, K a multiple of 128 up to 65536, E at most 4096.  Bit for bit the same from run to run.
+    w ``[E, N, K]`` float8_e4m3fn in checkpoint order, w_scale ``[E, ceil(N/128), K/128]``. N is of any size, K a multiple of
+    128 up to 65536, E at most 4096. Bit for bit the same from run to run.
     """
     return _grouped_block_scaled_mm(x, x_scale, offsets, w, w_scale)
 
